@@ -45,6 +45,9 @@ LIBRARIES = {
     "moe": (["moe.cu"], [], []),
     "gla": (["gla.cu"], [], []),
     "streams": (["streams.cu"], [], []),
+    "quantize": (["quantize.cu"], [], []),
+    "gemm_int8": (["gemm_int8.cu"], [], []),
+    "attention_int8": (["attention_int8.cu"], [], []),
 }
 HEADERS = ["common.cuh", "attn_decode_noalloc.h"]
 

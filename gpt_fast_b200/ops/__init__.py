@@ -15,7 +15,7 @@ from typing import Optional
 
 import torch
 
-from .types import BatchMeta, PagedKV
+from .types import BatchMeta, Int8KV, Int8Rows, PagedKV
 
 STATUS_WORDS = 4
 _STATUS_TEXT = {
@@ -129,7 +129,10 @@ def rmsnorm(x, weight, eps: float, out, rows=None, pending=None):
     """out[r] = x[rows[r] or r] * rsqrt(mean(x^2) + eps) * weight.  x float32
     [T, D]; weight [D] (bfloat16 or float32); out [R, D]; rows int32 [R] or None.
     pending (float32 [S, T, D], only without rows): partial sums still owed to x;
-    the kernel first completes x += sum_s pending[s] (written back), then norms."""
+    the kernel first completes x += sum_s pending[s] (written back), then norms.
+    out an `Int8Rows` [R, D]: the norm's 32-bit rows are quantised in the same pass (`quantize_rows`), without a rounding between."""
+    if isinstance(out, Int8Rows):
+        return kernels().rmsnorm_int8(x, weight, eps, out, rows, pending)
     return kernels().rmsnorm(x, weight, eps, out, rows, pending)
 
 
@@ -432,8 +435,29 @@ def linear(a, w, out, mode: str = "store", defer: bool = False):
     may return the partial sums (float32 [S, M, N]) INSTEAD of finishing `out`;
     the caller hands them to the kernel that consumes the result (`rmsnorm`'s
     `pending`, `rope_append`'s `partials`, or `add_partials`).  Returns None when
-    `out` is complete."""
+    `out` is complete.
+
+    w an `Int8Rows` [N, K]: a product of 8-bit integers with a scale per row of each side.  a is quantised per row on the way, or comes as an
+    `Int8Rows` [M, K]; the sum over K (at most 133,144) is an exact 32-bit integer, scaled and passed through the mode's function in 32 bits;
+    out is bfloat16 or float32 and always complete."""
+    if isinstance(w, Int8Rows):
+        return kernels().linear_int8(a, w, out, mode)
     return kernels().linear(a, w, out, mode, defer)
+
+
+def int8_rows(n_rows: int, cols: int, device) -> Int8Rows:
+    """Room for `n_rows` quantised rows of `cols` numbers, not yet written."""
+    return Int8Rows(torch.empty((n_rows, -(-cols // 16) * 16), dtype=torch.int8, device=device),
+                    torch.empty(n_rows, dtype=torch.float32, device=device), cols)
+
+
+def quantize_rows(x, out: Optional[Int8Rows] = None) -> Int8Rows:
+    """Rows of x [R, K] (bfloat16 or float32) as 8-bit integers with a scale each: scale = max |x| / 127, integers nearest to
+    127 x / max |x| (ties to even).  A row of zeros has scale 0; a row that holds a NaN or an infinity has scale NaN."""
+    if out is None:
+        out = int8_rows(x.shape[0], x.shape[1], x.device)
+    kernels().quantize_rows(x, out)
+    return out
 
 
 def add_partials(x, pending):
@@ -453,7 +477,12 @@ def rope_append(qkv, q_out, kv: PagedKV, batch: BatchMeta, table, n_head: int, n
     """Rotate the q and k heads of qkv [T, (H+2G)d] by each token's position;
     q goes to q_out [T, H, d]; k and v go to the token's place in the cache
     (unless append is False).  With partials (float32 [S, T, (H+2G)d], the
-    deferred result of `linear`) qkv is their sum and the `qkv` argument is not read."""
+    deferred result of `linear`) qkv is their sum and the `qkv` argument is not read.
+    kv an `Int8KV`: every key and value row is quantised on its way (as `quantize_rows` does, from the rotated 32-bit numbers); qkv is complete."""
+    if isinstance(kv, Int8KV):
+        if partials is not None:
+            raise KernelError("a cache of 8-bit integers takes complete rows, not the partial sums of a product")
+        return kernels().rope_append_int8(qkv, q_out, kv, batch, table, n_head, n_kv, head_dim, pairing, append)
     return kernels().rope_append(qkv, q_out, kv, batch, table, n_head, n_kv, head_dim, pairing, append, partials)
 
 
@@ -472,7 +501,14 @@ def attention(q, kv: PagedKV, batch: BatchMeta, out, n_head: int, n_kv: int, hea
     keep_first positions stay visible beyond the window.  maps = 2 with diff = (lambda, eps, out_scale): q is [T, H * 2, d],
     a cached key row holds two keys; each (query, key) pair is a softmax of its own over the same values, and the head's
     output is (o_1 - lambda o_2) / sqrt(mean((o_1 - lambda o_2)^2) + eps) * out_scale.  q may come spread out
-    ([T, H * 2, 2 d], see `spread_queries`)."""
+    ([T, H * 2, 2 d], see `spread_queries`).
+    kv an `Int8KV`: keys and values are integers times their row's scale; causal attention, with or without a window, is all it has."""
+    if isinstance(kv, Int8KV):
+        if (chunk is not None or sink is not None or v_head_dim not in (None, head_dim) or values_in_keys or bias is not None
+                or slopes is not None or softcap or keep_first or maps != 1 or diff is not None):
+            raise KernelError("attention over a cache of 8-bit integers is causal, with or without a window; it has no block mask, sink, "
+                              "distance bias, soft cap, kept positions, second map or value size of its own")
+        return kernels().attention_int8(q, kv, batch, out, n_head, n_kv, head_dim, scale, window)
     if softcap or keep_first or maps != 1:
         return kernels().attention(q, kv, batch, out, n_head, n_kv, head_dim, scale, window, chunk, sink, v_head_dim or head_dim,
                                    values_in_keys=values_in_keys, bias=bias, slopes=slopes, softcap=softcap, keep_first=keep_first,
@@ -494,12 +530,24 @@ def rope_append_attention(qkv, partials, kv: PagedKV, batch: BatchMeta, table, o
     Where a kernel does both in one launch (a decode step in bfloat16) that kernel runs; q then never goes
     through memory."""
     k = kernels()
+    if isinstance(kv, Int8KV):
+        q = torch.empty(batch.n_tokens, n_head, head_dim, dtype=out.dtype, device=out.device)
+        rope_append(qkv, q, kv, batch, table, n_head, n_kv, head_dim, pairing, append, partials)
+        return k.attention_int8(q, kv, batch, out, n_head, n_kv, head_dim, scale, window)
     fused = getattr(k, "rope_append_attention", None)
     if fused is not None and fused(qkv, partials, kv, batch, table, out, n_head, n_kv, head_dim, pairing, append, scale, window):
         return
     q = torch.empty(batch.n_tokens, n_head, head_dim, dtype=out.dtype, device=out.device)
     k.rope_append(qkv, q, kv, batch, table, n_head, n_kv, head_dim, pairing, append, partials)
     k.attention(q, kv, batch, out, n_head, n_kv, head_dim, scale, window)
+
+
+def read_cache(kv: Int8KV, batch: BatchMeta, k_out, v_out):
+    """What the cache of 8-bit integers holds at the places of the step's tokens, as numbers: k_out, v_out [T, G, d] (bfloat16 or float32).  A batch whose
+    lengths are 0 reads sequences from their first position on."""
+    if not isinstance(kv, Int8KV):
+        raise KernelError("read_cache reads a cache of 8-bit integers")
+    return kernels().read_cache_int8(kv, batch, k_out, v_out)
 
 
 def advance_lengths(batch: BatchMeta):

@@ -6,7 +6,7 @@ from typing import Optional
 import torch
 
 from ..csrc import build
-from .types import BatchMeta, PagedKV
+from .types import BatchMeta, Int8KV, Int8Rows, PagedKV
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 _EPI = {"store": 0, "add": 1, "swiglu": 2, "gelu": 4, "gelu_tanh": 5, "silu": 6, "relu2": 7}
@@ -1287,6 +1287,124 @@ class CudaKernels:
         return True
 
     # -- sampling --------------------------------------------------------------------------
+    # -- 8-bit integers: rows with a scale each, their products, a cache of them -----------------------------
+    @staticmethod
+    def _need_here(*tensors):
+        """The kernels run on the current device's current stream; their tensors have to be there."""
+        here = _device()
+        for t in tensors:
+            if t.device.index != here:
+                _fail(f"a tensor is on {t.device}, the current device is cuda:{here}")
+
+    @staticmethod
+    def _need_rows(r: Int8Rows, shape, name):
+        if r.shape != shape:
+            _fail(f"{name} must be {tuple(shape)} in 8-bit rows, got {tuple(r.shape)}")
+        _need(r.q, torch.int8, name=name)
+        if r.q.dim() != 2 or r.q.shape[1] < r.cols or r.q.shape[1] % 16:
+            _fail(f"{name}: rows of {r.cols} numbers need a pitch that is a multiple of 16, got {tuple(r.q.shape)}")
+        _need(r.scale, torch.float32, (shape[0],), f"scales of {name}")
+
+    def quantize_rows(self, x, out):
+        if x.dim() != 2:
+            _fail(f"rows to quantise are [R, K], got {tuple(x.shape)}")
+        _need(x, name="rows")
+        self._need_rows(out, x.shape, "quantised rows")
+        self._need_here(x, out.q)
+        self._call("quantize", "gfb_quantize_rows", _ptr(x), _dt(x), _ptr(out.q), _ptr(out.scale), x.shape[0], x.shape[1], out.q.shape[1], _stream())
+
+    def rmsnorm_int8(self, x, weight, eps, out, rows=None, pending=None):
+        T, D = x.shape
+        R = out.q.shape[0]
+        _need(x, torch.float32, name="norm input")
+        _need(weight, shape=(D,), name="norm weight")
+        self._need_rows(out, (R, D), "norm output")
+        self._need_here(x, out.q, weight)
+        if rows is not None:
+            _need(rows, torch.int32, (R,), "rows")
+            if pending is not None:
+                self.add_partials(x, pending)
+                pending = None
+        elif T != R:
+            _fail(f"norm output has {R} rows, input {T}")
+        S = 0
+        if pending is not None:
+            S = pending.shape[0]
+            _need(pending, torch.float32, (S, T, D), "pending partial sums")
+        self._call("quantize", "gfb_rmsnorm_quantize", _ptr(x), _ptr(pending), S, T * D, _ptr(weight), _dt(weight), _ptr(out.q), _ptr(out.scale),
+                   _ptr(rows), R, D, out.q.shape[1], eps, _stream())
+
+    MAX_INT8_K = 133144                    # 127^2 times this is the largest sum that 32 bits hold for sure
+
+    def linear_int8(self, a, w, out, mode="store"):
+        M, K = a.shape
+        N = w.q.shape[0]
+        if mode not in _EPI:
+            _fail(f"unknown mode '{mode}'")
+        if K > self.MAX_INT8_K:
+            _fail(f"rows of {K} 8-bit numbers: from {self.MAX_INT8_K + 1} on a sum may leave 32 bits")
+        self._need_rows(w, (N, K), "weight")
+        if mode == "swiglu" and N % 2:
+            _fail(f"SwiGLU needs pairs of gate and up rows, got {N} rows")
+        _need(out, shape=(M, N // 2 if mode == "swiglu" else N), name="product output")
+        if mode == "add" and out.dtype != torch.float32:
+            _fail("the residual sum is kept in float32")
+        self._need_here(w.q, out)
+        if not isinstance(a, Int8Rows):
+            _need(a, name="activation")
+            from . import int8_rows
+            rows = int8_rows(M, K, a.device)
+            self.quantize_rows(a, rows)
+            a = rows
+        else:
+            self._need_rows(a, (M, K), "activation")
+            self._need_here(a.q)
+        self._label = f"linear int8 {N}x{K} {mode}"
+        self._call("gemm_int8", "gfb_gemm_int8", _ptr(a.q), _ptr(a.scale), a.q.shape[1], _ptr(w.q), _ptr(w.scale), w.q.shape[1], _ptr(out), _dt(out),
+                   M, N, K, _EPI[mode], _ptr(self.status), _stream())
+
+    def _int8_kv_args(self, kv: Int8KV, n_kv, head_dim):
+        P = kv.k_pool.shape[0]
+        for pool, scale, name in ((kv.k_pool, kv.k_scale, "key"), (kv.v_pool, kv.v_scale, "value")):
+            _need(pool, torch.int8, (P, n_kv, kv.page_size, head_dim), f"{name} pool")
+            if scale is None:
+                _fail(f"a pool of 8-bit {name}s needs its scales")
+            _need(scale, torch.float32, (P, n_kv, kv.page_size), f"scales of the {name} pool")
+        _need(kv.page_table, torch.int32, name="page table")
+        return (_ptr(kv.k_pool), _ptr(kv.v_pool), _ptr(kv.k_scale), _ptr(kv.v_scale), _ptr(kv.page_table), kv.page_table.shape[1], kv.page_size, P)
+
+    def rope_append_int8(self, qkv, q_out, kv, batch, table, n_head, n_kv, head_dim, pairing, append):
+        T = batch.n_tokens
+        _need(qkv, shape=(T, (n_head + 2 * n_kv) * head_dim), name="qkv")
+        _need(q_out, qkv.dtype, (T, n_head, head_dim), "q_out")
+        _need(table, torch.float32, (table.shape[0], head_dim // 2, 2), "rotary table")
+        if pairing not in _PAIRING:
+            _fail(f"unknown rotary pairing '{pairing}'")
+        self._need_here(qkv, q_out, kv.k_pool, table)
+        self._call("quantize", "gfb_rope_append_int8", _ptr(qkv), _ptr(q_out), _dt(qkv), *self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch),
+                   _ptr(table), table.shape[0], n_head, n_kv, head_dim, _PAIRING[pairing], 1 if append else 0, _ptr(batch.status), _stream())
+
+    def read_cache_int8(self, kv, batch, k_out, v_out):
+        T = batch.n_tokens
+        n_kv, head_dim = kv.k_pool.shape[1], kv.k_pool.shape[3]
+        _need(k_out, shape=(T, n_kv, head_dim), name="keys")
+        _need(v_out, k_out.dtype, (T, n_kv, head_dim), "values")
+        self._need_here(kv.k_pool, k_out, v_out)
+        self._call("quantize", "gfb_read_cache_int8", *self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch), _ptr(k_out), _ptr(v_out),
+                   _dt(k_out), n_kv, head_dim, _ptr(batch.status), _stream())
+
+    def attention_int8(self, q, kv, batch, out, n_head, n_kv, head_dim, scale, window=None):
+        T = batch.n_tokens
+        if n_kv < 1 or n_head % n_kv:
+            _fail(f"{n_head} query heads do not divide into {n_kv} key/value heads")
+        if window is not None and window < 1:
+            _fail(f"a window of {window} positions")
+        _need(q, shape=(T, n_head, head_dim), name="q")
+        _need(out, q.dtype, (T, n_head * head_dim), "attention output")
+        self._need_here(q, out, kv.k_pool)
+        self._call("attention_int8", "gfb_attention_int8_generic", _ptr(q), _ptr(out), _dt(q), *self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch),
+                   n_head, n_kv, head_dim, scale, window or 0, _ptr(batch.status), _stream())
+
     def argmax(self, logits, out):
         B, V = logits.shape
         _need(logits, torch.float32, name="logits")

@@ -35,3 +35,32 @@ class PagedKV:
     page_table: torch.Tensor      # int32 [n_slots, max_pages]
     page_size: int
     workspace: Optional[object] = None   # scratch of the split-KV decode kernel
+
+
+@dataclass
+class Int8KV(PagedKV):
+    """The same in 8-bit integers: pools of int8 and, per cached row (page, key head, place), a 32-bit scale; a number is its integer times
+    the row's scale.  k_scale, v_scale: float32 [n_pages, n_kv, page_size]."""
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+
+@dataclass
+class Int8Rows:
+    """Rows of 8-bit integers with a 32-bit scale each: number (r, c) is q[r, c] * scale[r], c < cols.  q's pitch is a multiple of 16 and
+    its columns from `cols` on are zeros.  What `quantize_rows` makes: weights (a row per output) and activations (a row per token)."""
+    q: torch.Tensor               # int8 [R, pitch]
+    scale: torch.Tensor           # float32 [R]
+    cols: int
+
+    @property
+    def shape(self):
+        return torch.Size((self.q.shape[0], self.cols))
+
+    @property
+    def dtype(self):
+        return torch.int8
+
+    @property
+    def device(self):
+        return self.q.device
