@@ -50,9 +50,9 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* scratch
 // q [R, pitch] and scale [R] of x [R, K]; the columns from K to the pitch are zeros.  One block per row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int K, int pitch) {
+quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int K, int pitch, int early) {
     __shared__ uint32_t scratch[32];
-    gfb_pdl_launch();
+    if (early) gfb_pdl_launch();
     gfb_pdl_wait();
     const T* row = x + (size_t)blockIdx.x * K;
     uint32_t m = 0;
@@ -184,12 +184,14 @@ read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* __restrict__ k_out, TO* __rest
 
 }  // namespace
 
-GFB_API int gfb_quantize_rows(const void* x, int dt, void* q, float* scale, int R, int K, int pitch, cudaStream_t stream) {
+// early: the next kernel may start while this one runs and waits for it before it reads the rows.  A product asks for its weights ahead of that wait, so rows
+// that may become weights are made with early = 0: nothing starts before they are complete.
+GFB_API int gfb_quantize_rows(const void* x, int dt, void* q, float* scale, int R, int K, int pitch, int early, cudaStream_t stream) {
     if (R <= 0) return 0;
     if (K <= 0 || pitch < K) return gfb_fail("gfb_quantize_rows: rows of %d numbers with a pitch of %d", K, pitch);
     cudaError_t e;
-    if (dt == GFB_BF16) e = gfb_launch(quantize_rows_kernel<__nv_bfloat16>, dim3(R), dim3(256), 0, stream, (const __nv_bfloat16*)x, (int8_t*)q, scale, K, pitch);
-    else if (dt == GFB_F32) e = gfb_launch(quantize_rows_kernel<float>, dim3(R), dim3(256), 0, stream, (const float*)x, (int8_t*)q, scale, K, pitch);
+    if (dt == GFB_BF16) e = gfb_launch(quantize_rows_kernel<__nv_bfloat16>, dim3(R), dim3(256), 0, stream, (const __nv_bfloat16*)x, (int8_t*)q, scale, K, pitch, early);
+    else if (dt == GFB_F32) e = gfb_launch(quantize_rows_kernel<float>, dim3(R), dim3(256), 0, stream, (const float*)x, (int8_t*)q, scale, K, pitch, early);
     else return gfb_fail("gfb_quantize_rows: unknown type %d", dt);
     return gfb_check(e, "gfb_quantize_rows");
 }

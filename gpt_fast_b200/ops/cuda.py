@@ -148,6 +148,19 @@ def split_parts(K: int, splits: int) -> int:
     return -(-stages // -(-stages // min(splits, stages)))
 
 
+def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
+    """(bn, splits, stages) of a product of 8-bit integers.  Few tokens: 128 weight rows x bn tokens per block, K split over a cluster of up to 8
+    blocks until about two blocks per SM stream weights; many tokens: 256 x 256 tiles on pairs of SMs (bn 256).  Between 129 and 512 tokens the
+    first form, with several tiles of 128 tokens, while the second would leave most pairs without a tile; and for matrices of fewer than 256 rows."""
+    tiles = -(-M // 256) * -(-N // 256)
+    if M > 128 and N >= 256 and (M > 512 or mode == "swiglu" or tiles >= sm_count // 2):
+        return 256, 1, 6
+    bn = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
+    blocks = -(-N // 128) * -(-M // bn)
+    splits = max(1, min(8, -(-K // 128) // 4, 2 * sm_count // max(1, blocks)))
+    return bn, splits, max(2, min(8, 102400 // (16384 + bn * 128)))
+
+
 def rows_share_keys(rows: int, longest: int, max_kv_len: int, line: int, blocks: Optional[int] = None) -> bool:
     """Whether the rows (token, head) of a step's 32-bit attention share the keys and values of sixteen rows per block; the bits are the same.  `blocks`: of
     sixteen rows of one sequence and key head at most (default: all full).  A block has sixteen rows' work in a row and stages every key of its sequence, so
@@ -1305,13 +1318,14 @@ class CudaKernels:
             _fail(f"{name}: rows of {r.cols} numbers need a pitch that is a multiple of 16, got {tuple(r.q.shape)}")
         _need(r.scale, torch.float32, (shape[0],), f"scales of {name}")
 
-    def quantize_rows(self, x, out):
+    def quantize_rows(self, x, out, weights=True):
+        """weights=False: rows that no product takes as its weights, so that the kernel behind may start early."""
         if x.dim() != 2:
             _fail(f"rows to quantise are [R, K], got {tuple(x.shape)}")
         _need(x, name="rows")
         self._need_rows(out, x.shape, "quantised rows")
         self._need_here(x, out.q)
-        self._call("quantize", "gfb_quantize_rows", _ptr(x), _dt(x), _ptr(out.q), _ptr(out.scale), x.shape[0], x.shape[1], out.q.shape[1], _stream())
+        self._call("quantize", "gfb_quantize_rows", _ptr(x), _dt(x), _ptr(out.q), _ptr(out.scale), x.shape[0], x.shape[1], out.q.shape[1], 0 if weights else 1, _stream())
 
     def rmsnorm_int8(self, x, weight, eps, out, rows=None, pending=None):
         T, D = x.shape
@@ -1354,14 +1368,20 @@ class CudaKernels:
             _need(a, name="activation")
             from . import int8_rows
             rows = int8_rows(M, K, a.device)
-            self.quantize_rows(a, rows)
+            self.quantize_rows(a, rows, weights=False)
             a = rows
         else:
             self._need_rows(a, (M, K), "activation")
             self._need_here(a.q)
+        key = (M, N, K, mode, "int8")
+        plan = self._plans.get(key)
+        if plan is None:
+            if len(self._plans) > 4096:
+                self._plans.clear()
+            plan = self._plans[key] = int8_plan(M, N, K, mode, self.sm_count)
         self._label = f"linear int8 {N}x{K} {mode}"
         self._call("gemm_int8", "gfb_gemm_int8", _ptr(a.q), _ptr(a.scale), a.q.shape[1], _ptr(w.q), _ptr(w.scale), w.q.shape[1], _ptr(out), _dt(out),
-                   M, N, K, _EPI[mode], _ptr(self.status), _stream())
+                   M, N, K, _EPI[mode], *plan, _ptr(self.status), _stream())
 
     def _int8_kv_args(self, kv: Int8KV, n_kv, head_dim):
         P = kv.k_pool.shape[0]
