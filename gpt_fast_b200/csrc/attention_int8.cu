@@ -3,6 +3,8 @@
 // For a query q at position p, over the keys j it sees (j <= p, and p - j < window when there is one):
 //     s_j = scale ks_j (q . K_j),   w_j = exp(s_j - max s),   out = sum_j (w_j vs_j) V_j / sum_j w_j
 // with integers K_j, V_j and their scales ks_j, vs_j.  The scales stay out of the products: a key's joins its score, a value's its weight.
+#include <cuda.h>
+
 #include "common.cuh"
 
 GFB_DEFINE_LAST_ERROR()
@@ -86,7 +88,453 @@ attention_int8_generic_kernel(const T* __restrict__ q, T* __restrict__ out, Int8
     }
 }
 
+// ---- single tokens on the tensor cores: head sizes 64 and 128, pages of 64, at most 8 heads per key head -------------------------------
+// A block owns (token, key head, slice of the sequence's pages) and serves all query heads of the group from one pass over the integers, which are what it
+// is bound by.  A producer thread brings pages by TMA, NS of them in flight; each of four warps takes 16 of a page's 64 keys and runs an online
+// softmax of its own over them, without a block-wide step until the end.
+//
+// Both products are mma.sync m16n8k16 with the cached integers as the A operand and the heads as its 8 columns: S^T = K q^T (16 keys x 8 heads) and
+// O^T += V^T (w vs)^T (16 dims x 8 heads per chunk of 16 dims).  An 8-bit integer is exact in bfloat16; two become two bfloat16 numbers in three
+// operations (`pair`).  They are taken as bytes 0, 2 and bytes 1, 3 of a word, so no byte is moved: the order of the dims within a product over 16 of them
+// is free as long as q has it too, and of V's transposed words the two halves are the rows of dims 2g and 2g + 1.
+// Weights times their value's scale are rounded to bfloat16 for the second product (half a step, 2^-8, of a weight, as the 16-bit cache's attention does); the sum
+// of weights is of the unrounded ones.  The reference of the exponentials follows the maximum in steps of at least 2^8, so a rescale is rare.
+constexpr int DEC_WARPS = 4, DEC_THREADS = 32 * (DEC_WARPS + 1);
+constexpr int PAGE = 64;
+constexpr int MERGE_SLICES = 8;              // the largest portable cluster
+constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;   // a page that has not come after a second is given up
+constexpr float LAG = 8.f;                   // log2 by which a score may pass the reference
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ unsigned long long global_ns() {
+    unsigned long long v;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(v));
+    return v;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+// Wait for the phase with `parity` to complete; false when the block gives up or time runs out.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int which) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    for (;;) {
+        for (int i = 0; i < 128; i++)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*gave_up) return false;
+        if (global_ns() - t0 > WAIT_LIMIT_NS) {
+            *gave_up = 1;
+            gfb_report(status, GFB_ERR_WAIT_TIMEOUT, which, (int)(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z)));
+            return false;
+        }
+    }
+}
+// The same for a whole warp: one answer for all its lanes, which meet again at the aligned instructions behind it.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int which) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up, status, which));
+}
+__device__ __forceinline__ uint64_t l2_evict_first_policy() {
+    uint64_t pol;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
+    return pol;
+}
+__device__ __forceinline__ void tma_load_2d_hint(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "l"(pol) : "memory");
+}
+// `bytes` (a multiple of 16) from a 16-byte boundary of global memory to one of shared memory
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {        // an 8 x 8 matrix of 16-bit numbers over the warp
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Bytes 0 and 2 of x, signed, as two bfloat16 numbers: with s the sign bit and l the seven bits below it a byte is l - 128 s, 0x4300 | l is 128 + l, and
+// 0xC300 | 128 s is -128 - 128 s.
+__device__ __forceinline__ uint32_t pair(uint32_t x) {
+    const uint32_t a = (x & 0x007f007fu) | 0x43004300u, b = (x & 0x00800080u) | 0xC300C300u;
+    uint32_t y;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+// Byte offset of the 16-byte chunk at column `col` (a multiple of 16) of row `row` in a tile of rows of D bytes that came as lines of 128 bytes with 128-byte swizzle.
+template <int D>
+__device__ __forceinline__ uint32_t swz(int row, int col) {
+    const int f = row * D + col, line = f >> 7;
+    return (uint32_t)(line * 128 + ((((f >> 4) & 7) ^ (line & 7)) << 4));
+}
+
+template <int D, int NS>
+struct DecodeSmem {
+    static constexpr int TILE = PAGE * D, STAGE = 2 * TILE;            // K and V of a page
+    static constexpr int OP = D + 8;                                   // floats per row of the merge area, which lies where the pages were
+    static constexpr int SCALES = NS * STAGE, BARS = SCALES + NS * 2 * PAGE * 4;
+    static constexpr int BYTES = 1024 + BARS + 2 * NS * 8 + NS * 4 + 16;
+    static_assert(4 * 8 * OP * 4 + 64 * 4 + 8 * D * 4 + 16 * 4 <= NS * STAGE, "the merge area fits where the pages were");
+};
+
+// q [T, H, D], out [T, H * D]; with more than one slice the blocks of a (token, key head) are a cluster (merge) or leave their sums in scratch_o
+// [T, H, splits, D] and (reference, sum) in scratch_ml [T, H, splits, 2].
+template <int D, int NS>
+__global__ void __launch_bounds__(DEC_THREADS, 4)
+attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* __restrict__ q,
+                             __nv_bfloat16* __restrict__ out, float* __restrict__ scratch_o, float* __restrict__ scratch_ml, Int8KV kv, GfbBatch b, int H, int G,
+                             float scale_log2e, int window, int splits, int merge, int* status) {
+    using S = DecodeSmem<D, NS>;
+    constexpr int CH = D / 16;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;      // swizzled tiles start on 1024-byte boundaries
+    uint8_t* smem = smem_raw + (tiles - smem_u32(smem_raw));
+    const float* scales = reinterpret_cast<const float*>(smem + S::SCALES);      // per stage 64 of the keys, 64 of the values
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS);                // per stage: full, empty
+    int* dead = reinterpret_cast<int*>(bars + 2 * NS);                           // per stage: its page does not exist
+    int* gave_up = dead + NS;
+    const uint32_t bar0 = smem_u32(bars);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
+    const int t = blockIdx.x, g = blockIdx.y, z = blockIdx.z, rep = H / G;
+    if (threadIdx.x == 0) {
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
+        for (int i = 0; i < NS; i++) { mbar_init(bar0 + 16 * i, 1); mbar_init(bar0 + 16 * i + 8, DEC_WARPS); }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    gfb_pdl_launch();
+    const int s = b.tok_seq[t], slot = b.slots[s], q_off = t - b.cu_seqlens[s];
+    gfb_pdl_wait();
+    const int pos = b.lengths[slot] + q_off, lo = window > 0 ? max(0, pos - window + 1) : 0;
+    const int first = lo / PAGE, n_pages = pos / PAGE - first + 1, per = (n_pages + splits - 1) / splits;
+    const int p0 = first + z * per, n = max(0, min(per, n_pages - z * per));
+
+    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};           // of heads 2 t4, 2 t4 + 1
+#pragma unroll
+    for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    if (warp == DEC_WARPS) {
+        if (lane == 0) {
+            const int* pt = kv.page_table + (size_t)slot * kv.max_pages;
+            const uint64_t pol = l2_evict_first_policy();
+            int next = n > 0 && p0 < kv.max_pages ? pt[p0] : -1;
+            for (int i = 0; i < n; i++) {
+                const int st = i % NS, page = next;
+                next = i + 1 < n && p0 + i + 1 < kv.max_pages ? pt[p0 + i + 1] : -1;
+                if (i >= NS && !mbar_wait(bar0 + 16 * st + 8, ((i / NS) & 1) ^ 1, gave_up, status, 301)) break;
+                const uint32_t full = bar0 + 16 * st;
+                if (page < 0 || page >= kv.n_pages) {
+                    gfb_report(status, GFB_ERR_PAGE_TABLE, slot, p0 + i);
+                    dead[st] = 1;
+                    mbar_arrive(full);
+                    continue;
+                }
+                dead[st] = 0;
+                const size_t row = ((size_t)page * G + g) * PAGE;               // the page's first row in the pools
+                const int line = (int)(row * D / 128);
+                mbar_expect_tx(full, S::STAGE + 2 * PAGE * 4);
+                tma_load_2d_hint(tiles + st * S::STAGE, &map_k, 0, line, full, pol);
+                bulk_load(tiles + S::SCALES + st * 2 * PAGE * 4, kv.k_scale + row, PAGE * 4, full);
+                tma_load_2d_hint(tiles + st * S::STAGE + S::TILE, &map_v, 0, line, full, pol);
+                bulk_load(tiles + S::SCALES + st * 2 * PAGE * 4 + PAGE * 4, kv.v_scale + row, PAGE * 4, full);
+            }
+        }
+    } else {
+        // q as the B operand: column g4 is a head, its k numbers are the dims 4 t4 and + 2, and 4 t4 + 1 and + 3, of every 16
+        uint32_t qb[CH][2];
+        const __nv_bfloat16* qr = q + ((size_t)t * H + g * rep + min(g4, rep - 1)) * D;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const uint2 v = g4 < rep ? *reinterpret_cast<const uint2*>(qr + c * 16 + 4 * t4) : make_uint2(0u, 0u);
+            qb[c][0] = __byte_perm(v.x, v.y, 0x5410);
+            qb[c][1] = __byte_perm(v.x, v.y, 0x7632);
+        }
+        // this lane's row of the four matrices that one ldmatrix takes: keys 0-7 and 8-15 of the warp's, chunks c and c + 1
+        const int lrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), lcol = (lane >> 4) * 16;
+        for (int i = 0; i < n; i++) {
+            const int st = i % NS;
+            if (!mbar_wait_warp(bar0 + 16 * st, (i / NS) & 1, gave_up, status, 300)) break;
+            const uint32_t kt = tiles + st * S::STAGE, vt = kt + S::TILE;
+            float sc[4] = {0.f, 0.f, 0.f, 0.f};                                 // (key g4, heads 2 t4 and + 1), (key g4 + 8, the same)
+#pragma unroll
+            for (int c = 0; c < CH; c += 2) {
+                uint32_t r[4];
+                ldsm_x4(kt + swz<D>(lrow, c * 16 + lcol), r);
+                mma_bf16(sc, pair(r[0]), pair(r[1]), pair(r[0] >> 8), pair(r[1] >> 8), qb[c][0], qb[c][1]);
+                mma_bf16(sc, pair(r[2]), pair(r[3]), pair(r[2] >> 8), pair(r[3] >> 8), qb[c + 1][0], qb[c + 1][1]);
+            }
+            const float* ks = scales + st * 2 * PAGE + warp * 16 + g4;
+            const float k0 = ks[0] * scale_log2e, k1 = ks[8] * scale_log2e, v0 = ks[PAGE], v1 = ks[PAGE + 8];
+            sc[0] *= k0; sc[1] *= k0; sc[2] *= k1; sc[3] *= k1;
+            const int j = (p0 + i) * PAGE + warp * 16 + g4;
+            const bool all = !dead[st] && (p0 + i) * PAGE >= lo && (p0 + i) * PAGE + PAGE - 1 <= pos;       // uniform: every key of the page is seen
+            bool see0 = true, see1 = true;
+            if (!all) {
+                see0 = !dead[st] && j >= lo && j <= pos;
+                see1 = !dead[st] && j + 8 >= lo && j + 8 <= pos;
+                if (!see0) sc[0] = sc[1] = -INFINITY;
+                if (!see1) sc[2] = sc[3] = -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, fmaxf(sc[0], sc[2]) > m[0] + LAG || fmaxf(sc[1], sc[3]) > m[1] + LAG)) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float x = fmaxf(sc[e], sc[e + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    const float now = fmaxf(m[e], x), corr = m[e] == -INFINITY ? 0.f : exp2f(m[e] - now);
+                    m[e] = now;
+                    l[e] *= corr;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) { o[c][e] *= corr; o[c][e + 2] *= corr; }
+                }
+            }
+            const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
+            const float p00 = exp2f(sc[0] - r0), p01 = exp2f(sc[1] - r1), p10 = exp2f(sc[2] - r0), p11 = exp2f(sc[3] - r1);
+            l[0] += p00 + p10;
+            l[1] += p01 + p11;
+            // an unseen key's value scale can be anything
+            uint32_t wa = pack2(p00 * v0, p01 * v0), wb = pack2(p10 * v1, p11 * v1);
+            if (!see0) wa = 0u;
+            if (!see1) wb = 0u;
+            wa = transposed(wa);
+            wb = transposed(wb);
+#pragma unroll
+            for (int c = 0; c < CH; c += 2) {
+                uint32_t r[4];
+                ldsm_x4_trans(vt + swz<D>(lrow, c * 16 + lcol), r);
+                mma_bf16(o[c], pair(r[0]), pair(r[0] >> 8), pair(r[1]), pair(r[1] >> 8), wa, wb);
+                mma_bf16(o[c + 1], pair(r[2]), pair(r[2] >> 8), pair(r[3]), pair(r[3] >> 8), wa, wb);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
+        }
+    }
+    __syncthreads();                                               // every page has been read, or the block gave up
+    if (*gave_up) {
+        // copies that were issued may still be landing in this block's shared memory
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 50000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+
+    // Merge of the four warps: they exchange (reference, sum), each brings its sums to the common reference (and, with one slice, divides them).
+    float* Ow = reinterpret_cast<float*>(smem);                    // [4][8][OP]
+    float* mw = Ow + 4 * 8 * S::OP;                                // [4][8]
+    float* lw = mw + 32;                                           // [4][8]
+    float* mine = lw + 32;                                         // [8][D]
+    float* ml = mine + 8 * D;                                      // [8][2]
+    if (warp < DEC_WARPS) {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+        if (g4 == 0) {
+            mw[warp * 8 + 2 * t4] = m[0]; mw[warp * 8 + 2 * t4 + 1] = m[1];
+            lw[warp * 8 + 2 * t4] = l[0]; lw[warp * 8 + 2 * t4 + 1] = l[1];
+        }
+    }
+    __syncthreads();
+    if (warp < DEC_WARPS) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int h = 2 * t4 + e;
+            const float top = fmaxf(fmaxf(mw[h], mw[8 + h]), fmaxf(mw[16 + h], mw[24 + h]));
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                if (mw[w * 8 + h] != -INFINITY) sum += lw[w * 8 + h] * exp2f(mw[w * 8 + h] - top);
+            float f = m[e] == -INFINITY ? 0.f : exp2f(m[e] - top);
+            if (splits == 1) f = sum == 0.f ? 0.f : f / sum;
+            float* row = Ow + (warp * 8 + h) * S::OP + 2 * g4;
+#pragma unroll
+            for (int c = 0; c < CH; c++) *reinterpret_cast<float2*>(row + c * 16) = make_float2(o[c][e] * f, o[c][e + 2] * f);
+            if (warp == 0 && g4 == 0) { ml[2 * h] = top; ml[2 * h + 1] = sum; }
+        }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < rep * (D / 2); idx += DEC_THREADS) {
+        const int h = idx / (D / 2), dim = 2 * (idx - h * (D / 2)), head = g * rep + h;
+        float2 acc = *reinterpret_cast<const float2*>(Ow + h * S::OP + dim);
+#pragma unroll
+        for (int w = 1; w < 4; w++) {
+            const float2 a = *reinterpret_cast<const float2*>(Ow + (w * 8 + h) * S::OP + dim);
+            acc.x += a.x;
+            acc.y += a.y;
+        }
+        if (splits == 1) *reinterpret_cast<uint32_t*>(out + ((size_t)t * H + head) * D + dim) = pack2(acc.x, acc.y);
+        else if (merge) *reinterpret_cast<float2*>(mine + h * D + dim) = acc;
+        else *reinterpret_cast<float2*>(scratch_o + (((size_t)t * H + head) * splits + z) * D + dim) = acc;
+    }
+    if (splits == 1) return;
+    if (!merge) {
+        if ((int)threadIdx.x < rep) {
+            float* at = scratch_ml + (((size_t)t * H + g * rep + threadIdx.x) * splits + z) * 2;
+            at[0] = ml[2 * threadIdx.x];
+            at[1] = ml[2 * threadIdx.x + 1];
+        }
+        return;
+    }
+    // the slices are a cluster: each finishes its part of the numbers over all of them, in ascending order
+    gfb_cluster_sync();
+    for (int idx = z * DEC_THREADS + threadIdx.x; idx < rep * (D / 2); idx += splits * DEC_THREADS) {
+        const int h = idx / (D / 2), dim = 2 * (idx - h * (D / 2)), head = g * rep + h;
+        float2 part[MERGE_SLICES], row[MERGE_SLICES];
+#pragma unroll
+        for (int k = 0; k < MERGE_SLICES; k++)
+            if (k < splits) {
+                part[k] = gfb_cluster_load2(ml + 2 * h, k);
+                row[k] = gfb_cluster_load2(mine + h * D + dim, k);
+            }
+        float top = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < MERGE_SLICES; k++)
+            if (k < splits) top = fmaxf(top, part[k].x);
+#pragma unroll
+        for (int k = 0; k < MERGE_SLICES; k++)
+            if (k < splits && part[k].x != -INFINITY) {
+                const float e = exp2f(part[k].x - top);
+                sum = fmaf(part[k].y, e, sum);
+                o0 = fmaf(row[k].x, e, o0);
+                o1 = fmaf(row[k].y, e, o1);
+            }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint32_t*>(out + ((size_t)t * H + head) * D + dim) = pack2(o0 * inv, o1 * inv);
+    }
+    gfb_cluster_sync();                                            // no block leaves while another reads its shared memory
+}
+
+// The slices of a (token, head) through memory, in ascending order.
+__global__ void __launch_bounds__(128)
+attention_int8_combine_kernel(const float* __restrict__ scratch_o, const float* __restrict__ scratch_ml, __nv_bfloat16* __restrict__ out, int H, int d, int splits) {
+    gfb_pdl_launch();
+    gfb_pdl_wait();
+    const size_t row = (size_t)blockIdx.x * H + blockIdx.y;
+    const float* ml = scratch_ml + row * splits * 2;
+    float top = -INFINITY, sum = 0.f;
+    for (int k = 0; k < splits; k++) top = fmaxf(top, ml[2 * k]);
+    for (int k = 0; k < splits; k++)
+        if (ml[2 * k] != -INFINITY) sum = fmaf(ml[2 * k + 1], exp2f(ml[2 * k] - top), sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int dim = threadIdx.x; dim < d; dim += blockDim.x) {
+        float o = 0.f;
+        for (int k = 0; k < splits; k++)
+            if (ml[2 * k] != -INFINITY) o = fmaf(scratch_o[(row * splits + k) * d + dim], exp2f(ml[2 * k] - top), o);
+        out[row * d + dim] = __float2bfloat16_rn(o * inv);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    if (fn == nullptr) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)p;
+    }
+    return fn;
+}
+
+// A pool as lines of 128 bytes; a box is the 64 rows of one head of a page.
+int pool_map(CUtensorMap* map, const void* pool, int n_pages, int G, int d) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return gfb_fail("gfb_attention_int8: the driver does not export cuTensorMapEncodeTiled");
+    cuuint64_t dims[2] = {128, (cuuint64_t)n_pages * G * PAGE * d / 128};
+    cuuint64_t strides[1] = {128};
+    cuuint32_t box[2] = {128, (cuuint32_t)(PAGE * d / 128)};
+    cuuint32_t estr[2] = {1, 1};
+    if (dims[1] > 0x7fffffffull) return gfb_fail("gfb_attention_int8: a pool of %d pages exceeds a tensor map's coordinates", n_pages);
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return gfb_fail("gfb_attention_int8: cuTensorMapEncodeTiled failed with %d (%d pages)", (int)r, n_pages);
+    return 0;
+}
+
+constexpr int MAX_DEVICES = 64;
+
+// Shared memory beyond 48 KB is granted per kernel and device; asked for once for each.
+template <typename F>
+int room(F kern, size_t smem, bool (&configured)[MAX_DEVICES]) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= MAX_DEVICES) return gfb_fail("gfb_attention_int8: device %d", dev);
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return gfb_fail("gfb_attention_int8: %zu bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
+        configured[dev] = true;
+    }
+    return 0;
+}
+
+template <int D, int NS>
+int launch_decode(const void* q, void* out, float* scratch, const Int8KV& kv, const GfbBatch& b, int H, int G, float scale, int window, int splits, int* status,
+                  cudaStream_t stream) {
+    auto kern = attention_int8_decode_kernel<D, NS>;
+    const size_t smem = DecodeSmem<D, NS>::BYTES;
+    static bool configured[MAX_DEVICES] = {};
+    if (room(kern, smem, configured)) return 1;
+    CUtensorMap mk, mv;
+    if (pool_map(&mk, kv.k_pool, kv.n_pages, G, D) || pool_map(&mv, kv.v_pool, kv.n_pages, G, D)) return 1;
+    const int merge = splits > 1 && scratch == nullptr;
+    float* ml = scratch ? scratch + (size_t)b.n_tokens * H * splits * D : nullptr;
+    int rc = gfb_check(gfb_launch_clusters(kern, dim3(b.n_tokens, G, splits), dim3(DEC_THREADS), smem, stream, dim3(1, 1, merge ? splits : 1), mk, mv,
+                                           (const __nv_bfloat16*)q, (__nv_bfloat16*)out, scratch, ml, kv, b, H, G, scale * 1.4426950408889634f, window, splits, merge,
+                                           status), "gfb_attention_int8_decode");
+    if (rc || splits == 1 || merge) return rc;
+    return gfb_check(gfb_launch(attention_int8_combine_kernel, dim3(b.n_tokens, H), dim3(128), 0, stream, (const float*)scratch, (const float*)ml, (__nv_bfloat16*)out,
+                                H, D, splits), "gfb_attention_int8_decode (combine)");
+}
+
 }  // namespace
+
+// One new token per sequence, bfloat16, d 64 or 128, pages of 64, at most 8 heads per key head.  Each sequence in `splits` slices (1 to 48): up to 8 without
+// scratch merge within a cluster of blocks; scratch: float32 [n_tokens * H * splits * (d + 2)], through which they merge in a second kernel.
+GFB_API int gfb_attention_int8_decode(const void* q, void* out, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                                      const int* page_table, int max_pages, int page_size, int n_pages,
+                                      const int* cu_seqlens, const int* tok_seq, const int* slots, const int* lengths, int n_seqs, int n_tokens,
+                                      int H, int G, int d, float scale, int window, int splits, float* scratch, int* status, cudaStream_t stream) {
+    if (n_tokens <= 0) return 0;
+    if ((d != 64 && d != 128) || page_size != PAGE) return gfb_fail("gfb_attention_int8_decode: heads of %d, pages of %d", d, page_size);
+    if (G <= 0 || H % G || H / G > 8 || G > 65535) return gfb_fail("gfb_attention_int8_decode: %d heads over %d", H, G);
+    if (splits < 1 || splits > 48 || (splits > MERGE_SLICES && scratch == nullptr)) return gfb_fail("gfb_attention_int8_decode: %d slices", splits);
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15)
+        return gfb_fail("gfb_attention_int8_decode: everything must be 16-byte aligned");
+    const Int8KV kv{(const int8_t*)k_pool, (const int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages};
+    const GfbBatch b{cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens};
+    if (d == 128) return launch_decode<128, 3>(q, out, scratch, kv, b, H, G, scale, window, splits, status, stream);
+    return launch_decode<64, 6>(q, out, scratch, kv, b, H, G, scale, window, splits, status, stream);
+}
 
 // q [T, H, d] and out [T, H * d] of type dt.  Any d up to 512, any page size.
 GFB_API int gfb_attention_int8_generic(const void* q, void* out, int dt, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,

@@ -161,6 +161,17 @@ def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
     return bn, splits, max(2, min(8, 102400 // (16384 + bn * 128)))
 
 
+def int8_slices(max_kv_len: int, page_size: int, blocks: int, sm_count: int) -> int:
+    """`decode_slices` for a cache of 8-bit integers, four blocks of which share an SM."""
+    pages = -(-max(max_kv_len, 1) // page_size)
+    best, best_cost = 1, None
+    for s in range(1, max(1, min(pages // 2, 48)) + 1):
+        cost = -(-blocks * s // (4 * sm_count)) * (pages / s + 4.0)
+        if best_cost is None or cost < best_cost - 1e-9:
+            best, best_cost = s, cost
+    return best
+
+
 def rows_share_keys(rows: int, longest: int, max_kv_len: int, line: int, blocks: Optional[int] = None) -> bool:
     """Whether the rows (token, head) of a step's 32-bit attention share the keys and values of sixteen rows per block; the bits are the same.  `blocks`: of
     sixteen rows of one sequence and key head at most (default: all full).  A block has sixteen rows' work in a row and stages every key of its sequence, so
@@ -1422,8 +1433,13 @@ class CudaKernels:
         _need(q, shape=(T, n_head, head_dim), name="q")
         _need(out, q.dtype, (T, n_head * head_dim), "attention output")
         self._need_here(q, out, kv.k_pool)
-        self._call("attention_int8", "gfb_attention_int8_generic", _ptr(q), _ptr(out), _dt(q), *self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch),
-                   n_head, n_kv, head_dim, scale, window or 0, _ptr(batch.status), _stream())
+        args = (*self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch), n_head, n_kv, head_dim, scale, window or 0)
+        if q.dtype == torch.bfloat16 and batch.max_q_len == 1 and head_dim in (64, 128) and kv.page_size == 64 and n_head // n_kv <= 8:
+            reach = batch.max_kv_len if not window else min(batch.max_kv_len, window + kv.page_size)
+            splits = int8_slices(reach, kv.page_size, T * n_kv, self.sm_count)
+            scratch = torch.empty(T * n_head * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > MERGED_SLICES else None
+            return self._call("attention_int8", "gfb_attention_int8_decode", _ptr(q), _ptr(out), *args, splits, _ptr(scratch), _ptr(batch.status), _stream())
+        self._call("attention_int8", "gfb_attention_int8_generic", _ptr(q), _ptr(out), _dt(q), *args, _ptr(batch.status), _stream())
 
     def argmax(self, logits, out):
         B, V = logits.shape
