@@ -4,6 +4,7 @@
 //     s_j = scale ks_j (q . K_j),   w_j = exp(s_j - max s),   out = sum_j (w_j vs_j) V_j / sum_j w_j
 // with integers K_j, V_j and their scales ks_j, vs_j.  The scales stay out of the products: a key's joins its score, a value's its weight.
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 
@@ -93,17 +94,22 @@ attention_int8_generic_kernel(const T* __restrict__ q, T* __restrict__ out, Int8
 // is bound by.  A producer thread brings pages by TMA, NS of them in flight; each of four warps takes 16 of a page's 64 keys and runs an online
 // softmax of its own over them, without a block-wide step until the end.
 //
-// Both products are mma.sync m16n8k16 with the cached integers as the A operand and the heads as its 8 columns: S^T = K q^T (16 keys x 8 heads) and
-// O^T += V^T (w vs)^T (16 dims x 8 heads per chunk of 16 dims).  An 8-bit integer is exact in bfloat16; two become two bfloat16 numbers in three
-// operations (`pair`).  They are taken as bytes 0, 2 and bytes 1, 3 of a word, so no byte is moved: the order of the dims within a product over 16 of them
-// is free as long as q has it too, and of V's transposed words the two halves are the rows of dims 2g and 2g + 1.
-// Weights times their value's scale are rounded to bfloat16 for the second product (half a step, 2^-8, of a weight, as the 16-bit cache's attention does); the sum
-// of weights is of the unrounded ones.  The reference of the exponentials follows the maximum in steps of at least 2^8, so a rescale is rare.
+// Both products are mma.sync m16n8k16 in float16 with the cached integers as the A operand and the heads as its 8 columns: S^T = K q^T (16 keys x 8 heads)
+// and O^T += V^T (w vs)^T (16 dims x 8 heads per chunk of 16 dims).  Two 8-bit integers become two float16 numbers in two operations (`pair`), exactly.  They
+// are taken as bytes 0, 2 and bytes 1, 3 of a word, so no byte is moved: the order of the dims within a product over 16 of them is free as long as q
+// has it too, and of V's transposed words the two halves are the rows of dims 2g and 2g + 1.  (As bfloat16 numbers they cost twice the integer
+// operations, and the pipe for those, 74 % busy, was the limit: two sequences of 100,000 tokens 96 us, NOW so.)
+// float16 has few exponents.  A query row comes times the power of two that takes its largest number to 2^14 .. 2^15: bfloat16 numbers down to 2^-32 of that
+// stay exact.  The weights times their value's scale, w vs, have a reference M of their own beside the scores' reference m: the
+// largest lies between 2^9 and 2^15, one 2^-26 of it keeps eleven bits.  Rounding them there is the only rounding ahead of the result's (a bfloat16 weight
+// would be eight times coarser).  The sum of weights is of the unrounded ones.  Both references follow their maximum in steps, so a rescale is rare.
 constexpr int DEC_WARPS = 4, DEC_THREADS = 32 * (DEC_WARPS + 1);
 constexpr int PAGE = 64;
 constexpr int MERGE_SLICES = 8;              // the largest portable cluster
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;   // a page that has not come after a second is given up
 constexpr float LAG = 8.f;                   // log2 by which a score may pass the reference
+constexpr float LIFT = 12.f;                 // log2 of what a weight at its reference is worth; it may pass it by 2^3
+constexpr float LEAST_LOG_SCALE = -100.f;    // a smaller scale of values counts as this for the reference, which keeps 2^(m - M + LIFT) finite
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ unsigned long long global_ns() {
@@ -171,20 +177,23 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {        // an 8 x 8 
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Bytes 0 and 2 of x, signed, as two bfloat16 numbers: with s the sign bit and l the seven bits below it a byte is l - 128 s, 0x4300 | l is 128 + l, and
-// 0xC300 | 128 s is -128 - 128 s.
+// Bytes 0 and 2 of x, signed, as two float16 numbers: a byte with its sign bit turned is the number + 128, behind 0x64 it is 1024 + that, and 1152 is taken off.
 __device__ __forceinline__ uint32_t pair(uint32_t x) {
-    const uint32_t a = (x & 0x007f007fu) | 0x43004300u, b = (x & 0x00800080u) | 0xC300C300u;
+    const uint32_t a = (x & 0x00ff00ffu) ^ 0x64806480u;
     uint32_t y;
-    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(0xE480E480u));
     return y;
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2_f16(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
 }
 // Byte offset of the 16-byte chunk at column `col` (a multiple of 16) of row `row` in a tile of rows of D bytes that came as lines of 128 bytes with 128-byte swizzle.
@@ -237,7 +246,8 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     const int first = lo / PAGE, n_pages = pos / PAGE - first + 1, per = (n_pages + splits - 1) / splits;
     const int p0 = first + z * per, n = max(0, min(per, n_pages - z * per));
 
-    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};           // of heads 2 t4, 2 t4 + 1
+    // of heads 2 t4 and 2 t4 + 1: sums of w vs V times 2^(LIFT - M), references of scores and of weighted scales (log2), sums of weights
+    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
     if (warp == DEC_WARPS) {
@@ -269,15 +279,35 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     } else {
         // q as the B operand: column g4 is a head, its k numbers are the dims 4 t4 and + 2, and 4 t4 + 1 and + 3, of every 16
         uint32_t qb[CH][2];
-        const __nv_bfloat16* qr = q + ((size_t)t * H + g * rep + min(g4, rep - 1)) * D;
+        float unit[2];                               // what a product of integers and lifted queries is worth, log2(e) in it, for heads 2 t4 and + 1
+        {
+            const __nv_bfloat16* qr = q + ((size_t)t * H + g * rep + min(g4, rep - 1)) * D;
+            uint2 v[CH];
+            uint32_t top = 0;
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const uint2 v = g4 < rep ? *reinterpret_cast<const uint2*>(qr + c * 16 + 4 * t4) : make_uint2(0u, 0u);
-            qb[c][0] = __byte_perm(v.x, v.y, 0x5410);
-            qb[c][1] = __byte_perm(v.x, v.y, 0x7632);
+            for (int c = 0; c < CH; c++) {
+                v[c] = g4 < rep ? *reinterpret_cast<const uint2*>(qr + c * 16 + 4 * t4) : make_uint2(0u, 0u);
+                top = max(top, max(max(v[c].x & 0x7fffu, (v[c].x >> 16) & 0x7fffu), max(v[c].y & 0x7fffu, (v[c].y >> 16) & 0x7fffu)));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // exponent of the row's largest number (zeros, subnormal and infinite ones: as they are within what a float's exponent takes)
+            const int e = min(max((int)(top >> 7) - 127, -100), 100);
+            const float lift = exp2f((float)(14 - e));
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                const float f0 = __uint_as_float(v[c].x << 16) * lift, f1 = __uint_as_float(v[c].x & 0xffff0000u) * lift;
+                const float f2 = __uint_as_float(v[c].y << 16) * lift, f3 = __uint_as_float(v[c].y & 0xffff0000u) * lift;
+                qb[c][0] = pack2_f16(f0, f2);
+                qb[c][1] = pack2_f16(f1, f3);
+            }
+            const float mine = exp2f((float)(e - 14)) * scale_log2e;
+            unit[0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
+            unit[1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
         }
         // this lane's row of the four matrices that one ldmatrix takes: keys 0-7 and 8-15 of the warp's, chunks c and c + 1
         const int lrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), lcol = (lane >> 4) * 16;
+        float F[2] = {0.f, 0.f};                     // 2^(m - M + LIFT)
         for (int i = 0; i < n; i++) {
             const int st = i % NS;
             if (!mbar_wait_warp(bar0 + 16 * st, (i / NS) & 1, gave_up, status, 300)) break;
@@ -287,12 +317,12 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             for (int c = 0; c < CH; c += 2) {
                 uint32_t r[4];
                 ldsm_x4(kt + swz<D>(lrow, c * 16 + lcol), r);
-                mma_bf16(sc, pair(r[0]), pair(r[1]), pair(r[0] >> 8), pair(r[1] >> 8), qb[c][0], qb[c][1]);
-                mma_bf16(sc, pair(r[2]), pair(r[3]), pair(r[2] >> 8), pair(r[3] >> 8), qb[c + 1][0], qb[c + 1][1]);
+                mma_f16(sc, pair(r[0]), pair(r[1]), pair(r[0] >> 8), pair(r[1] >> 8), qb[c][0], qb[c][1]);
+                mma_f16(sc, pair(r[2]), pair(r[3]), pair(r[2] >> 8), pair(r[3] >> 8), qb[c + 1][0], qb[c + 1][1]);
             }
             const float* ks = scales + st * 2 * PAGE + warp * 16 + g4;
-            const float k0 = ks[0] * scale_log2e, k1 = ks[8] * scale_log2e, v0 = ks[PAGE], v1 = ks[PAGE + 8];
-            sc[0] *= k0; sc[1] *= k0; sc[2] *= k1; sc[3] *= k1;
+            const float k0 = ks[0], k1 = ks[8], v0 = ks[PAGE], v1 = ks[PAGE + 8];
+            sc[0] *= k0 * unit[0]; sc[1] *= k0 * unit[1]; sc[2] *= k1 * unit[0]; sc[3] *= k1 * unit[1];
             const int j = (p0 + i) * PAGE + warp * 16 + g4;
             const bool all = !dead[st] && (p0 + i) * PAGE >= lo && (p0 + i) * PAGE + PAGE - 1 <= pos;       // uniform: every key of the page is seen
             bool see0 = true, see1 = true;
@@ -302,35 +332,46 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 if (!see0) sc[0] = sc[1] = -INFINITY;
                 if (!see1) sc[2] = sc[3] = -INFINITY;
             }
-            if (__any_sync(0xffffffffu, fmaxf(sc[0], sc[2]) > m[0] + LAG || fmaxf(sc[1], sc[3]) > m[1] + LAG)) {
+            float p[4], w[4];
+            auto weigh = [&]() {
+                const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
+                p[0] = exp2f(sc[0] - r0); p[1] = exp2f(sc[1] - r1); p[2] = exp2f(sc[2] - r0); p[3] = exp2f(sc[3] - r1);
+                w[0] = see0 ? p[0] * (v0 * F[0]) : 0.f; w[1] = see0 ? p[1] * (v0 * F[1]) : 0.f;     // an unseen key's value scale can be anything
+                w[2] = see1 ? p[2] * (v1 * F[0]) : 0.f; w[3] = see1 ? p[3] * (v1 * F[1]) : 0.f;
+            };
+            weigh();
+            const bool far = fmaxf(sc[0], sc[2]) > m[0] + LAG || fmaxf(sc[1], sc[3]) > m[1] + LAG || fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > 32768.f;
+            if (__any_sync(0xffffffffu, far)) {
+                const float lv0 = fmaxf(log2f(v0), LEAST_LOG_SCALE), lv1 = fmaxf(log2f(v1), LEAST_LOG_SCALE);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     float x = fmaxf(sc[e], sc[e + 2]);
+                    float y = fmaxf(see0 ? sc[e] + lv0 : -INFINITY, see1 ? sc[e + 2] + lv1 : -INFINITY);
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    const float now = fmaxf(m[e], x), corr = m[e] == -INFINITY ? 0.f : exp2f(m[e] - now);
+                    for (int d = 4; d < 32; d <<= 1) {
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+                    }
+                    const float now = fmaxf(m[e], x), Now = fmaxf(M[e], y);
+                    l[e] *= m[e] == -INFINITY ? 0.f : exp2f(m[e] - now);
+                    const float corr = M[e] == -INFINITY ? 0.f : exp2f(M[e] - Now);
                     m[e] = now;
-                    l[e] *= corr;
+                    M[e] = Now;
+                    F[e] = now == -INFINITY ? 0.f : exp2f(now - Now + LIFT);
 #pragma unroll
                     for (int c = 0; c < CH; c++) { o[c][e] *= corr; o[c][e + 2] *= corr; }
                 }
+                weigh();
             }
-            const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
-            const float p00 = exp2f(sc[0] - r0), p01 = exp2f(sc[1] - r1), p10 = exp2f(sc[2] - r0), p11 = exp2f(sc[3] - r1);
-            l[0] += p00 + p10;
-            l[1] += p01 + p11;
-            // an unseen key's value scale can be anything
-            uint32_t wa = pack2(p00 * v0, p01 * v0), wb = pack2(p10 * v1, p11 * v1);
-            if (!see0) wa = 0u;
-            if (!see1) wb = 0u;
-            wa = transposed(wa);
-            wb = transposed(wb);
+            l[0] += p[0] + p[2];
+            l[1] += p[1] + p[3];
+            const uint32_t wa = transposed(pack2_f16(w[0], w[1])), wb = transposed(pack2_f16(w[2], w[3]));
 #pragma unroll
             for (int c = 0; c < CH; c += 2) {
                 uint32_t r[4];
                 ldsm_x4_trans(vt + swz<D>(lrow, c * 16 + lcol), r);
-                mma_bf16(o[c], pair(r[0]), pair(r[0] >> 8), pair(r[1]), pair(r[1] >> 8), wa, wb);
-                mma_bf16(o[c + 1], pair(r[2]), pair(r[2] >> 8), pair(r[3]), pair(r[3] >> 8), wa, wb);
+                mma_f16(o[c], pair(r[0]), pair(r[0] >> 8), pair(r[1]), pair(r[1] >> 8), wa, wb);
+                mma_f16(o[c + 1], pair(r[2]), pair(r[2] >> 8), pair(r[3]), pair(r[3] >> 8), wa, wb);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
@@ -344,7 +385,7 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         __syncthreads();
     }
 
-    // Merge of the four warps: they exchange (reference, sum), each brings its sums to the common reference (and, with one slice, divides them).
+    // Merge of the four warps: they exchange (reference, sum), each brings its sums to the common reference of the scores (and, with one slice, divides them).
     float* Ow = reinterpret_cast<float*>(smem);                    // [4][8][OP]
     float* mw = Ow + 4 * 8 * S::OP;                                // [4][8]
     float* lw = mw + 32;                                           // [4][8]
@@ -370,7 +411,7 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
             for (int w = 0; w < 4; w++)
                 if (mw[w * 8 + h] != -INFINITY) sum += lw[w * 8 + h] * exp2f(mw[w * 8 + h] - top);
-            float f = m[e] == -INFINITY ? 0.f : exp2f(m[e] - top);
+            float f = m[e] == -INFINITY ? 0.f : exp2f(M[e] - LIFT - top);
             if (splits == 1) f = sum == 0.f ? 0.f : f / sum;
             float* row = Ow + (warp * 8 + h) * S::OP + 2 * g4;
 #pragma unroll
