@@ -26,7 +26,7 @@ constexpr int MAX_DPT = 4;      // head_dim <= CHUNK * MAX_DPT
 // position with an online softmax between them, so a query's result is the same bits in any batch.
 template <typename T>
 __global__ void __launch_bounds__(CHUNK)
-attention_int8_generic_kernel(const T* __restrict__ q, T* __restrict__ out, Int8KV kv, GfbBatch b, int H, int G, int d, float scale, int window, int* status) {
+attention_int8_generic_kernel(const T* q, T* out, Int8KV kv, GfbBatch b, int H, int G, int d, float scale, int window, int* status) {
     extern __shared__ __align__(16) float smem[];
     float* qs = smem;              // [d]
     __shared__ float ps[CHUNK];    // w_j vs_j
@@ -212,13 +212,162 @@ struct DecodeSmem {
     static_assert(4 * 8 * OP * 4 + 64 * 4 + 8 * D * 4 + 16 * 4 <= NS * STAGE, "the merge area fits where the pages were");
 };
 
-// q [T, H, D], out [T, H * D]; with more than one slice the blocks of a (token, key head) are a cluster (merge) or leave their sums in scratch_o
-// [T, H, splits, D] and (reference, sum) in scratch_ml [T, H, splits, 2].
+// 2^x, 0 below 2^-126
+__device__ __forceinline__ float power2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// What a warp keeps of a (token, key head) while it walks over pages: of every lane the heads 2 t4 and 2 t4 + 1 (e = 0, 1), dims 16 c + 2 g4 and + 1.
+template <int D>
+struct WarpRows {
+    static constexpr int CH = D / 16;
+    float o[CH][4];              // sums of w vs V times 2^(LIFT - M)
+    float m[2], M[2];            // references of scores and of weighted scales, log2
+    float l[2];                  // sums of weights, this lane's keys
+    float F[2];                  // 2^(m - M + LIFT)
+    uint32_t qb[CH][2];          // q as the B operand: column g4 is a head, its k numbers are the dims 4 t4 and + 2, and 4 t4 + 1 and + 3, of every 16
+    float unit[2];               // what a product of integers and lifted queries is worth, log2(e) in it
+
+    // `row`: the first of the group's query rows, `rep` of them
+    __device__ __forceinline__ void start(const __nv_bfloat16* row, int rep, float scale_log2e, int g4, int t4) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+        m[0] = m[1] = M[0] = M[1] = -INFINITY;
+        l[0] = l[1] = F[0] = F[1] = 0.f;
+        const __nv_bfloat16* qr = row + min(g4, rep - 1) * D;
+        uint2 v[CH];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            v[c] = g4 < rep ? *reinterpret_cast<const uint2*>(qr + c * 16 + 4 * t4) : make_uint2(0u, 0u);
+            top = max(top, max(max(v[c].x & 0x7fffu, (v[c].x >> 16) & 0x7fffu), max(v[c].y & 0x7fffu, (v[c].y >> 16) & 0x7fffu)));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // exponent of the row's largest number (of zeros, tiny and huge ones as far as the factor stays within a float's exponents)
+        const int e = min(max((int)(top >> 7) - 127, -100), 100);
+        const float lift = exp2f((float)(14 - e));
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const float f0 = __uint_as_float(v[c].x << 16) * lift, f1 = __uint_as_float(v[c].x & 0xffff0000u) * lift;
+            const float f2 = __uint_as_float(v[c].y << 16) * lift, f3 = __uint_as_float(v[c].y & 0xffff0000u) * lift;
+            qb[c][0] = pack2_f16(f0, f2);
+            qb[c][1] = pack2_f16(f1, f3);
+        }
+        const float mine = exp2f((float)(e - 14)) * scale_log2e;
+        unit[0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
+        unit[1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
+    }
+
+    // The warp's 16 keys of a page: tiles of K and V, scales of the warp's first key on (ks, and PAGE further the values'); off: where this lane's row of the
+    // four matrices that one ldmatrix takes lies, chunks 2 i and 2 i + 1.  see0, see1: whether keys g4 and g4 + 8 are seen.
+    __device__ __forceinline__ void page(uint32_t kt, uint32_t vt, const uint32_t (&off)[CH / 2], const float* ks, bool see0, bool see1) {
+        float sc[4] = {0.f, 0.f, 0.f, 0.f};                                 // (key g4, heads 2 t4 and + 1), (key g4 + 8, the same)
+#pragma unroll
+        for (int c = 0; c < CH; c += 2) {
+            uint32_t r[4];
+            ldsm_x4(kt + off[c / 2], r);
+            mma_f16(sc, pair(r[0]), pair(r[1]), pair(r[0] >> 8), pair(r[1] >> 8), qb[c][0], qb[c][1]);
+            mma_f16(sc, pair(r[2]), pair(r[3]), pair(r[2] >> 8), pair(r[3] >> 8), qb[c + 1][0], qb[c + 1][1]);
+        }
+        const float k0 = ks[0], k1 = ks[8], v0 = ks[PAGE], v1 = ks[PAGE + 8];
+        sc[0] = see0 ? sc[0] * (k0 * unit[0]) : -INFINITY;
+        sc[1] = see0 ? sc[1] * (k0 * unit[1]) : -INFINITY;
+        sc[2] = see1 ? sc[2] * (k1 * unit[0]) : -INFINITY;
+        sc[3] = see1 ? sc[3] * (k1 * unit[1]) : -INFINITY;
+        float p[4], w[4];
+        auto weigh = [&]() {
+            const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
+            p[0] = power2(sc[0] - r0); p[1] = power2(sc[1] - r1); p[2] = power2(sc[2] - r0); p[3] = power2(sc[3] - r1);
+            w[0] = see0 ? p[0] * (v0 * F[0]) : 0.f; w[1] = see0 ? p[1] * (v0 * F[1]) : 0.f;     // an unseen key's value scale can be anything
+            w[2] = see1 ? p[2] * (v1 * F[0]) : 0.f; w[3] = see1 ? p[3] * (v1 * F[1]) : 0.f;
+        };
+        weigh();
+        const bool far = fmaxf(sc[0], sc[2]) > m[0] + LAG || fmaxf(sc[1], sc[3]) > m[1] + LAG || fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > 32768.f;
+        if (__any_sync(0xffffffffu, far)) {
+            const float lv0 = fmaxf(log2f(v0), LEAST_LOG_SCALE), lv1 = fmaxf(log2f(v1), LEAST_LOG_SCALE);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float x = fmaxf(sc[e], sc[e + 2]);
+                float y = fmaxf(see0 ? sc[e] + lv0 : -INFINITY, see1 ? sc[e + 2] + lv1 : -INFINITY);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+                }
+                const float now = fmaxf(m[e], x), Now = fmaxf(M[e], y);
+                l[e] *= m[e] == -INFINITY ? 0.f : power2(m[e] - now);
+                const float corr = M[e] == -INFINITY ? 0.f : power2(M[e] - Now);
+                m[e] = now;
+                M[e] = Now;
+                F[e] = now == -INFINITY ? 0.f : power2(now - Now + LIFT);
+#pragma unroll
+                for (int c = 0; c < CH; c++) { o[c][e] *= corr; o[c][e + 2] *= corr; }
+            }
+            weigh();
+        }
+        l[0] += p[0] + p[2];
+        l[1] += p[1] + p[3];
+        const uint32_t wa = transposed(pack2_f16(w[0], w[1])), wb = transposed(pack2_f16(w[2], w[3]));
+#pragma unroll
+        for (int c = 0; c < CH; c += 2) {
+            uint32_t r[4];
+            ldsm_x4_trans(vt + off[c / 2], r);
+            mma_f16(o[c], pair(r[0]), pair(r[0] >> 8), pair(r[1]), pair(r[1] >> 8), wa, wb);
+            mma_f16(o[c + 1], pair(r[2]), pair(r[2] >> 8), pair(r[3]), pair(r[3] >> 8), wa, wb);
+        }
+    }
+
+    __device__ __forceinline__ void sum_lanes() {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+    }
+};
+
+// What the four warps of a block made of a head, brought together: the common reference of the scores, the sum of weights under it, and the factor that
+// brings a warp's own sums (references m, M) there.
+struct Common { float top, sum, factor; };
+__device__ __forceinline__ Common common_of(const float* mw, const float* lw, int h, float m, float M) {
+    Common c;
+    c.top = fmaxf(fmaxf(mw[h], mw[8 + h]), fmaxf(mw[16 + h], mw[24 + h]));
+    c.sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+        if (mw[w * 8 + h] != -INFINITY) c.sum += lw[w * 8 + h] * exp2f(mw[w * 8 + h] - c.top);
+    c.factor = m == -INFINITY ? 0.f : exp2f(M - LIFT - c.top);
+    return c;
+}
+
+// A page's integers and scales into a stage of the ring; a page that the table does not have is reported, its stage marked and nothing asked for.
+template <int D>
+__device__ __forceinline__ void fetch_page(const CUtensorMap* map_k, const CUtensorMap* map_v, const Int8KV& kv, int G, int g, int page, int slot, int index,
+                                           uint32_t tile, uint32_t scales, uint32_t full, int* dead, uint64_t pol, int* status) {
+    if (page < 0 || page >= kv.n_pages) {
+        gfb_report(status, GFB_ERR_PAGE_TABLE, slot, index);
+        *dead = 1;
+        mbar_arrive(full);
+        return;
+    }
+    *dead = 0;
+    const size_t row = ((size_t)page * G + g) * PAGE;               // the page's first row in the pools
+    const int line = (int)(row * D / 128);
+    mbar_expect_tx(full, 2 * PAGE * D + 2 * PAGE * 4);
+    tma_load_2d_hint(tile, map_k, 0, line, full, pol);
+    bulk_load(scales, kv.k_scale + row, PAGE * 4, full);
+    tma_load_2d_hint(tile + PAGE * D, map_v, 0, line, full, pol);
+    bulk_load(scales + PAGE * 4, kv.v_scale + row, PAGE * 4, full);
+}
+
+// Few pages altogether: a block per (token, key head, slice); the slices of a (token, key head) are a cluster and merge through its shared memory.
+// q [T, H, D], out [T, H * D].
 template <int D, int NS>
 __global__ void __launch_bounds__(DEC_THREADS, 4)
-attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* __restrict__ q,
-                             __nv_bfloat16* __restrict__ out, float* __restrict__ scratch_o, float* __restrict__ scratch_ml, Int8KV kv, GfbBatch b, int H, int G,
-                             float scale_log2e, int window, int splits, int merge, int* status) {
+attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* q,
+                             __nv_bfloat16* out, Int8KV kv, GfbBatch b, int H, int G, float scale_log2e, int window, int splits, int* status) {
     using S = DecodeSmem<D, NS>;
     constexpr int CH = D / 16;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -246,10 +395,7 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     const int first = lo / PAGE, n_pages = pos / PAGE - first + 1, per = (n_pages + splits - 1) / splits;
     const int p0 = first + z * per, n = max(0, min(per, n_pages - z * per));
 
-    // of heads 2 t4 and 2 t4 + 1: sums of w vs V times 2^(LIFT - M), references of scores and of weighted scales (log2), sums of weights
-    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    WarpRows<D> rows;
     if (warp == DEC_WARPS) {
         if (lane == 0) {
             const int* pt = kv.page_table + (size_t)slot * kv.max_pages;
@@ -259,120 +405,22 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 const int st = i % NS, page = next;
                 next = i + 1 < n && p0 + i + 1 < kv.max_pages ? pt[p0 + i + 1] : -1;
                 if (i >= NS && !mbar_wait(bar0 + 16 * st + 8, ((i / NS) & 1) ^ 1, gave_up, status, 301)) break;
-                const uint32_t full = bar0 + 16 * st;
-                if (page < 0 || page >= kv.n_pages) {
-                    gfb_report(status, GFB_ERR_PAGE_TABLE, slot, p0 + i);
-                    dead[st] = 1;
-                    mbar_arrive(full);
-                    continue;
-                }
-                dead[st] = 0;
-                const size_t row = ((size_t)page * G + g) * PAGE;               // the page's first row in the pools
-                const int line = (int)(row * D / 128);
-                mbar_expect_tx(full, S::STAGE + 2 * PAGE * 4);
-                tma_load_2d_hint(tiles + st * S::STAGE, &map_k, 0, line, full, pol);
-                bulk_load(tiles + S::SCALES + st * 2 * PAGE * 4, kv.k_scale + row, PAGE * 4, full);
-                tma_load_2d_hint(tiles + st * S::STAGE + S::TILE, &map_v, 0, line, full, pol);
-                bulk_load(tiles + S::SCALES + st * 2 * PAGE * 4 + PAGE * 4, kv.v_scale + row, PAGE * 4, full);
+                fetch_page<D>(&map_k, &map_v, kv, G, g, page, slot, p0 + i, tiles + st * S::STAGE, tiles + S::SCALES + st * 2 * PAGE * 4, bar0 + 16 * st, dead + st,
+                              pol, status);
             }
         }
     } else {
-        // q as the B operand: column g4 is a head, its k numbers are the dims 4 t4 and + 2, and 4 t4 + 1 and + 3, of every 16
-        uint32_t qb[CH][2];
-        float unit[2];                               // what a product of integers and lifted queries is worth, log2(e) in it, for heads 2 t4 and + 1
-        {
-            const __nv_bfloat16* qr = q + ((size_t)t * H + g * rep + min(g4, rep - 1)) * D;
-            uint2 v[CH];
-            uint32_t top = 0;
+        rows.start(q + ((size_t)t * H + g * rep) * D, rep, scale_log2e, g4, t4);
+        uint32_t off[CH / 2];
 #pragma unroll
-            for (int c = 0; c < CH; c++) {
-                v[c] = g4 < rep ? *reinterpret_cast<const uint2*>(qr + c * 16 + 4 * t4) : make_uint2(0u, 0u);
-                top = max(top, max(max(v[c].x & 0x7fffu, (v[c].x >> 16) & 0x7fffu), max(v[c].y & 0x7fffu, (v[c].y >> 16) & 0x7fffu)));
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // exponent of the row's largest number (zeros, subnormal and infinite ones: as they are within what a float's exponent takes)
-            const int e = min(max((int)(top >> 7) - 127, -100), 100);
-            const float lift = exp2f((float)(14 - e));
-#pragma unroll
-            for (int c = 0; c < CH; c++) {
-                const float f0 = __uint_as_float(v[c].x << 16) * lift, f1 = __uint_as_float(v[c].x & 0xffff0000u) * lift;
-                const float f2 = __uint_as_float(v[c].y << 16) * lift, f3 = __uint_as_float(v[c].y & 0xffff0000u) * lift;
-                qb[c][0] = pack2_f16(f0, f2);
-                qb[c][1] = pack2_f16(f1, f3);
-            }
-            const float mine = exp2f((float)(e - 14)) * scale_log2e;
-            unit[0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
-            unit[1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
-        }
-        // this lane's row of the four matrices that one ldmatrix takes: keys 0-7 and 8-15 of the warp's, chunks c and c + 1
-        const int lrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), lcol = (lane >> 4) * 16;
-        float F[2] = {0.f, 0.f};                     // 2^(m - M + LIFT)
+        for (int c = 0; c < CH / 2; c++) off[c] = swz<D>(warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c * 32 + (lane >> 4) * 16);
         for (int i = 0; i < n; i++) {
             const int st = i % NS;
             if (!mbar_wait_warp(bar0 + 16 * st, (i / NS) & 1, gave_up, status, 300)) break;
-            const uint32_t kt = tiles + st * S::STAGE, vt = kt + S::TILE;
-            float sc[4] = {0.f, 0.f, 0.f, 0.f};                                 // (key g4, heads 2 t4 and + 1), (key g4 + 8, the same)
-#pragma unroll
-            for (int c = 0; c < CH; c += 2) {
-                uint32_t r[4];
-                ldsm_x4(kt + swz<D>(lrow, c * 16 + lcol), r);
-                mma_f16(sc, pair(r[0]), pair(r[1]), pair(r[0] >> 8), pair(r[1] >> 8), qb[c][0], qb[c][1]);
-                mma_f16(sc, pair(r[2]), pair(r[3]), pair(r[2] >> 8), pair(r[3] >> 8), qb[c + 1][0], qb[c + 1][1]);
-            }
-            const float* ks = scales + st * 2 * PAGE + warp * 16 + g4;
-            const float k0 = ks[0], k1 = ks[8], v0 = ks[PAGE], v1 = ks[PAGE + 8];
-            sc[0] *= k0 * unit[0]; sc[1] *= k0 * unit[1]; sc[2] *= k1 * unit[0]; sc[3] *= k1 * unit[1];
-            const int j = (p0 + i) * PAGE + warp * 16 + g4;
-            const bool all = !dead[st] && (p0 + i) * PAGE >= lo && (p0 + i) * PAGE + PAGE - 1 <= pos;       // uniform: every key of the page is seen
-            bool see0 = true, see1 = true;
-            if (!all) {
-                see0 = !dead[st] && j >= lo && j <= pos;
-                see1 = !dead[st] && j + 8 >= lo && j + 8 <= pos;
-                if (!see0) sc[0] = sc[1] = -INFINITY;
-                if (!see1) sc[2] = sc[3] = -INFINITY;
-            }
-            float p[4], w[4];
-            auto weigh = [&]() {
-                const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
-                p[0] = exp2f(sc[0] - r0); p[1] = exp2f(sc[1] - r1); p[2] = exp2f(sc[2] - r0); p[3] = exp2f(sc[3] - r1);
-                w[0] = see0 ? p[0] * (v0 * F[0]) : 0.f; w[1] = see0 ? p[1] * (v0 * F[1]) : 0.f;     // an unseen key's value scale can be anything
-                w[2] = see1 ? p[2] * (v1 * F[0]) : 0.f; w[3] = see1 ? p[3] * (v1 * F[1]) : 0.f;
-            };
-            weigh();
-            const bool far = fmaxf(sc[0], sc[2]) > m[0] + LAG || fmaxf(sc[1], sc[3]) > m[1] + LAG || fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > 32768.f;
-            if (__any_sync(0xffffffffu, far)) {
-                const float lv0 = fmaxf(log2f(v0), LEAST_LOG_SCALE), lv1 = fmaxf(log2f(v1), LEAST_LOG_SCALE);
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float x = fmaxf(sc[e], sc[e + 2]);
-                    float y = fmaxf(see0 ? sc[e] + lv0 : -INFINITY, see1 ? sc[e + 2] + lv1 : -INFINITY);
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) {
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-                    }
-                    const float now = fmaxf(m[e], x), Now = fmaxf(M[e], y);
-                    l[e] *= m[e] == -INFINITY ? 0.f : exp2f(m[e] - now);
-                    const float corr = M[e] == -INFINITY ? 0.f : exp2f(M[e] - Now);
-                    m[e] = now;
-                    M[e] = Now;
-                    F[e] = now == -INFINITY ? 0.f : exp2f(now - Now + LIFT);
-#pragma unroll
-                    for (int c = 0; c < CH; c++) { o[c][e] *= corr; o[c][e + 2] *= corr; }
-                }
-                weigh();
-            }
-            l[0] += p[0] + p[2];
-            l[1] += p[1] + p[3];
-            const uint32_t wa = transposed(pack2_f16(w[0], w[1])), wb = transposed(pack2_f16(w[2], w[3]));
-#pragma unroll
-            for (int c = 0; c < CH; c += 2) {
-                uint32_t r[4];
-                ldsm_x4_trans(vt + swz<D>(lrow, c * 16 + lcol), r);
-                mma_f16(o[c], pair(r[0]), pair(r[0] >> 8), pair(r[1]), pair(r[1] >> 8), wa, wb);
-                mma_f16(o[c + 1], pair(r[2]), pair(r[2] >> 8), pair(r[3]), pair(r[3] >> 8), wa, wb);
-            }
+            const uint32_t kt = tiles + st * S::STAGE;
+            const int j0 = (p0 + i) * PAGE, j = j0 + warp * 16 + g4;
+            const bool here = !dead[st], all = here && j0 >= lo && j0 + PAGE - 1 <= pos;       // uniform: every key of the page is seen
+            rows.page(kt, kt + S::TILE, off, scales + st * 2 * PAGE + warp * 16 + g4, all || (here && j >= lo && j <= pos), all || (here && j + 8 >= lo && j + 8 <= pos));
             __syncwarp();
             if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
         }
@@ -392,13 +440,10 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     float* mine = lw + 32;                                         // [8][D]
     float* ml = mine + 8 * D;                                      // [8][2]
     if (warp < DEC_WARPS) {
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+        rows.sum_lanes();
         if (g4 == 0) {
-            mw[warp * 8 + 2 * t4] = m[0]; mw[warp * 8 + 2 * t4 + 1] = m[1];
-            lw[warp * 8 + 2 * t4] = l[0]; lw[warp * 8 + 2 * t4 + 1] = l[1];
+            mw[warp * 8 + 2 * t4] = rows.m[0]; mw[warp * 8 + 2 * t4 + 1] = rows.m[1];
+            lw[warp * 8 + 2 * t4] = rows.l[0]; lw[warp * 8 + 2 * t4 + 1] = rows.l[1];
         }
     }
     __syncthreads();
@@ -406,17 +451,12 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const int h = 2 * t4 + e;
-            const float top = fmaxf(fmaxf(mw[h], mw[8 + h]), fmaxf(mw[16 + h], mw[24 + h]));
-            float sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; w++)
-                if (mw[w * 8 + h] != -INFINITY) sum += lw[w * 8 + h] * exp2f(mw[w * 8 + h] - top);
-            float f = m[e] == -INFINITY ? 0.f : exp2f(M[e] - LIFT - top);
-            if (splits == 1) f = sum == 0.f ? 0.f : f / sum;
+            const Common c = common_of(mw, lw, h, rows.m[e], rows.M[e]);
+            const float f = splits > 1 ? c.factor : c.sum == 0.f ? 0.f : c.factor / c.sum;
             float* row = Ow + (warp * 8 + h) * S::OP + 2 * g4;
 #pragma unroll
-            for (int c = 0; c < CH; c++) *reinterpret_cast<float2*>(row + c * 16) = make_float2(o[c][e] * f, o[c][e + 2] * f);
-            if (warp == 0 && g4 == 0) { ml[2 * h] = top; ml[2 * h + 1] = sum; }
+            for (int i = 0; i < CH; i++) *reinterpret_cast<float2*>(row + i * 16) = make_float2(rows.o[i][e] * f, rows.o[i][e + 2] * f);
+            if (warp == 0 && g4 == 0) { ml[2 * h] = c.top; ml[2 * h + 1] = c.sum; }
         }
     }
     __syncthreads();
@@ -430,19 +470,10 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             acc.y += a.y;
         }
         if (splits == 1) *reinterpret_cast<uint32_t*>(out + ((size_t)t * H + head) * D + dim) = pack2(acc.x, acc.y);
-        else if (merge) *reinterpret_cast<float2*>(mine + h * D + dim) = acc;
-        else *reinterpret_cast<float2*>(scratch_o + (((size_t)t * H + head) * splits + z) * D + dim) = acc;
+        else *reinterpret_cast<float2*>(mine + h * D + dim) = acc;
     }
     if (splits == 1) return;
-    if (!merge) {
-        if ((int)threadIdx.x < rep) {
-            float* at = scratch_ml + (((size_t)t * H + g * rep + threadIdx.x) * splits + z) * 2;
-            at[0] = ml[2 * threadIdx.x];
-            at[1] = ml[2 * threadIdx.x + 1];
-        }
-        return;
-    }
-    // the slices are a cluster: each finishes its part of the numbers over all of them, in ascending order
+    // each slice finishes its part of the numbers over all of them, in ascending order
     gfb_cluster_sync();
     for (int idx = z * DEC_THREADS + threadIdx.x; idx < rep * (D / 2); idx += splits * DEC_THREADS) {
         const int h = idx / (D / 2), dim = 2 * (idx - h * (D / 2)), head = g * rep + h;
@@ -471,23 +502,272 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     gfb_cluster_sync();                                            // no block leaves while another reads its shared memory
 }
 
-// The slices of a (token, head) through memory, in ascending order.
-__global__ void __launch_bounds__(128)
-attention_int8_combine_kernel(const float* __restrict__ scratch_o, const float* __restrict__ scratch_ml, __nv_bfloat16* __restrict__ out, int H, int d, int splits) {
+// ---- many pages: every block an equal share of them ---------------------------------------------------------------
+// The pages of all (token, key head) pairs, one after the other, are one row of U units; block c of C walks over the units c U / C .. (c + 1) U / C, across
+// pairs, whatever the sequences' lengths are, which only the device knows: it adds them up for itself.  A pair that one block has whole is finished there; of the others every
+// block leaves its sums under the common reference in scratch, slot 2 c + 1 for a pair that it begins and does not end, slot 2 c for one that it does not
+// begin, and a second kernel merges a pair's blocks in ascending order.  The producer runs ahead across pairs, so the stream never stops between them.
+// (A block per (token, key head, equal slice) waits for the longest sequence: 64 of 501 to 8,190 tokens 168 us, EVEN so.)
+constexpr int LEAST_UNITS = 4;               // pages that a block takes at least
+
+template <int D, int NS>
+struct ShareSmem {
+    static constexpr int TILE = PAGE * D, STAGE = 2 * TILE;
+    static constexpr int SCALES = NS * STAGE, REFS = SCALES + NS * 2 * PAGE * 4, BARS = REFS + 64 * 4;
+    static constexpr int BYTES = 1024 + BARS + 2 * NS * 8 + (NS + 4) * 4;
+    static_assert(4 * 8 * D * 4 == STAGE, "a stage holds the sums of four warps");
+};
+
+// The pages that the token's query sees: first one, how many, and the positions.
+struct Seen {
+    int slot, pos, lo, first, n;
+    __device__ __forceinline__ Seen(const GfbBatch& b, int t, int window) {
+        const int s = b.tok_seq[t];
+        slot = b.slots[s];
+        pos = b.lengths[slot] + (t - b.cu_seqlens[s]);
+        lo = window > 0 ? max(0, pos - window + 1) : 0;
+        first = lo / PAGE;
+        n = max(1, pos / PAGE - first + 1);
+    }
+};
+
+// How the units are shared out.
+constexpr int MOST_TOKENS = 4096;            // whose pages are counted where the ring of stages will be
+
+struct Shares {
+    long long U;
+    int C;
+    __device__ __forceinline__ Shares(long long units, int blocks) : U(units), C((int)max(1ll, min((long long)blocks, units / LEAST_UNITS))) {}
+    __device__ __forceinline__ long long begin(int c) const { return (long long)c * U / C; }
+    __device__ __forceinline__ int owner(long long u) const { return (int)(((u + 1) * C - 1) / U); }
+};
+
+// before [T + 1]: pages of the tokens ahead of each, and of all; scratch_o [2 gridDim.x][rep][D], scratch_ml [2 gridDim.x][rep][2].
+template <int D, int NS>
+__global__ void __launch_bounds__(DEC_THREADS, 4)
+attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* q,
+                             __nv_bfloat16* out, float* scratch_o, float* scratch_ml, int* before,
+                             Int8KV kv, GfbBatch b, int H, int G, float scale_log2e, int window, int* status) {
+    using S = ShareSmem<D, NS>;
+    constexpr int CH = D / 16;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (tiles - smem_u32(smem_raw));
+    const float* scales = reinterpret_cast<const float*>(smem + S::SCALES);
+    float* mw = reinterpret_cast<float*>(smem + S::REFS);                        // [4][8]
+    float* lw = mw + 32;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS);
+    int* dead = reinterpret_cast<int*>(bars + 2 * NS);
+    int* gave_up = dead + NS;
+    int* begin = gave_up + 1;                                                    // token of the block's first unit, units of it that others have, units of this block
+    const uint32_t bar0 = smem_u32(bars);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
+    const int rep = H / G, T = b.n_tokens;
+    if (threadIdx.x == 0) {
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
+        for (int i = 0; i < NS; i++) { mbar_init(bar0 + 16 * i, 1); mbar_init(bar0 + 16 * i + 8, DEC_WARPS); }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     gfb_pdl_launch();
     gfb_pdl_wait();
-    const size_t row = (size_t)blockIdx.x * H + blockIdx.y;
-    const float* ml = scratch_ml + row * splits * 2;
-    float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < splits; k++) top = fmaxf(top, ml[2 * k]);
-    for (int k = 0; k < splits; k++)
-        if (ml[2 * k] != -INFINITY) sum = fmaf(ml[2 * k + 1], exp2f(ml[2 * k] - top), sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int dim = threadIdx.x; dim < d; dim += blockDim.x) {
-        float o = 0.f;
-        for (int k = 0; k < splits; k++)
-            if (ml[2 * k] != -INFINITY) o = fmaf(scratch_o[(row * splits + k) * d + dim], exp2f(ml[2 * k] - top), o);
-        out[row * d + dim] = __float2bfloat16_rn(o * inv);
+    int* pages_of = reinterpret_cast<int*>(smem);                                // [T], where the ring will be
+    for (int t = threadIdx.x; t < T; t += DEC_THREADS) pages_of[t] = Seen(b, t, window).n;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                 // pages come by TMA where the counts are
+    __syncthreads();
+    if (warp == DEC_WARPS) {
+        int total = 0;
+        for (int t = lane; t < T; t += 32) total += pages_of[t];
+        total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+        const Shares sh((long long)total * G, (int)gridDim.x);
+        const bool idle = (int)blockIdx.x >= sh.C || total == 0;
+        const long long u0 = idle ? 0 : sh.begin(blockIdx.x), u1 = idle ? 0 : sh.begin(blockIdx.x + 1);
+        int ahead = 0, t = 0, skip = 0;                                          // the token of the block's first unit, and its units that other blocks have
+        for (int t0 = 0; t0 < T; t0 += 32) {
+            const int n = t0 + lane < T ? pages_of[t0 + lane] : 0;
+            int sum = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += x;
+            }
+            const long long mine = (long long)(ahead + sum - n) * G;             // the token's first unit
+            const unsigned found = __ballot_sync(0xffffffffu, u0 < u1 && mine <= u0 && u0 < mine + (long long)n * G);
+            if (found) {
+                t = t0 + __ffs(found) - 1;
+                skip = __shfl_sync(0xffffffffu, (int)(u0 - mine), __ffs(found) - 1);
+            }
+            if (blockIdx.x == 0 && t0 + lane < T) before[t0 + lane] = ahead + sum - n;
+            ahead += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (blockIdx.x == 0 && lane == 0) before[T] = ahead;
+        if (lane == 0) { begin[0] = t; begin[1] = skip; begin[2] = (int)(u1 - u0); }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+
+    // Every warp walks over the same shares; a wait that runs out voids the results (the status says so), and the warps go on to meet at the barriers.
+    int t = begin[0], left = begin[2];
+    if (left > 0) {
+        Seen seen(b, t, window);
+        int g = begin[1] / seen.n, p = begin[1] - g * seen.n, it = 0;            // it: pages so far
+        uint32_t off[CH / 2];
+#pragma unroll
+        for (int c = 0; c < CH / 2; c++) off[c] = swz<D>((warp & 3) * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c * 32 + (lane >> 4) * 16);
+        for (;;) {
+            const int n = min(seen.n - p, left);
+            if (warp == DEC_WARPS) {
+                if (lane == 0) {
+                    const uint64_t pol = l2_evict_first_policy();
+                    const int* pt = kv.page_table + (size_t)seen.slot * kv.max_pages;
+                    const int p0 = seen.first + p;
+                    int next = p0 < kv.max_pages ? pt[p0] : -1;
+                    for (int i = 0; i < n; i++) {
+                        const int k = it + i, st = k % NS, page = next;
+                        next = i + 1 < n && p0 + i + 1 < kv.max_pages ? pt[p0 + i + 1] : -1;
+                        if (k >= NS && !mbar_wait(bar0 + 16 * st + 8, ((k / NS) & 1) ^ 1, gave_up, status, 303)) break;
+                        fetch_page<D>(&map_k, &map_v, kv, G, g, page, seen.slot, p0 + i, tiles + st * S::STAGE, tiles + S::SCALES + st * 2 * PAGE * 4, bar0 + 16 * st,
+                                      dead + st, pol, status);
+                    }
+                }
+                __syncwarp();
+            } else {
+                WarpRows<D> rows;
+                rows.start(q + ((size_t)t * H + g * rep) * D, rep, scale_log2e, g4, t4);
+                const int j1 = (seen.first + p) * PAGE;
+                for (int i = 0; i < n; i++) {
+                    const int st = (it + i) % NS;
+                    if (!mbar_wait_warp(bar0 + 16 * st, ((it + i) / NS) & 1, gave_up, status, 302)) continue;
+                    const uint32_t kt = tiles + st * S::STAGE;
+                    const int j0 = j1 + i * PAGE, j = j0 + warp * 16 + g4;
+                    const bool here = !dead[st], all = here && j0 >= seen.lo && j0 + PAGE - 1 <= seen.pos;
+                    rows.page(kt, kt + S::TILE, off, scales + st * 2 * PAGE + warp * 16 + g4, all || (here && j >= seen.lo && j <= seen.pos),
+                              all || (here && j + 8 >= seen.lo && j + 8 <= seen.pos));
+                    __syncwarp();
+                    if (lane == 0 && i + 1 < n) mbar_arrive(bar0 + 16 * st + 8);
+                }
+                // The four warps' sums meet where the share's last page was: [4][8][D], the 16 numbers of a chunk exchanged by the head's lane group so
+                // that a warp's rows fall on different banks.
+                const int st = (it + n - 1) % NS;
+                float* Ow = reinterpret_cast<float*>(smem + st * S::STAGE);
+                rows.sum_lanes();
+                if (g4 == 0) {
+                    mw[warp * 8 + 2 * t4] = rows.m[0]; mw[warp * 8 + 2 * t4 + 1] = rows.m[1];
+                    lw[warp * 8 + 2 * t4] = rows.l[0]; lw[warp * 8 + 2 * t4 + 1] = rows.l[1];
+                }
+                asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory");
+                const bool whole = n == seen.n;
+                const size_t part = 2 * (size_t)blockIdx.x + (p == 0 ? 1 : 0);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int h = 2 * t4 + e;
+                    const Common c = common_of(mw, lw, h, rows.m[e], rows.M[e]);
+                    const float f = !whole ? c.factor : c.sum == 0.f ? 0.f : c.factor / c.sum;
+                    if (!whole && warp == 0 && g4 == 0 && h < rep) *reinterpret_cast<float2*>(scratch_ml + (part * rep + h) * 2) = make_float2(c.top, c.sum);
+                    float* row = Ow + (warp * 8 + h) * D + 2 * g4;
+#pragma unroll
+                    for (int i = 0; i < CH; i++) *reinterpret_cast<float2*>(row + (i ^ t4) * 16) = make_float2(rows.o[i][e] * f, rows.o[i][e + 2] * f);
+                }
+                asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory");
+                for (int idx = threadIdx.x; idx < rep * (D / 2); idx += 32 * DEC_WARPS) {
+                    const int h = idx / (D / 2), dim = 2 * (idx - h * (D / 2));
+                    const float* at = Ow + h * D + (((dim >> 4) ^ (h >> 1)) << 4) + (dim & 15);
+                    float2 x = *reinterpret_cast<const float2*>(at);
+#pragma unroll
+                    for (int w = 1; w < DEC_WARPS; w++) {
+                        const float2 y = *reinterpret_cast<const float2*>(at + w * 8 * D);
+                        x.x += y.x;
+                        x.y += y.y;
+                    }
+                    if (whole) *reinterpret_cast<uint32_t*>(out + ((size_t)t * H + g * rep + h) * D + dim) = pack2(x.x, x.y);
+                    else *reinterpret_cast<float2*>(scratch_o + (part * rep + h) * D + dim) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the next page comes by TMA where these numbers are
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
+            }
+            it += n;
+            left -= n;
+            if (left <= 0) break;
+            p = 0;
+            if (++g == G) {
+                g = 0;
+                seen = Seen(b, ++t, window);
+            }
+        }
+    }
+    __syncthreads();
+    if (*gave_up) {
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 50000ull) __nanosleep(1000);
+    }
+}
+
+// The pairs that several blocks share, merged over them.  One block per (token, head): its four warps take every fourth of a pair's parts, in ascending order with
+// four of them in flight, and what they have is added in ascending order of the warps.  blocks: of the kernel ahead.
+template <int D>
+__global__ void __launch_bounds__(128)
+attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, const int* before, __nv_bfloat16* out,
+                            int T, int H, int G, int blocks) {
+    constexpr int V = D / 32;                                     // numbers per lane
+    __shared__ float refs[4][2];
+    __shared__ float sums[4][D];
+    gfb_pdl_launch();
+    gfb_pdl_wait();
+    const int t = blockIdx.x, head = blockIdx.y, rep = H / G, g = head / rep, h = head - g * rep, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ahead = before[t], n = before[t + 1] - ahead;
+    if (n <= 0) return;
+    const Shares sh((long long)before[T] * G, blocks);
+    const long long u = (long long)ahead * G + (long long)g * n;
+    const int c0 = sh.owner(u), c1 = sh.owner(u + n - 1);
+    if (c0 == c1) return;
+    float top = -INFINITY, sum = 0.f, o[V] = {};
+    for (int c = c0 + warp; c <= c1; c += 16) {
+        float2 ml[4];
+        float x[4][V];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int part = min(c + 4 * k, c1);                  // (past the end: the last one again, with no weight)
+            const size_t at = (2 * (size_t)part + (part == c0)) * rep + h;
+            ml[k] = *reinterpret_cast<const float2*>(scratch_ml + at * 2);
+            if (c + 4 * k > c1) ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int v = 0; v < V; v++) x[k][v] = scratch_o[at * D + lane + 32 * v];
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < 4; k++) now = fmaxf(now, ml[k].x);
+        const float down = top == -INFINITY ? 0.f : exp2f(top - now);
+        top = now;
+        sum *= down;
+#pragma unroll
+        for (int v = 0; v < V; v++) o[v] *= down;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (ml[k].x == -INFINITY) continue;
+            const float w = exp2f(ml[k].x - now);
+            sum = fmaf(ml[k].y, w, sum);
+#pragma unroll
+            for (int v = 0; v < V; v++) o[v] = fmaf(x[k][v], w, o[v]);
+        }
+    }
+    if (lane == 0) { refs[warp][0] = top; refs[warp][1] = sum; }
+#pragma unroll
+    for (int v = 0; v < V; v++) sums[warp][lane + 32 * v] = o[v];
+    __syncthreads();
+    const float all = fmaxf(fmaxf(refs[0][0], refs[1][0]), fmaxf(refs[2][0], refs[3][0]));
+    float total = 0.f, w[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        w[k] = refs[k][0] == -INFINITY ? 0.f : exp2f(refs[k][0] - all);
+        total = fmaf(refs[k][1], w[k], total);
+    }
+    for (int dim = threadIdx.x; dim < D; dim += 128) {
+        float y = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) y = fmaf(sums[k][dim], w[k], y);
+        out[((size_t)t * H + head) * D + dim] = __float2bfloat16_rn(total == 0.f ? 0.f : y / total);
     }
 }
 
@@ -538,43 +818,67 @@ int room(F kern, size_t smem, bool (&configured)[MAX_DEVICES]) {
     return 0;
 }
 
+// What the host hands to the decode kernels.
+struct Decode {
+    const void* q;
+    void* out;
+    Int8KV kv;
+    GfbBatch b;
+    int H, G;
+    float scale;
+    int window;
+    int* status;
+    cudaStream_t stream;
+};
+
 template <int D, int NS>
-int launch_decode(const void* q, void* out, float* scratch, const Int8KV& kv, const GfbBatch& b, int H, int G, float scale, int window, int splits, int* status,
-                  cudaStream_t stream) {
+int launch_decode(const Decode& a, int splits) {
     auto kern = attention_int8_decode_kernel<D, NS>;
     const size_t smem = DecodeSmem<D, NS>::BYTES;
     static bool configured[MAX_DEVICES] = {};
     if (room(kern, smem, configured)) return 1;
     CUtensorMap mk, mv;
-    if (pool_map(&mk, kv.k_pool, kv.n_pages, G, D) || pool_map(&mv, kv.v_pool, kv.n_pages, G, D)) return 1;
-    const int merge = splits > 1 && scratch == nullptr;
-    float* ml = scratch ? scratch + (size_t)b.n_tokens * H * splits * D : nullptr;
-    int rc = gfb_check(gfb_launch_clusters(kern, dim3(b.n_tokens, G, splits), dim3(DEC_THREADS), smem, stream, dim3(1, 1, merge ? splits : 1), mk, mv,
-                                           (const __nv_bfloat16*)q, (__nv_bfloat16*)out, scratch, ml, kv, b, H, G, scale * 1.4426950408889634f, window, splits, merge,
-                                           status), "gfb_attention_int8_decode");
-    if (rc || splits == 1 || merge) return rc;
-    return gfb_check(gfb_launch(attention_int8_combine_kernel, dim3(b.n_tokens, H), dim3(128), 0, stream, (const float*)scratch, (const float*)ml, (__nv_bfloat16*)out,
-                                H, D, splits), "gfb_attention_int8_decode (combine)");
+    if (pool_map(&mk, a.kv.k_pool, a.kv.n_pages, a.G, D) || pool_map(&mv, a.kv.v_pool, a.kv.n_pages, a.G, D)) return 1;
+    return gfb_check(gfb_launch_clusters(kern, dim3(a.b.n_tokens, a.G, splits), dim3(DEC_THREADS), smem, a.stream, dim3(1, 1, splits), mk, mv,
+                                         (const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out, a.kv, a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, splits,
+                                         a.status), "gfb_attention_int8_decode");
+}
+
+template <int D, int NS>
+int launch_shares(const Decode& a, int blocks, float* scratch) {
+    auto kern = attention_int8_shares_kernel<D, NS>;
+    const size_t smem = ShareSmem<D, NS>::BYTES;
+    static bool configured[MAX_DEVICES] = {};
+    if (room(kern, smem, configured)) return 1;
+    CUtensorMap mk, mv;
+    if (pool_map(&mk, a.kv.k_pool, a.kv.n_pages, a.G, D) || pool_map(&mv, a.kv.v_pool, a.kv.n_pages, a.G, D)) return 1;
+    const int rep = a.H / a.G;
+    float* ml = scratch + (size_t)2 * blocks * rep * D;
+    int* before = (int*)(ml + (size_t)2 * blocks * rep * 2);
+    if (gfb_check(gfb_launch(kern, dim3(blocks), dim3(DEC_THREADS), smem, a.stream, mk, mv, (const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out, scratch, ml, before, a.kv,
+                             a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, a.status), "gfb_attention_int8_decode (shares)")) return 1;
+    return gfb_check(gfb_launch(attention_int8_merge_kernel<D>, dim3(a.b.n_tokens, a.H), dim3(128), 0, a.stream, (const float*)scratch, (const float*)ml, (const int*)before,
+                                (__nv_bfloat16*)a.out, a.b.n_tokens, a.H, a.G, blocks), "gfb_attention_int8_decode (merge)");
 }
 
 }  // namespace
 
-// One new token per sequence, bfloat16, d 64 or 128, pages of 64, at most 8 heads per key head.  Each sequence in `splits` slices (1 to 48): up to 8 without
-// scratch merge within a cluster of blocks; scratch: float32 [n_tokens * H * splits * (d + 2)], through which they merge in a second kernel.
+// One new token per sequence, bfloat16, d 64 or 128, pages of 64, at most 8 heads per key head.  Without scratch each sequence in `splits` equal slices (1 to 8),
+// which merge within a cluster of blocks.  With scratch (float32 [2 blocks (H / G) (d + 2) + n_tokens + 1]) all pages in equal shares for `blocks` blocks.
 GFB_API int gfb_attention_int8_decode(const void* q, void* out, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                                       const int* page_table, int max_pages, int page_size, int n_pages,
                                       const int* cu_seqlens, const int* tok_seq, const int* slots, const int* lengths, int n_seqs, int n_tokens,
-                                      int H, int G, int d, float scale, int window, int splits, float* scratch, int* status, cudaStream_t stream) {
+                                      int H, int G, int d, float scale, int window, int splits, int blocks, float* scratch, int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     if ((d != 64 && d != 128) || page_size != PAGE) return gfb_fail("gfb_attention_int8_decode: heads of %d, pages of %d", d, page_size);
     if (G <= 0 || H % G || H / G > 8 || G > 65535) return gfb_fail("gfb_attention_int8_decode: %d heads over %d", H, G);
-    if (splits < 1 || splits > 48 || (splits > MERGE_SLICES && scratch == nullptr)) return gfb_fail("gfb_attention_int8_decode: %d slices", splits);
-    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15)
+    if (scratch == nullptr ? splits < 1 || splits > MERGE_SLICES : blocks < 1 || n_tokens > MOST_TOKENS) return gfb_fail("gfb_attention_int8_decode: %d slices, %d blocks, %d tokens", splits, blocks, n_tokens);
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)scratch) & 15)
         return gfb_fail("gfb_attention_int8_decode: everything must be 16-byte aligned");
-    const Int8KV kv{(const int8_t*)k_pool, (const int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages};
-    const GfbBatch b{cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens};
-    if (d == 128) return launch_decode<128, 3>(q, out, scratch, kv, b, H, G, scale, window, splits, status, stream);
-    return launch_decode<64, 6>(q, out, scratch, kv, b, H, G, scale, window, splits, status, stream);
+    const Decode a{q, out, {(const int8_t*)k_pool, (const int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages},
+                   {cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens}, H, G, scale, window, status, stream};
+    if (scratch != nullptr) return d == 128 ? launch_shares<128, 3>(a, blocks, scratch) : launch_shares<64, 6>(a, blocks, scratch);
+    return d == 128 ? launch_decode<128, 3>(a, splits) : launch_decode<64, 6>(a, splits);
 }
 
 // q [T, H, d] and out [T, H * d] of type dt.  Any d up to 512, any page size.

@@ -240,8 +240,8 @@ struct Barriers {
 // map_w: W [N, K], map_a: A [M, K].  Block (x, y, z): weight rows 128 x .., tokens BN y .., part z of K; the parts of a tile are one cluster.
 template <int BN, int KIND, typename TO>
 __global__ void __launch_bounds__(192)
-gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ a_scale,
-                     const float* __restrict__ w_scale, TO* __restrict__ out, int M, int N, int K, int ldo, int kb_per_split, int stages, int vec, int epi, int* status) {
+gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* a_scale,
+                     const float* w_scale, TO* out, int M, int N, int K, int ldo, int kb_per_split, int stages, int vec, int epi, int* status) {
     constexpr int Y_TILE_BYTES = BN * BK;
     constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
     constexpr int GROUP = BN < 32 ? BN : 32;
@@ -488,8 +488,8 @@ __device__ __forceinline__ void drain_chunk(float* stage, uint32_t taddr, int c0
 
 template <int KIND, typename TO>
 __global__ void __launch_bounds__(192)
-gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const float* __restrict__ a_scale,
-                      const float* __restrict__ w_scale, TO* __restrict__ out, int M, int N, int K, int ldo, int stages, int vec, int epi, int* status) {
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const float* a_scale,
+                      const float* w_scale, TO* out, int M, int N, int K, int ldo, int stages, int vec, int epi, int* status) {
     extern __shared__ uint8_t smem_raw[];
     if (threadIdx.x == 32) { prefetch_map(&map_a); prefetch_map(&map_w); }
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;

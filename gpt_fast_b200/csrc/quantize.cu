@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* scratch
 // q [R, pitch] and scale [R] of x [R, K]; the columns from K to the pitch are zeros.  One block per row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int K, int pitch, int early) {
+quantize_rows_kernel(const T* x, int8_t* q, float* scale, int K, int pitch, int early) {
     __shared__ uint32_t scratch[32];
     if (early) gfb_pdl_launch();
     gfb_pdl_wait();
@@ -66,8 +66,8 @@ quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __r
 // The same of h = x * rsqrt(mean(x^2) + eps) * w in 32 bits, x float32 [T, D] with pending partial sums and picked rows as in gfb_rmsnorm.
 template <typename TW>
 __global__ void __launch_bounds__(256)
-rmsnorm_quantize_kernel(float* __restrict__ x, const float* __restrict__ pending, int S, size_t slice, const TW* __restrict__ w,
-                        int8_t* __restrict__ q, float* __restrict__ scale, const int* __restrict__ rows, int D, int pitch, float eps) {
+rmsnorm_quantize_kernel(float* x, const float* pending, int S, size_t slice, const TW* w,
+                        int8_t* q, float* scale, const int* rows, int D, int pitch, float eps) {
     __shared__ float fscratch[32];
     __shared__ uint32_t scratch[32];
     gfb_pdl_launch();
@@ -111,7 +111,7 @@ __device__ __forceinline__ long long cache_row(const int* page_table, int max_pa
 // One warp per head of a token; the rotation rounds each product and sum by itself.
 template <typename T>
 __global__ void __launch_bounds__(128)
-rope_append_int8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, Int8KV kv, GfbBatch b, const float* __restrict__ table, int table_len,
+rope_append_int8_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const float* table, int table_len,
                         int H, int G, int d, int pairing, int append, int* status) {
     gfb_pdl_launch();
     gfb_pdl_wait();
@@ -165,7 +165,7 @@ rope_append_int8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, Int8KV
 // What the cache holds at the places of the step's tokens: k_out, v_out [T, G, d].  One block per token.
 template <typename TO>
 __global__ void __launch_bounds__(256)
-read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* __restrict__ k_out, TO* __restrict__ v_out, int G, int d, int* status) {
+read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d, int* status) {
     gfb_pdl_launch();
     gfb_pdl_wait();
     const int t = blockIdx.x;

@@ -161,15 +161,13 @@ def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
     return bn, splits, max(2, min(8, 102400 // (16384 + bn * 128)))
 
 
-def int8_slices(max_kv_len: int, page_size: int, blocks: int, sm_count: int) -> int:
-    """`decode_slices` for a cache of 8-bit integers, four blocks of which share an SM."""
+def int8_shares(max_kv_len: int, page_size: int, pairs: int, sm_count: int):
+    """(slices, blocks) of a decode step over a cache of 8-bit integers, `pairs` (token, key head) pairs of sequences of at most max_kv_len tokens.  blocks 0: every
+    pair in that many equal slices, a cluster of at most 8 blocks; otherwise all pages in equal shares for that many blocks."""
     pages = -(-max(max_kv_len, 1) // page_size)
-    best, best_cost = 1, None
-    for s in range(1, max(1, min(pages // 2, 48)) + 1):
-        cost = -(-blocks * s // (4 * sm_count)) * (pages / s + 4.0)
-        if best_cost is None or cost < best_cost - 1e-9:
-            best, best_cost = s, cost
-    return best
+    if pairs * pages > 4 * sm_count * 4:
+        return 1, 4 * sm_count
+    return max(1, min(8, pages // 2, 4 * sm_count // max(pairs, 1))), 0
 
 
 def rows_share_keys(rows: int, longest: int, max_kv_len: int, line: int, blocks: Optional[int] = None) -> bool:
@@ -1436,9 +1434,9 @@ class CudaKernels:
         args = (*self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch), n_head, n_kv, head_dim, scale, window or 0)
         if q.dtype == torch.bfloat16 and batch.max_q_len == 1 and head_dim in (64, 128) and kv.page_size == 64 and n_head // n_kv <= 8:
             reach = batch.max_kv_len if not window else min(batch.max_kv_len, window + kv.page_size)
-            splits = int8_slices(reach, kv.page_size, T * n_kv, self.sm_count)
-            scratch = torch.empty(T * n_head * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > MERGED_SLICES else None
-            return self._call("attention_int8", "gfb_attention_int8_decode", _ptr(q), _ptr(out), *args, splits, _ptr(scratch), _ptr(batch.status), _stream())
+            splits, blocks = int8_shares(reach, kv.page_size, T * n_kv, self.sm_count)
+            scratch = torch.empty(2 * blocks * (n_head // n_kv) * (head_dim + 2) + T + 1, dtype=torch.float32, device=q.device) if blocks else None
+            return self._call("attention_int8", "gfb_attention_int8_decode", _ptr(q), _ptr(out), *args, splits, blocks, _ptr(scratch), _ptr(batch.status), _stream())
         self._call("attention_int8", "gfb_attention_int8_generic", _ptr(q), _ptr(out), _dt(q), *args, _ptr(batch.status), _stream())
 
     def argmax(self, logits, out):
