@@ -108,6 +108,7 @@ constexpr int PAGE = 64;
 constexpr int MERGE_SLICES = 8;              // the largest portable cluster
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;   // a page that has not come after a second is given up
 constexpr float LAG = 8.f;                   // log2 by which a score may pass the reference
+constexpr float NONE = -1e30f;               // the reference ahead of the first key: below every score, and finite, so that no difference is infinity less infinity
 constexpr float LIFT = 12.f;                 // log2 of what a weight at its reference is worth; it may pass it by 2^3
 constexpr float LEAST_LOG_SCALE = -100.f;    // a smaller scale of values counts as this for the reference, which keeps 2^(m - M + LIFT) finite
 
@@ -169,8 +170,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
+template <int AHEAD>                                                // AHEAD bytes behind addr
 __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4+%5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "n"(AHEAD));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {        // an 8 x 8 matrix of 16-bit numbers over the warp
     uint32_t y;
@@ -234,7 +237,7 @@ struct WarpRows {
     __device__ __forceinline__ void start(const __nv_bfloat16* row, int rep, float scale_log2e, int g4, int t4) {
 #pragma unroll
         for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-        m[0] = m[1] = M[0] = M[1] = -INFINITY;
+        m[0] = m[1] = M[0] = M[1] = NONE;
         l[0] = l[1] = F[0] = F[1] = 0.f;
         const __nv_bfloat16* qr = row + min(g4, rep - 1) * D;
         uint2 v[CH];
@@ -261,9 +264,10 @@ struct WarpRows {
         unit[1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
     }
 
-    // The warp's 16 keys of a page: tiles of K and V, scales of the warp's first key on (ks, and PAGE further the values'); off: where this lane's row of the
-    // four matrices that one ldmatrix takes lies, chunks 2 i and 2 i + 1.  see0, see1: whether keys g4 and g4 + 8 are seen.
-    __device__ __forceinline__ void page(uint32_t kt, uint32_t vt, const uint32_t (&off)[CH / 2], const float* ks, bool see0, bool see1) {
+    // The warp's 16 keys of a page: the tile of K, with V's behind it, scales of the warp's first key on (ks, and PAGE further the values'); off: where this
+    // lane's row of the four matrices that one ldmatrix takes lies, chunks 2 i and 2 i + 1.  ALL: every key is seen; else see0, see1: whether g4 and g4 + 8 are.
+    template <bool ALL>
+    __device__ __forceinline__ void page(uint32_t kt, const uint32_t (&off)[CH / 2], const float* ks, bool see0 = true, bool see1 = true) {
         float sc[4] = {0.f, 0.f, 0.f, 0.f};                                 // (key g4, heads 2 t4 and + 1), (key g4 + 8, the same)
 #pragma unroll
         for (int c = 0; c < CH; c += 2) {
@@ -273,16 +277,19 @@ struct WarpRows {
             mma_f16(sc, pair(r[2]), pair(r[3]), pair(r[2] >> 8), pair(r[3] >> 8), qb[c + 1][0], qb[c + 1][1]);
         }
         const float k0 = ks[0], k1 = ks[8], v0 = ks[PAGE], v1 = ks[PAGE + 8];
-        sc[0] = see0 ? sc[0] * (k0 * unit[0]) : -INFINITY;
-        sc[1] = see0 ? sc[1] * (k0 * unit[1]) : -INFINITY;
-        sc[2] = see1 ? sc[2] * (k1 * unit[0]) : -INFINITY;
-        sc[3] = see1 ? sc[3] * (k1 * unit[1]) : -INFINITY;
+        sc[0] *= k0 * unit[0]; sc[1] *= k0 * unit[1]; sc[2] *= k1 * unit[0]; sc[3] *= k1 * unit[1];
+        if (!ALL) {
+            if (!see0) sc[0] = sc[1] = -INFINITY;
+            if (!see1) sc[2] = sc[3] = -INFINITY;
+        }
         float p[4], w[4];
         auto weigh = [&]() {
-            const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
-            p[0] = power2(sc[0] - r0); p[1] = power2(sc[1] - r1); p[2] = power2(sc[2] - r0); p[3] = power2(sc[3] - r1);
-            w[0] = see0 ? p[0] * (v0 * F[0]) : 0.f; w[1] = see0 ? p[1] * (v0 * F[1]) : 0.f;     // an unseen key's value scale can be anything
-            w[2] = see1 ? p[2] * (v1 * F[0]) : 0.f; w[3] = see1 ? p[3] * (v1 * F[1]) : 0.f;
+            p[0] = power2(sc[0] - m[0]); p[1] = power2(sc[1] - m[1]); p[2] = power2(sc[2] - m[0]); p[3] = power2(sc[3] - m[1]);
+            w[0] = p[0] * (v0 * F[0]); w[1] = p[1] * (v0 * F[1]); w[2] = p[2] * (v1 * F[0]); w[3] = p[3] * (v1 * F[1]);
+            if (!ALL) {                                                     // an unseen key's value scale can be anything
+                if (!see0) w[0] = w[1] = 0.f;
+                if (!see1) w[2] = w[3] = 0.f;
+            }
         };
         weigh();
         const bool far = fmaxf(sc[0], sc[2]) > m[0] + LAG || fmaxf(sc[1], sc[3]) > m[1] + LAG || fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > 32768.f;
@@ -291,18 +298,17 @@ struct WarpRows {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 float x = fmaxf(sc[e], sc[e + 2]);
-                float y = fmaxf(see0 ? sc[e] + lv0 : -INFINITY, see1 ? sc[e + 2] + lv1 : -INFINITY);
+                float y = fmaxf(ALL || see0 ? sc[e] + lv0 : -INFINITY, ALL || see1 ? sc[e + 2] + lv1 : -INFINITY);
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
                 }
-                const float now = fmaxf(m[e], x), Now = fmaxf(M[e], y);
-                l[e] *= m[e] == -INFINITY ? 0.f : power2(m[e] - now);
-                const float corr = M[e] == -INFINITY ? 0.f : power2(M[e] - Now);
+                const float now = fmaxf(m[e], x), Now = fmaxf(M[e], y), corr = power2(M[e] - Now);
+                l[e] *= power2(m[e] - now);
                 m[e] = now;
                 M[e] = Now;
-                F[e] = now == -INFINITY ? 0.f : power2(now - Now + LIFT);
+                F[e] = power2(now - Now + LIFT);
 #pragma unroll
                 for (int c = 0; c < CH; c++) { o[c][e] *= corr; o[c][e + 2] *= corr; }
             }
@@ -314,10 +320,16 @@ struct WarpRows {
 #pragma unroll
         for (int c = 0; c < CH; c += 2) {
             uint32_t r[4];
-            ldsm_x4_trans(vt + off[c / 2], r);
+            ldsm_x4_trans<PAGE * D>(kt + off[c / 2], r);
             mma_f16(o[c], pair(r[0]), pair(r[0] >> 8), pair(r[1]), pair(r[1] >> 8), wa, wb);
             mma_f16(o[c + 1], pair(r[2]), pair(r[2] >> 8), pair(r[3]), pair(r[3] >> 8), wa, wb);
         }
+    }
+
+    // The same for a page whose first position is j0, of which [lo, pos] are seen; none of a dead one.
+    __device__ __forceinline__ void page_at(uint32_t kt, const uint32_t (&off)[CH / 2], const float* ks, int j0, int j, int lo, int pos, bool dead) {
+        if (!dead && j0 >= lo && j0 + PAGE - 1 <= pos) page<true>(kt, off, ks);
+        else page<false>(kt, off, ks, !dead && j >= lo && j <= pos, !dead && j + 8 >= lo && j + 8 <= pos);
     }
 
     __device__ __forceinline__ void sum_lanes() {
@@ -329,16 +341,15 @@ struct WarpRows {
 };
 
 // What the four warps of a block made of a head, brought together: the common reference of the scores, the sum of weights under it, and the factor that
-// brings a warp's own sums (references m, M) there.
+// brings a warp's own sums (reference M) there.
 struct Common { float top, sum, factor; };
-__device__ __forceinline__ Common common_of(const float* mw, const float* lw, int h, float m, float M) {
+__device__ __forceinline__ Common common_of(const float* mw, const float* lw, int h, float M) {
     Common c;
     c.top = fmaxf(fmaxf(mw[h], mw[8 + h]), fmaxf(mw[16 + h], mw[24 + h]));
     c.sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; w++)
-        if (mw[w * 8 + h] != -INFINITY) c.sum += lw[w * 8 + h] * exp2f(mw[w * 8 + h] - c.top);
-    c.factor = m == -INFINITY ? 0.f : exp2f(M - LIFT - c.top);
+    for (int w = 0; w < 4; w++) c.sum = fmaf(lw[w * 8 + h], power2(mw[w * 8 + h] - c.top), c.sum);
+    c.factor = power2(M - LIFT - c.top);
     return c;
 }
 
@@ -414,15 +425,14 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         uint32_t off[CH / 2];
 #pragma unroll
         for (int c = 0; c < CH / 2; c++) off[c] = swz<D>(warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c * 32 + (lane >> 4) * 16);
-        for (int i = 0; i < n; i++) {
-            const int st = i % NS;
-            if (!mbar_wait_warp(bar0 + 16 * st, (i / NS) & 1, gave_up, status, 300)) break;
-            const uint32_t kt = tiles + st * S::STAGE;
-            const int j0 = (p0 + i) * PAGE, j = j0 + warp * 16 + g4;
-            const bool here = !dead[st], all = here && j0 >= lo && j0 + PAGE - 1 <= pos;       // uniform: every key of the page is seen
-            rows.page(kt, kt + S::TILE, off, scales + st * 2 * PAGE + warp * 16 + g4, all || (here && j >= lo && j <= pos), all || (here && j + 8 >= lo && j + 8 <= pos));
+        int st = 0, j0 = p0 * PAGE;
+        uint32_t ph = 0;
+        for (int i = 0; i < n; i++, j0 += PAGE) {
+            if (!mbar_wait_warp(bar0 + 16 * st, ph, gave_up, status, 300)) break;
+            rows.page_at(tiles + st * S::STAGE, off, scales + st * 2 * PAGE + warp * 16 + g4, j0, j0 + warp * 16 + g4, lo, pos, dead[st] != 0);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
+            if (++st == NS) { st = 0; ph ^= 1u; }
         }
     }
     __syncthreads();                                               // every page has been read, or the block gave up
@@ -451,7 +461,7 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const int h = 2 * t4 + e;
-            const Common c = common_of(mw, lw, h, rows.m[e], rows.M[e]);
+            const Common c = common_of(mw, lw, h, rows.M[e]);
             const float f = splits > 1 ? c.factor : c.sum == 0.f ? 0.f : c.factor / c.sum;
             float* row = Ow + (warp * 8 + h) * S::OP + 2 * g4;
 #pragma unroll
@@ -484,14 +494,14 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 part[k] = gfb_cluster_load2(ml + 2 * h, k);
                 row[k] = gfb_cluster_load2(mine + h * D + dim, k);
             }
-        float top = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
+        float top = NONE, sum = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
         for (int k = 0; k < MERGE_SLICES; k++)
             if (k < splits) top = fmaxf(top, part[k].x);
 #pragma unroll
         for (int k = 0; k < MERGE_SLICES; k++)
-            if (k < splits && part[k].x != -INFINITY) {
-                const float e = exp2f(part[k].x - top);
+            if (k < splits) {
+                const float e = power2(part[k].x - top);
                 sum = fmaf(part[k].y, e, sum);
                 o0 = fmaf(row[k].x, e, o0);
                 o1 = fmaf(row[k].y, e, o1);
@@ -611,7 +621,9 @@ attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __
     int t = begin[0], left = begin[2];
     if (left > 0) {
         Seen seen(b, t, window);
-        int g = begin[1] / seen.n, p = begin[1] - g * seen.n, it = 0;            // it: pages so far
+        int g = begin[1] / seen.n, p = begin[1] - g * seen.n, st = 0;            // st, ph: the next page's stage and the phase of its barriers
+        uint32_t ph = 0;
+        bool again = false;                                                      // the producer: the ring has been filled once
         uint32_t off[CH / 2];
 #pragma unroll
         for (int c = 0; c < CH / 2; c++) off[c] = swz<D>((warp & 3) * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c * 32 + (lane >> 4) * 16);
@@ -624,33 +636,31 @@ attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     const int p0 = seen.first + p;
                     int next = p0 < kv.max_pages ? pt[p0] : -1;
                     for (int i = 0; i < n; i++) {
-                        const int k = it + i, st = k % NS, page = next;
+                        const int page = next;
                         next = i + 1 < n && p0 + i + 1 < kv.max_pages ? pt[p0 + i + 1] : -1;
-                        if (k >= NS && !mbar_wait(bar0 + 16 * st + 8, ((k / NS) & 1) ^ 1, gave_up, status, 303)) break;
+                        if (again && !mbar_wait(bar0 + 16 * st + 8, ph ^ 1u, gave_up, status, 303)) break;
                         fetch_page<D>(&map_k, &map_v, kv, G, g, page, seen.slot, p0 + i, tiles + st * S::STAGE, tiles + S::SCALES + st * 2 * PAGE * 4, bar0 + 16 * st,
                                       dead + st, pol, status);
+                        if (++st == NS) { st = 0; ph ^= 1u; again = true; }
                     }
                 }
                 __syncwarp();
             } else {
                 WarpRows<D> rows;
                 rows.start(q + ((size_t)t * H + g * rep) * D, rep, scale_log2e, g4, t4);
-                const int j1 = (seen.first + p) * PAGE;
-                for (int i = 0; i < n; i++) {
-                    const int st = (it + i) % NS;
-                    if (!mbar_wait_warp(bar0 + 16 * st, ((it + i) / NS) & 1, gave_up, status, 302)) continue;
-                    const uint32_t kt = tiles + st * S::STAGE;
-                    const int j0 = j1 + i * PAGE, j = j0 + warp * 16 + g4;
-                    const bool here = !dead[st], all = here && j0 >= seen.lo && j0 + PAGE - 1 <= seen.pos;
-                    rows.page(kt, kt + S::TILE, off, scales + st * 2 * PAGE + warp * 16 + g4, all || (here && j >= seen.lo && j <= seen.pos),
-                              all || (here && j + 8 >= seen.lo && j + 8 <= seen.pos));
-                    __syncwarp();
-                    if (lane == 0 && i + 1 < n) mbar_arrive(bar0 + 16 * st + 8);
+                int j0 = (seen.first + p) * PAGE, last = st;
+                for (int i = 0; i < n; i++, j0 += PAGE) {
+                    last = st;
+                    if (mbar_wait_warp(bar0 + 16 * st, ph, gave_up, status, 302)) {
+                        rows.page_at(tiles + st * S::STAGE, off, scales + st * 2 * PAGE + warp * 16 + g4, j0, j0 + warp * 16 + g4, seen.lo, seen.pos, dead[st] != 0);
+                        __syncwarp();
+                        if (lane == 0 && i + 1 < n) mbar_arrive(bar0 + 16 * st + 8);
+                    }
+                    if (++st == NS) { st = 0; ph ^= 1u; }
                 }
                 // The four warps' sums meet where the share's last page was: [4][8][D], the 16 numbers of a chunk exchanged by the head's lane group so
                 // that a warp's rows fall on different banks.
-                const int st = (it + n - 1) % NS;
-                float* Ow = reinterpret_cast<float*>(smem + st * S::STAGE);
+                float* Ow = reinterpret_cast<float*>(smem + last * S::STAGE);
                 rows.sum_lanes();
                 if (g4 == 0) {
                     mw[warp * 8 + 2 * t4] = rows.m[0]; mw[warp * 8 + 2 * t4 + 1] = rows.m[1];
@@ -662,7 +672,7 @@ attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int h = 2 * t4 + e;
-                    const Common c = common_of(mw, lw, h, rows.m[e], rows.M[e]);
+                    const Common c = common_of(mw, lw, h, rows.M[e]);
                     const float f = !whole ? c.factor : c.sum == 0.f ? 0.f : c.factor / c.sum;
                     if (!whole && warp == 0 && g4 == 0 && h < rep) *reinterpret_cast<float2*>(scratch_ml + (part * rep + h) * 2) = make_float2(c.top, c.sum);
                     float* row = Ow + (warp * 8 + h) * D + 2 * g4;
@@ -685,9 +695,8 @@ attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the next page comes by TMA where these numbers are
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
+                if (lane == 0) mbar_arrive(bar0 + 16 * last + 8);
             }
-            it += n;
             left -= n;
             if (left <= 0) break;
             p = 0;
@@ -722,7 +731,7 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
     const long long u = (long long)ahead * G + (long long)g * n;
     const int c0 = sh.owner(u), c1 = sh.owner(u + n - 1);
     if (c0 == c1) return;
-    float top = -INFINITY, sum = 0.f, o[V] = {};
+    float top = NONE, sum = 0.f, o[V] = {};
     for (int c = c0 + warp; c <= c1; c += 16) {
         float2 ml[4];
         float x[4][V];
@@ -731,22 +740,21 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
             const int part = min(c + 4 * k, c1);                  // (past the end: the last one again, with no weight)
             const size_t at = (2 * (size_t)part + (part == c0)) * rep + h;
             ml[k] = *reinterpret_cast<const float2*>(scratch_ml + at * 2);
-            if (c + 4 * k > c1) ml[k] = make_float2(-INFINITY, 0.f);
+            if (c + 4 * k > c1) ml[k] = make_float2(NONE, 0.f);
 #pragma unroll
             for (int v = 0; v < V; v++) x[k][v] = scratch_o[at * D + lane + 32 * v];
         }
         float now = top;
 #pragma unroll
         for (int k = 0; k < 4; k++) now = fmaxf(now, ml[k].x);
-        const float down = top == -INFINITY ? 0.f : exp2f(top - now);
+        const float down = power2(top - now);
         top = now;
         sum *= down;
 #pragma unroll
         for (int v = 0; v < V; v++) o[v] *= down;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (ml[k].x == -INFINITY) continue;
-            const float w = exp2f(ml[k].x - now);
+            const float w = c + 4 * k <= c1 ? power2(ml[k].x - now) : 0.f;
             sum = fmaf(ml[k].y, w, sum);
 #pragma unroll
             for (int v = 0; v < V; v++) o[v] = fmaf(x[k][v], w, o[v]);
@@ -760,7 +768,7 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
     float total = 0.f, w[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        w[k] = refs[k][0] == -INFINITY ? 0.f : exp2f(refs[k][0] - all);
+        w[k] = power2(refs[k][0] - all);
         total = fmaf(refs[k][1], w[k], total);
     }
     for (int dim = threadIdx.x; dim < D; dim += 128) {
@@ -769,6 +777,649 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
         for (int k = 0; k < 4; k++) y = fmaf(sums[k][dim], w[k], y);
         out[((size_t)t * H + head) * D + dim] = __float2bfloat16_rn(total == 0.f ? 0.f : y / total);
     }
+}
+
+// ---- runs of new tokens on tcgen05: head sizes 64 and 128, pages of 64 ----------------------------------------------------------------
+// A work item is two tiles of 128 rows, a row being (token, head of the group): 2 TQ consecutive tokens of one sequence and key head, TQ = 128 / (heads per
+// group), against the item's keys, or one of `splits` equal parts of them where items are few.  Blocks are persistent, one per SM.  Per 128 keys:
+//
+//   converters (4 warps)    the integers of K and V from the cache through registers into shared memory as float16 (`pair`, exact), with the 128-byte swizzle
+//                           the tensor cores read; the scales beside them
+//   MMA (one thread)        S = Q K^T (128 x 128, A and B from shared memory) and O += W V (W from tensor memory, V as it lies, [key][dim]); the pipe
+//                           alternates between the two tiles, so one's softmax runs under the other's products
+//   softmax (4 warps per tile, a row per thread)   s = S ks unit;  p = 2^(s - M + LIFT), l += p;  W = p vs as float16, over the first half of its own scores
+//
+// The arithmetic is the single-token kernel's: queries as float16 times a power of two per row, W rounded once, M the reference of weights times scales, which
+// follows their maximum in steps of 2^3 or more.  Here the sum has the same reference (p stays below 2^105 for scales from 2^-90 up).  M counts the largest
+// scale of the 128 keys for each of them; where the scales of 128 keys differ by more than 2^8 it is worked out key by key.
+// The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
+//
+// What bounds it: the exponentials and the seven other operations per score of the softmax warps beside a tensor pipe that is busy TODO.
+constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
+constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
+constexpr int PROMPT_THREADS = 512;
+constexpr float PROMPT_LEAST_LOG = -90.f, WIDE_LOG = 8.f, ABSENT = 1e30f;
+
+struct PromptBars {
+    unsigned long long q_full[2], q_empty[2];
+    unsigned long long k_full[KV_STAGES], k_empty[KV_STAGES], v_full[KV_STAGES], v_empty[KV_STAGES];
+    unsigned long long sc_full[SC_STAGES];
+    unsigned long long s_full[2], p_ready[2], pv_done[2];
+    uint32_t tmem_base;
+    int gave_up;
+};
+struct Scales {
+    float k[KEYS], v[KEYS];
+    float most[4], least[4];                 // log2 of the values' scales, per converter warp
+};
+template <int D>
+struct PromptSmem {
+    static constexpr int TILE = (D / 64) * HALF_BYTES;
+    static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, BARS = SC + SC_STAGES * (int)sizeof(Scales);
+    static constexpr int BYTES = 1024 + BARS + (int)sizeof(PromptBars);
+};
+
+// K-major operand tile with 128-byte swizzle (rows of 128 bytes, 8-row groups 1024 bytes apart)
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// MN-major: rows are keys, 64 dims per 128-byte row; the next 64 dims one half tile further (leading offset)
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(HALF_BYTES >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// float16 x float16 -> 32-bit
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major) {
+    return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+// The same load without the wait, and the wait as a separate step that names the registers, so that the compiler
+// keeps every use of them behind it: several loads can then be in flight before one wait.
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+          "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+          "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+          "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+        :: "memory");
+}
+// a whole row of 128 scores: four loads in flight, then the wait
+__device__ __forceinline__ void tmem_ld_row128(uint32_t taddr, float (*v)[32]) {
+    uint32_t r[4][32];
+#pragma unroll
+    for (int c = 0; c < 4; c++) tmem_ld32_issue(taddr + c * 32, r[c]);
+#pragma unroll
+    for (int c = 0; c < 4; c++) tmem_ld_wait32(r[c]);
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[c][i] = __uint_as_float(r[c][i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr),
+          "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+          "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+          "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+          "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15])),
+          "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])), "r"(__float_as_uint(v[18])), "r"(__float_as_uint(v[19])),
+          "r"(__float_as_uint(v[20])), "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])), "r"(__float_as_uint(v[23])),
+          "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])), "r"(__float_as_uint(v[27])),
+          "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])), "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// two 32-bit numbers per instruction
+__device__ __forceinline__ uint64_t both(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// One work item; the same for every warp of a block.
+struct PromptItem {
+    int g, z, seq, slot, t0;                 // key head, part of the keys, sequence, its slot, the first tile's first token
+    int nq[2], pos0[2], lo[2], hi[2];        // per tile: tokens, first position, key blocks [lo, hi)
+    int blk0, n, last_pos;                   // the item's key blocks, the last position any row sees
+    // items are ordered from a sequence's last tiles (most keys) to its first, heads next to each other; false: no such item
+    __device__ __forceinline__ bool set(const GfbBatch& b, int w, int n_x, int G, int splits, int TQ, int window) {
+        const int xz = w / G, xi = xz / splits;
+        g = w - xz * G;
+        z = xz - xi * splits;
+        int left = n_x - 1 - xi, at = 0, qlen = 0;
+        for (seq = 0; seq < b.n_seqs; seq++) {
+            at = b.cu_seqlens[seq];
+            qlen = b.cu_seqlens[seq + 1] - at;
+            const int nt = (qlen + 2 * TQ - 1) / (2 * TQ);
+            if (left < nt) break;
+            left -= nt;
+        }
+        if (seq == b.n_seqs) return false;
+        slot = b.slots[seq];
+        const int tq0 = left * 2 * TQ, len0 = b.lengths[slot];
+        t0 = at + tq0;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            nq[x] = max(0, min(TQ, qlen - (tq0 + x * TQ)));
+            pos0[x] = len0 + tq0 + x * TQ;
+            lo[x] = hi[x] = 0;
+            if (nq[x] > 0) {
+                lo[x] = (window > 0 ? max(0, pos0[x] - window + 1) : 0) / KEYS;
+                hi[x] = (pos0[x] + nq[x] - 1) / KEYS + 1;
+            }
+        }
+        last_pos = pos0[0] + nq[0] + nq[1] - 1;
+        const int all = max(hi[0], hi[1]) - lo[0], per = (all + splits - 1) / splits;     // (the second tile's keys begin no earlier)
+        blk0 = lo[0] + z * per;
+        n = max(0, min(per, all - z * per));
+        return true;
+    }
+    __device__ __forceinline__ bool active(int x, int j) const { return blk0 + j >= lo[x] && blk0 + j < hi[x]; }
+};
+// The items are sorted by weight, so blocks take them in a snake: P ascending, P descending, ...
+__device__ __forceinline__ int snake_item(int pass, int block, int P) { return pass * P + ((pass & 1) ? P - 1 - block : block); }
+
+// What a softmax thread keeps of its row.
+template <int D>
+struct PromptRow {
+    float unit;                              // of S times a key's scale, log2(e) in it
+    // The row's query into the tile at `tile` (shared memory), as float16 times a power of two; zeros where there is none.
+    __device__ __forceinline__ void put_query(uint8_t* tile, int r, const __nv_bfloat16* src, float scale_log2e) {
+        uint4 v[D / 8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) {
+            v[i] = src != nullptr ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+        }
+        const int e = min(max((int)(top >> 7) - 127, -100), 100);
+        const float lift = exp2f((float)(14 - e));
+        unit = exp2f((float)(e - 14)) * scale_log2e;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                const float f0 = __uint_as_float(w[k] << 16) * lift, f1 = __uint_as_float(w[k] & 0xffff0000u) * lift;
+                const float f2 = __uint_as_float(w[k + 1] << 16) * lift, f3 = __uint_as_float(w[k + 1] & 0xffff0000u) * lift;
+                o[k] = pack2_f16(f0, f2);
+                o[k + 1] = pack2_f16(f1, f3);
+            }
+            *reinterpret_cast<uint4*>(tile + (i >> 3) * HALF_BYTES + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+};
+
+// q [T, H, D], out [T, H * D]; with splits > 1 instead scratch_o [T, H, splits, D] and scratch_ml [T, H, splits, 2] (M, l).
+template <int D>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* scratch_o, float* scratch_ml, Int8KV kv, GfbBatch b, int H, int G, float scale_log2e,
+                             int window, int splits, int n_x, int n_items, int* status) {
+    using S = PromptSmem<D>;
+    constexpr int TILE = S::TILE;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+    Scales* scales = reinterpret_cast<Scales*>(smem + S::SC);
+    PromptBars* bars = reinterpret_cast<PromptBars*>(smem + S::BARS);
+    volatile int* gave_up = &bars->gave_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rep = H / G, TQ = ROWS / rep, P = gridDim.x;
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < 2; x++) {
+            mbar_init(smem_u32(&bars->q_full[x]), 4);
+            mbar_init(smem_u32(&bars->q_empty[x]), 1);
+            mbar_init(smem_u32(&bars->s_full[x]), 1);
+            mbar_init(smem_u32(&bars->p_ready[x]), 4);
+            mbar_init(smem_u32(&bars->pv_done[x]), 1);
+        }
+        for (int s = 0; s < KV_STAGES; s++) {
+            mbar_init(smem_u32(&bars->k_full[s]), 4);
+            mbar_init(smem_u32(&bars->k_empty[s]), 1);
+            mbar_init(smem_u32(&bars->v_full[s]), 4);
+            mbar_init(smem_u32(&bars->v_empty[s]), 1);
+        }
+        for (int s = 0; s < SC_STAGES; s++) mbar_init(smem_u32(&bars->sc_full[s]), 4);
+        bars->gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+    gfb_pdl_launch();
+    gfb_pdl_wait();
+
+    // Registers per thread: 72 + 40 + 200 + 200 for the four warpgroups, 512 together, which is what 512 threads of 128 came with.
+    PromptItem it;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- converters: a warp has 32 keys of the 128, half of one page; a lane 16 bytes of a row at a time
+        constexpr int CH = D / 16, RPI = 32 / CH, LOADS = 32 / RPI;      // 16-byte chunks of a row, rows per load of a warp, loads
+        const int row0 = warp * 32 + lane / CH, c = lane % CH;
+        int gj = 0;                                                      // key blocks so far
+        bool ok = true;
+        for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
+            if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
+            const int* pt = kv.page_table + (size_t)it.slot * kv.max_pages;
+            const int last_page = it.last_pos / PAGE;
+            for (int j = 0; j < it.n && ok; j++, gj++) {
+                const int s = gj % KV_STAGES, sc = gj % SC_STAGES;
+                const uint32_t empty = ((uint32_t)(gj / KV_STAGES) & 1u) ^ 1u;
+                const int pi = (it.blk0 + j) * 2 + (warp >> 1);
+                int page = -1;
+                if (pi <= last_page) {
+                    page = pi < kv.max_pages ? pt[pi] : -1;
+                    if (page < 0 || page >= kv.n_pages) {
+                        if (lane == 0) gfb_report(status, GFB_ERR_PAGE_TABLE, it.slot, pi);
+                        page = -1;
+                    }
+                }
+                const size_t first = ((size_t)max(page, 0) * G + it.g) * PAGE + (warp & 1) * 32;      // the warp's first row in the pools
+                auto fetch = [&](const int8_t* pool, uint4 (&v)[LOADS]) {
+#pragma unroll
+                    for (int i = 0; i < LOADS; i++)
+                        v[i] = page >= 0 ? *reinterpret_cast<const uint4*>(pool + (first + i * RPI + lane / CH) * D + c * 16) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                };
+                auto store = [&](uint8_t* tile, const uint4 (&v)[LOADS]) {
+#pragma unroll
+                    for (int i = 0; i < LOADS; i++) {
+                        const int r = row0 + i * RPI;
+                        uint8_t* line = tile + (c >> 2) * HALF_BYTES + r * 128;
+                        const uint4 a = make_uint4(pair(v[i].x), pair(v[i].x >> 8), pair(v[i].y), pair(v[i].y >> 8));
+                        const uint4 d = make_uint4(pair(v[i].z), pair(v[i].z >> 8), pair(v[i].w), pair(v[i].w >> 8));
+                        // lanes of the second 64 dims write their two halves in the other order, so that the eight lanes of a row meet eight bank groups
+                        const int swap = (c >> 2) & 1, k0 = 2 * (c & 3);
+                        *reinterpret_cast<uint4*>(line + (((k0 + swap) ^ (r & 7)) << 4)) = swap ? d : a;
+                        *reinterpret_cast<uint4*>(line + (((k0 + 1 - swap) ^ (r & 7)) << 4)) = swap ? a : d;
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor cores read it
+                    __syncwarp();
+                };
+                uint4 v[LOADS];
+                fetch(kv.k_pool, v);
+                const int key = (it.blk0 + j) * KEYS + warp * 32 + lane;
+                const bool here = page >= 0 && key <= it.last_pos;
+                const float k_scale = here ? kv.k_scale[first + lane] : 0.f, v_scale = here ? kv.v_scale[first + lane] : 0.f;
+                ok = mbar_wait_warp(smem_u32(&bars->k_empty[s]), empty, gave_up, status, 401);
+                if (!ok) break;
+                scales[sc].k[warp * 32 + lane] = k_scale;
+                scales[sc].v[warp * 32 + lane] = v_scale;
+                const float lv = fmaxf(log2f(v_scale), PROMPT_LEAST_LOG);
+                const float most = gfb_warp_max(here ? lv : -ABSENT), least = -gfb_warp_max(here ? -lv : -ABSENT);
+                if (lane == 0) {
+                    scales[sc].most[warp] = most;
+                    scales[sc].least[warp] = least;
+                }
+                store(smem + S::K + s * TILE, v);
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&bars->sc_full[sc]));
+                    mbar_arrive(smem_u32(&bars->k_full[s]));
+                }
+                fetch(kv.v_pool, v);
+                ok = mbar_wait_warp(smem_u32(&bars->v_empty[s]), empty, gave_up, status, 402);
+                if (!ok) break;
+                store(smem + S::V + s * TILE, v);
+                if (lane == 0) mbar_arrive(smem_u32(&bars->v_full[s]));
+            }
+        }
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 4 && lane == 0) {
+            constexpr uint32_t idesc_s = idesc_f16(ROWS, KEYS, 0), idesc_o = idesc_f16(ROWS, D, 1);
+            uint32_t n_pv[2] = {0, 0}, n_item = 0;                       // products W V issued per tile, items with keys
+            int g0 = 0;                                                  // key blocks ahead of the item
+            bool ok = true;
+            for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
+                if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window) || it.n == 0) continue;
+                for (int x = 0; x < 2 && ok; x++) ok = mbar_wait(smem_u32(&bars->q_full[x]), n_item & 1u, gave_up, status, 403);
+                n_item++;
+                uint32_t mine[2] = {0, 0};                               // of this item
+                auto issue_s = [&](int x, int j) {
+                    const uint32_t kt = base + S::K + ((g0 + j) % KV_STAGES) * TILE;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t off = (k >> 2) * HALF_BYTES;
+                        umma_ss(tmem + 128 * x, desc_kmajor(base + x * TILE + off) + 2 * (k & 3), desc_kmajor(kt + off) + 2 * (k & 3), idesc_s, k != 0);
+                    }
+                    umma_commit(smem_u32(&bars->s_full[x]));
+                };
+                auto k_ready = [&](int j) {
+                    return mbar_wait(smem_u32(&bars->k_full[(g0 + j) % KV_STAGES]), (uint32_t)((g0 + j) / KV_STAGES) & 1u, gave_up, status, 404);
+                };
+                auto scores_issued = [&](int j) {                        // K of block j is free when they are done, and behind the last block Q is
+                    umma_commit(smem_u32(&bars->k_empty[(g0 + j) % KV_STAGES]));
+                    if (j + 1 == it.n) {
+                        umma_commit(smem_u32(&bars->q_empty[0]));
+                        umma_commit(smem_u32(&bars->q_empty[1]));
+                    }
+                };
+                if (ok) ok = k_ready(0);
+                if (ok) {
+                    tc_fence_after();
+                    if (it.active(0, 0)) issue_s(0, 0);
+                    if (it.active(1, 0)) issue_s(1, 0);
+                    scores_issued(0);
+                }
+                for (int j = 0; j < it.n && ok; j++) {
+                    const int s = (g0 + j) % KV_STAGES;
+                    bool k_next = false;                                 // whether K of block j + 1 has been waited for
+                    ok = mbar_wait(smem_u32(&bars->v_full[s]), (uint32_t)((g0 + j) / KV_STAGES) & 1u, gave_up, status, 405);
+#pragma unroll
+                    for (int x = 0; x < 2 && ok; x++) {
+                        if (it.active(x, j)) {
+                            ok = mbar_wait(smem_u32(&bars->p_ready[x]), n_pv[x] & 1u, gave_up, status, 406);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int kk = 0; kk < 8; kk++)               // 16 keys per MMA: 8 columns of W, 2 KB of V
+                                umma_ts(tmem + 256 + 128 * x, tmem + 128 * x + kk * 8, desc_mnmajor(base + S::V + s * TILE + kk * 2048), idesc_o,
+                                        (mine[x] | (uint32_t)kk) != 0);
+                            umma_commit(smem_u32(&bars->pv_done[x]));
+                            n_pv[x]++;
+                            mine[x]++;
+                        }
+                        if (j + 1 < it.n && it.active(x, j + 1)) {       // the tile's next scores, behind its W V
+                            if (!k_next) { ok = k_ready(j + 1); k_next = true; if (!ok) break; tc_fence_after(); }
+                            issue_s(x, j + 1);
+                        }
+                    }
+                    if (!ok) break;
+                    umma_commit(smem_u32(&bars->v_empty[s]));
+                    if (j + 1 < it.n) {
+                        if (!k_next) { ok = k_ready(j + 1); if (!ok) break; }
+                        scores_issued(j + 1);
+                    }
+                }
+                g0 += it.n;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int x = (warp - 8) >> 2, w4 = warp & 3, r = w4 * 32 + lane, tq = r / rep;      // tile, the warp's 32 lanes of tensor memory, row, its token
+        const uint32_t lanes = tmem + ((uint32_t)(w4 * 32) << 16), col_s = lanes + 128 * x, col_o = lanes + 256 + 128 * x;
+        uint8_t* tile = smem + x * TILE;
+        PromptRow<D> row;
+        uint32_t n_item = 0;                                             // items with keys so far
+        auto ask = [&](const PromptItem& i) -> bool {                    // the item's queries into shared memory
+            if (!mbar_wait_warp(smem_u32(&bars->q_empty[x]), (n_item++ & 1u) ^ 1u, gave_up, status, 411)) return false;
+            const bool mine = tq < i.nq[x];
+            row.put_query(tile, r, mine ? q + ((size_t)(i.t0 + x * TQ + tq) * H + i.g * rep + (r - tq * rep)) * D : nullptr, scale_log2e);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars->q_full[x]));
+            return true;
+        };
+        int g0 = 0;
+        uint32_t n_done = 0;                                             // this tile's blocks so far
+        bool ok = true;
+        for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
+            if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
+            if (it.n > 0 && !ask(it)) break;
+            const bool row_ok = tq < it.nq[x];
+            const int row_pos = it.pos0[x] + tq, row_lo = window > 0 ? max(0, row_pos - window + 1) : 0;
+            const int last_lo = window > 0 ? max(0, it.pos0[x] + max(it.nq[x], 1) - window) : 0;
+            float M = NONE, l = 0.f;
+            uint32_t here = 0;                                           // blocks of this item
+            for (int j = 0; j < it.n && ok; j++) {
+                if (!it.active(x, j)) continue;
+                const int key0 = (it.blk0 + j) * KEYS;
+                const Scales& sc = scales[(g0 + j) % SC_STAGES];
+                ok = mbar_wait_warp(smem_u32(&bars->sc_full[(g0 + j) % SC_STAGES]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
+                     && mbar_wait_warp(smem_u32(&bars->s_full[x]), n_done & 1u, gave_up, status, 408);
+                if (!ok) break;
+                tc_fence_after();
+                const bool need_mask = key0 + KEYS - 1 > it.pos0[x] || key0 < last_lo;
+                float v[4][32];
+                tmem_ld_row128(col_s, v);
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 k = *reinterpret_cast<const float4*>(sc.k + c * 32 + i);
+                        apart(mul2(both(v[c][i], v[c][i + 1]), both(k.x, k.y)), v[c][i], v[c][i + 1]);
+                        apart(mul2(both(v[c][i + 2], v[c][i + 3]), both(k.z, k.w)), v[c][i + 2], v[c][i + 3]);
+                    }
+                if (need_mask) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const int kj = key0 + c * 32 + i;
+                            if (!(kj <= row_pos && kj >= row_lo)) v[c][i] = -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (sc.most[c] == -ABSENT) {                         // none of these 32 keys exists (uniform, and rare)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[c][i] = -INFINITY;
+                    }
+                float mx = -INFINITY;
+                const float4 most4 = *reinterpret_cast<const float4*>(sc.most), least4 = *reinterpret_cast<const float4*>(sc.least);
+                const float most = fmaxf(fmaxf(most4.x, most4.y), fmaxf(most4.z, most4.w)), least = fminf(fminf(least4.x, least4.y), fminf(least4.z, least4.w));
+                float y;                                                 // at least the largest of score + log2 of the value's scale
+                if (most - least <= WIDE_LOG) {                          // uniform
+                    float mx4[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        mx4[c] = fmaxf(v[c][0], v[c][1]);
+#pragma unroll
+                        for (int i = 2; i < 32; i += 2) mx4[c] = max3(mx4[c], v[c][i], v[c][i + 1]);
+                    }
+                    mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                    y = fmaf(mx, row.unit, most);
+                } else {
+                    y = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) y = fmaxf(y, fmaf(v[c][i], row.unit, fmaxf(log2f(sc.v[c * 32 + i]), PROMPT_LEAST_LOG)));
+                }
+                const float M_new = y > M + (15.f - LIFT) ? y : M;
+                const float corr = power2(M - M_new);
+                const uint64_t unit2 = both(row.unit, row.unit), off2 = both(LIFT - M_new, LIFT - M_new);
+                uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 vs = *reinterpret_cast<const float4*>(sc.v + c * 32 + i);
+                        float t0, t1, t2, t3;
+                        apart(fma2(both(v[c][i], v[c][i + 1]), unit2, off2), t0, t1);
+                        apart(fma2(both(v[c][i + 2], v[c][i + 3]), unit2, off2), t2, t3);
+                        const uint64_t p01 = both(power2(t0), power2(t1)), p23 = both(power2(t2), power2(t3));
+                        sum[0] = add2(sum[0], p01);
+                        sum[1] = add2(sum[1], p23);
+                        float w0, w1, w2, w3;
+                        apart(mul2(p01, both(vs.x, vs.y)), w0, w1);
+                        apart(mul2(p23, both(vs.z, vs.w)), w2, w3);
+                        if (need_mask) {                                 // an unseen key's value scale can be anything
+                            const int kj = key0 + c * 32 + i;
+                            if (!(kj <= row_pos && kj >= row_lo)) w0 = 0.f;
+                            if (!(kj + 1 <= row_pos && kj + 1 >= row_lo)) w1 = 0.f;
+                            if (!(kj + 2 <= row_pos && kj + 2 >= row_lo)) w2 = 0.f;
+                            if (!(kj + 3 <= row_pos && kj + 3 >= row_lo)) w3 = 0.f;
+                        }
+                        pk[i >> 1] = pack2_f16(w0, w1);
+                        pk[(i >> 1) + 1] = pack2_f16(w2, w3);
+                    }
+                    tmem_st16(col_s + c * 16, pk);
+                }
+                // O follows the reference, rarely (S of this block was issued behind the tile's previous W V, so that phase is over)
+                if (here > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                    ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        float o[32];
+                        tmem_ld32(col_o + c * 32, o);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] *= corr;
+                        tmem_st32(col_o + c * 32, o);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&bars->p_ready[x]));
+                float s0, s1, s2, s3;
+                apart(sum[0], s0, s1);
+                apart(sum[1], s2, s3);
+                l = l * corr + ((s0 + s1) + (s2 + s3));
+                M = M_new;
+                n_done++;
+                here++;
+            }
+            if (ok && here > 0) ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
+            if (ok) {
+                tc_fence_after();
+                const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
+                const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                if (splits > 1 && row_ok) *reinterpret_cast<float2*>(scratch_ml + (at * splits + it.z) * 2) = make_float2(here > 0 ? M : NONE, here > 0 ? l : 0.f);
+#pragma unroll 1
+                for (int c = 0; c < D / 32; c++) {
+                    if (here == 0 && splits > 1) break;                  // nothing of this row in this part: its (M, l) say so
+                    float o[32];
+                    if (here > 0) tmem_ld32(col_o + c * 32, o);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = 0.f;
+                    }
+                    if (!row_ok) continue;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {                    // dims 0, 2, 1, 3 of every four
+                        if (splits > 1) {
+                            float* dst = scratch_o + (at * splits + it.z) * D + c * 32 + i;
+                            *reinterpret_cast<float4*>(dst) = make_float4(o[i], o[i + 2], o[i + 1], o[i + 3]);
+                            *reinterpret_cast<float4*>(dst + 4) = make_float4(o[i + 4], o[i + 6], o[i + 5], o[i + 7]);
+                        } else {
+                            *reinterpret_cast<uint4*>(out + at * D + c * 32 + i) =
+                                make_uint4(pack2(o[i] * inv, o[i + 2] * inv), pack2(o[i + 1] * inv, o[i + 3] * inv),
+                                           pack2(o[i + 4] * inv, o[i + 6] * inv), pack2(o[i + 5] * inv, o[i + 7] * inv));
+                        }
+                    }
+                }
+                tc_fence_before();
+            }
+            g0 += it.n;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*gave_up) {
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 50000ull) __nanosleep(1000);
+    }
+    if (warp == 4) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// The parts of a row, merged in ascending order: a warp per (token, head).
+template <int D>
+__global__ void __launch_bounds__(128)
+attention_int8_parts_kernel(const float* scratch_o, const float* scratch_ml, __nv_bfloat16* out, long rows, int splits) {
+    constexpr int V = D / 32;
+    gfb_pdl_launch();
+    gfb_pdl_wait();
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    float top = NONE, sum = 0.f, o[V] = {};
+    for (int k = 0; k < splits; k++) {
+        const float2 ml = *reinterpret_cast<const float2*>(scratch_ml + (row * splits + k) * 2);
+        if (ml.x == NONE) continue;                                      // a part without a key of the row has written nothing
+        const float now = fmaxf(top, ml.x), down = power2(top - now), w = power2(ml.x - now);
+        const float* x = scratch_o + (row * splits + k) * D + lane * V;
+        top = now;
+        sum = sum * down + ml.y * w;
+#pragma unroll
+        for (int v = 0; v < V; v++) o[v] = fmaf(x[v], w, o[v] * down);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(out + row * D + lane * V + v) = pack2(o[v] * inv, o[v + 1] * inv);
 }
 
 // ---- host side ----------------------------------------------------------------------------
@@ -861,6 +1512,27 @@ int launch_shares(const Decode& a, int blocks, float* scratch) {
                                 (__nv_bfloat16*)a.out, a.b.n_tokens, a.H, a.G, blocks), "gfb_attention_int8_decode (merge)");
 }
 
+template <int D>
+int launch_prompt(const Decode& a, int n_x, int splits, float* scratch) {
+    auto kern = attention_int8_prompt_kernel<D>;
+    const size_t smem = PromptSmem<D>::BYTES;
+    static bool configured[MAX_DEVICES] = {};
+    if (room(kern, smem, configured)) return 1;
+    int dev = 0, sms = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const long items = (long)n_x * a.G * splits;
+    if (items > 0x3fffffffL) return gfb_fail("gfb_attention_int8_prompt: %ld work items", items);
+    const long rows = (long)a.b.n_tokens * a.H;
+    float* ml = scratch ? scratch + rows * splits * D : nullptr;
+    if (gfb_check(gfb_launch(kern, dim3((unsigned)(items < sms ? items : sms)), dim3(PROMPT_THREADS), smem, a.stream, (const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out,
+                             scratch, ml, a.kv, a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, splits, n_x, (int)items, a.status),
+                  "gfb_attention_int8_prompt")) return 1;
+    if (splits == 1) return 0;
+    return gfb_check(gfb_launch(attention_int8_parts_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, a.stream, (const float*)scratch, (const float*)ml,
+                                (__nv_bfloat16*)a.out, rows, splits), "gfb_attention_int8_prompt (parts)");
+}
+
 }  // namespace
 
 // One new token per sequence, bfloat16, d 64 or 128, pages of 64, at most 8 heads per key head.  Without scratch each sequence in `splits` equal slices (1 to 8),
@@ -879,6 +1551,25 @@ GFB_API int gfb_attention_int8_decode(const void* q, void* out, const void* k_po
                    {cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens}, H, G, scale, window, status, stream};
     if (scratch != nullptr) return d == 128 ? launch_shares<128, 3>(a, blocks, scratch) : launch_shares<64, 6>(a, blocks, scratch);
     return d == 128 ? launch_decode<128, 3>(a, splits) : launch_decode<64, 6>(a, splits);
+}
+
+// Any number of new tokens per sequence, bfloat16, d 64 or 128, pages of 64, at most 128 heads per key head, scale > 0.  n_x: at least the tile pairs there are,
+// sum over sequences of ceil(new tokens / (2 floor(128 / (H / G)))).  splits > 1: every pair's keys in that many parts, which merge through scratch (float32
+// [n_tokens * H * splits * (d + 2)]).
+GFB_API int gfb_attention_int8_prompt(const void* q, void* out, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                                      const int* page_table, int max_pages, int page_size, int n_pages,
+                                      const int* cu_seqlens, const int* tok_seq, const int* slots, const int* lengths, int n_seqs, int n_tokens,
+                                      int H, int G, int d, float scale, int window, int n_x, int splits, float* scratch, int* status, cudaStream_t stream) {
+    if (n_tokens <= 0 || n_seqs <= 0) return 0;
+    if ((d != 64 && d != 128) || page_size != PAGE) return gfb_fail("gfb_attention_int8_prompt: heads of %d, pages of %d", d, page_size);
+    if (G <= 0 || H % G || H / G > ROWS) return gfb_fail("gfb_attention_int8_prompt: %d heads over %d", H, G);
+    if (!(scale > 0.f)) return gfb_fail("gfb_attention_int8_prompt: a scale of %g (the maximum is taken of unscaled scores)", (double)scale);
+    if (splits < 1 || splits > 64 || (splits > 1 && scratch == nullptr) || n_x < 1) return gfb_fail("gfb_attention_int8_prompt: %d parts, %d pairs of tiles", splits, n_x);
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch) & 15)
+        return gfb_fail("gfb_attention_int8_prompt: everything must be 16-byte aligned");
+    const Decode a{q, out, {(const int8_t*)k_pool, (const int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages},
+                   {cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens}, H, G, scale, window, status, stream};
+    return d == 128 ? launch_prompt<128>(a, n_x, splits, splits > 1 ? scratch : nullptr) : launch_prompt<64>(a, n_x, splits, splits > 1 ? scratch : nullptr);
 }
 
 // q [T, H, d] and out [T, H * d] of type dt.  Any d up to 512, any page size.

@@ -1,6 +1,7 @@
 """ctypes bindings of the kernel libraries: host-side checks, kernel choice,
 launch on the current stream."""
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -161,13 +162,43 @@ def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
     return bn, splits, max(2, min(8, 102400 // (16384 + bn * 128)))
 
 
+@functools.lru_cache(maxsize=4096)
 def int8_shares(max_kv_len: int, page_size: int, pairs: int, sm_count: int):
     """(slices, blocks) of a decode step over a cache of 8-bit integers, `pairs` (token, key head) pairs of sequences of at most max_kv_len tokens.  blocks 0: every
-    pair in that many equal slices, a cluster of at most 8 blocks; otherwise all pages in equal shares for that many blocks."""
-    pages = -(-max(max_kv_len, 1) // page_size)
-    if pairs * pages > 4 * sm_count * 4:
-        return 1, 4 * sm_count
-    return max(1, min(8, pages // 2, 4 * sm_count // max(pairs, 1))), 0
+    pair in that many equal slices, a cluster of at most 8 blocks; otherwise all pages in equal shares for that many blocks.
+
+    A cost model in us fitted to measurements on a B200 (heads of 128; 1 to 600 sequences of 100 to 100,000 tokens, equal and ragged): four blocks share an SM; a
+    page takes a block 0.6 us alone, 1.5 us where four share the SM, which is then what memory gives; a block 2 us besides.  Shares cost a merge behind them and
+    2.85 ns a page.  The step knows the longest sequence only, and shares gain where others are shorter, so they win from 10 % behind (20 % where the longest has
+    6,000 tokens).  us in slices | in
+    shares: one sequence of 911 6 | 11, of 30,000 42 | 25; 8 of 4,000 20 | 25; 32 of 4,000 53 | 57, of 300 to 4,000 44 | 39; 64 of 501 to 8,190 124 | 106;
+    128 of 2,000 87 | 105."""
+    pages, at_once = -(-max(max_kv_len, 1) // page_size), 4 * sm_count
+    best, best_cost = 1, None
+    for s in range(1, min(8, pages) + 1):
+        blocks = pairs * s
+        page = max(0.6, min(1.5, 0.433 * blocks / sm_count))
+        cost = 3.5 + max(1.0, blocks / at_once) * (2.0 + -(-pages // s) * page)
+        if best_cost is None or cost < best_cost - 1e-9:
+            best, best_cost = s, cost
+    if (0.8 if pages >= 96 else 0.9) * (12.0 + 2.85e-3 * pairs * pages) < best_cost:
+        return 1, at_once
+    return best, 0
+
+
+@functools.lru_cache(maxsize=4096)
+def int8_parts(n_tokens: int, n_seqs: int, max_kv_len: int, rep: int, n_kv: int, sm_count: int):
+    """(pairs of tiles, parts of their keys) of a prompt's attention over a cache of 8-bit integers: how many pairs of tiles of 128 // rep tokens there are at
+    most, and into how many parts each pair's keys are cut.  A block per SM works on a part at a time, about 2 us per 128 keys and 4 such besides; the parts of
+    a row are 4 d bytes each, written and read again."""
+    two = 2 * (128 // rep)
+    pairs = (n_tokens + n_seqs * (two - 1)) // two
+    blocks, best, best_cost = -(-max_kv_len // 128), 1, None
+    for s in range(1, max(1, min(16, blocks // 4)) + 1):
+        cost = -(-pairs * n_kv * s // sm_count) * (-(-blocks // s) + 4) * 2.0 + (4.0 + n_tokens * n_kv * rep * s * 2.5e-4 if s > 1 else 0.0)
+        if best_cost is None or cost < best_cost - 1e-9:
+            best, best_cost = s, cost
+    return pairs, best
 
 
 def rows_share_keys(rows: int, longest: int, max_kv_len: int, line: int, blocks: Optional[int] = None) -> bool:
@@ -1434,9 +1465,15 @@ class CudaKernels:
         args = (*self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch), n_head, n_kv, head_dim, scale, window or 0)
         if q.dtype == torch.bfloat16 and batch.max_q_len == 1 and head_dim in (64, 128) and kv.page_size == 64 and n_head // n_kv <= 8:
             reach = batch.max_kv_len if not window else min(batch.max_kv_len, window + kv.page_size)
-            splits, blocks = int8_shares(reach, kv.page_size, T * n_kv, self.sm_count)
+            splits, blocks = int8_shares(-(-reach // kv.page_size) * kv.page_size, kv.page_size, T * n_kv, self.sm_count)
+            if T > 4096:                          # whose pages the shares kernel does not count
+                splits, blocks = 1, 0
             scratch = torch.empty(2 * blocks * (n_head // n_kv) * (head_dim + 2) + T + 1, dtype=torch.float32, device=q.device) if blocks else None
             return self._call("attention_int8", "gfb_attention_int8_decode", _ptr(q), _ptr(out), *args, splits, blocks, _ptr(scratch), _ptr(batch.status), _stream())
+        if q.dtype == torch.bfloat16 and head_dim in (64, 128) and kv.page_size == 64 and n_head // n_kv <= 128 and scale > 0:
+            pairs, splits = int8_parts(T, batch.n_seqs, batch.max_kv_len if not window else min(batch.max_kv_len, window + 256), n_head // n_kv, n_kv, self.sm_count)
+            scratch = torch.empty(T * n_head * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+            return self._call("attention_int8", "gfb_attention_int8_prompt", _ptr(q), _ptr(out), *args, pairs, splits, _ptr(scratch), _ptr(batch.status), _stream())
         self._call("attention_int8", "gfb_attention_int8_generic", _ptr(q), _ptr(out), _dt(q), *args, _ptr(batch.status), _stream())
 
     def argmax(self, logits, out):
