@@ -783,21 +783,23 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // A work item is two tiles of 128 rows, a row being (token, head of the group): 2 TQ consecutive tokens of one sequence and key head, TQ = 128 / (heads per
 // group), against the item's keys, or one of `splits` equal parts of them where items are few.  Blocks are persistent, one per SM.  Per 128 keys:
 //
-//   converters (4 warps)    the integers of K and V from the cache through registers into shared memory as float16 (`pair`, exact), with the 128-byte swizzle
+//   converters (3 warps)    the integers of K and V from the cache through registers into shared memory as float16 (`pair`, exact), with the 128-byte swizzle
 //                           the tensor cores read; the scales beside them
 //   MMA (one thread)        S = Q K^T (128 x 128, A and B from shared memory) and O += W V (W from tensor memory, V as it lies, [key][dim]); the pipe
 //                           alternates between the two tiles, so one's softmax runs under the other's products
-//   softmax (4 warps per tile, a row per thread)   s = S ks unit;  p = 2^(s - M + LIFT), l += p;  W = p vs as float16, over the first half of its own scores
+//   softmax (8 warps per tile, two threads per row, 64 keys each)   s = S ks unit;  p = 2^(s - M + LIFT), l += p;  W = p vs as float16, over the first half of
+//                           the thread's own scores
 //
 // The arithmetic is the single-token kernel's: queries as float16 times a power of two per row, W rounded once, M the reference of weights times scales, which
 // follows their maximum in steps of 2^3 or more.  Here the sum has the same reference (p stays below 2^105 for scales from 2^-90 up).  M counts the largest
-// scale of the 128 keys for each of them; where the scales of 128 keys differ by more than 2^8 it is worked out key by key.
+// scale of the 128 keys for each of them; where the scales of 128 keys differ by more than 2^8, or one is not finite, a slower way works it out key by key.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
 //
-// What bounds it: the exponentials and the seven other operations per score of the softmax warps beside a tensor pipe that is busy TODO.
+// What bounds it: the softmax warps' instructions.  (One thread per row, 128 scores in registers, everything unrolled: 1,198 us for 512 tokens behind 32,001; the
+// MMA thread waited for its instructions to come into the cache, 400 cycles per MMA.)
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
-constexpr int PROMPT_THREADS = 512;
+constexpr int SOFT_WARPS = 16, CONV_WARPS = 3, MMA_WARP = SOFT_WARPS + CONV_WARPS, PROMPT_THREADS = 32 * (MMA_WARP + 1);     // five warps per quarter of an SM: 96 registers each
 constexpr float PROMPT_LEAST_LOG = -90.f, WIDE_LOG = 8.f, ABSENT = 1e30f;
 
 struct PromptBars {
@@ -809,13 +811,14 @@ struct PromptBars {
     int gave_up;
 };
 struct Scales {
-    float k[KEYS], v[KEYS];
-    float most[4], least[4];                 // log2 of the values' scales, per converter warp
+    float k[KEYS], v[KEYS], log_v[KEYS];     // log2 of the values' scales, at least PROMPT_LEAST_LOG
+    float most[4], least[4];                 // of them, per 32 keys (least: -ABSENT where a scale is not finite; most: -ABSENT where there is no key)
 };
 template <int D>
 struct PromptSmem {
     static constexpr int TILE = (D / 64) * HALF_BYTES;
-    static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, BARS = SC + SC_STAGES * (int)sizeof(Scales);
+    static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, ROWS_AT = SC + SC_STAGES * (int)sizeof(Scales);
+    static constexpr int BARS = ROWS_AT + 2 * 2 * ROWS * 4;
     static constexpr int BYTES = 1024 + BARS + (int)sizeof(PromptBars);
 };
 
@@ -882,18 +885,6 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
           "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
         :: "memory");
 }
-// a whole row of 128 scores: four loads in flight, then the wait
-__device__ __forceinline__ void tmem_ld_row128(uint32_t taddr, float (*v)[32]) {
-    uint32_t r[4][32];
-#pragma unroll
-    for (int c = 0; c < 4; c++) tmem_ld32_issue(taddr + c * 32, r[c]);
-#pragma unroll
-    for (int c = 0; c < 4; c++) tmem_ld_wait32(r[c]);
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int i = 0; i < 32; i++) v[c][i] = __uint_as_float(r[c][i]);
-}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -915,6 +906,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+// one column: a number per lane
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(v) : "memory");
+}
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r) :: "memory");
+    return __uint_as_float(r);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // two 32-bit numbers per instruction
@@ -988,39 +989,33 @@ struct PromptItem {
 // The items are sorted by weight, so blocks take them in a snake: P ascending, P descending, ...
 __device__ __forceinline__ int snake_item(int pass, int block, int P) { return pass * P + ((pass & 1) ? P - 1 - block : block); }
 
-// What a softmax thread keeps of its row.
+// A row's query into the tile at `tile` (shared memory) as float16 times a power of two, zeros where there is none; one thread writes the dims [first, first + n),
+// and every thread of the row gets what S times a key's scale is worth, log2(e) in it.
 template <int D>
-struct PromptRow {
-    float unit;                              // of S times a key's scale, log2(e) in it
-    // The row's query into the tile at `tile` (shared memory), as float16 times a power of two; zeros where there is none.
-    __device__ __forceinline__ void put_query(uint8_t* tile, int r, const __nv_bfloat16* src, float scale_log2e) {
-        uint4 v[D / 8];
-        uint32_t top = 0;
-#pragma unroll
+__device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bfloat16* src, float scale_log2e, int first, int n) {
+    uint32_t top = 0;
+    if (src != nullptr) {
+#pragma unroll 4
         for (int i = 0; i < D / 8; i++) {
-            v[i] = src != nullptr ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-            for (int k = 0; k < 4; k++) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-        }
-        const int e = min(max((int)(top >> 7) - 127, -100), 100);
-        const float lift = exp2f((float)(14 - e));
-        unit = exp2f((float)(e - 14)) * scale_log2e;
-#pragma unroll
-        for (int i = 0; i < D / 8; i++) {
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-                const float f0 = __uint_as_float(w[k] << 16) * lift, f1 = __uint_as_float(w[k] & 0xffff0000u) * lift;
-                const float f2 = __uint_as_float(w[k + 1] << 16) * lift, f3 = __uint_as_float(w[k + 1] & 0xffff0000u) * lift;
-                o[k] = pack2_f16(f0, f2);
-                o[k + 1] = pack2_f16(f1, f3);
-            }
-            *reinterpret_cast<uint4*>(tile + (i >> 3) * HALF_BYTES + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            const uint4 v = *reinterpret_cast<const uint4*>(src + 8 * i);
+            top = max(top, max(max(v.x & 0x7fffu, (v.x >> 16) & 0x7fffu), max(v.y & 0x7fffu, (v.y >> 16) & 0x7fffu)));
+            top = max(top, max(max(v.z & 0x7fffu, (v.z >> 16) & 0x7fffu), max(v.w & 0x7fffu, (v.w >> 16) & 0x7fffu)));
         }
     }
-};
+    const int e = min(max((int)(top >> 7) - 127, -100), 100);
+    const float lift = exp2f((float)(14 - e));
+#pragma unroll 2
+    for (int i = first / 8; i < (first + n) / 8; i++) {
+        const uint4 v = src != nullptr ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+        const float f0 = __uint_as_float(v.x << 16) * lift, f1 = __uint_as_float(v.x & 0xffff0000u) * lift;
+        const float f2 = __uint_as_float(v.y << 16) * lift, f3 = __uint_as_float(v.y & 0xffff0000u) * lift;
+        const float f4 = __uint_as_float(v.z << 16) * lift, f5 = __uint_as_float(v.z & 0xffff0000u) * lift;
+        const float f6 = __uint_as_float(v.w << 16) * lift, f7 = __uint_as_float(v.w & 0xffff0000u) * lift;
+        *reinterpret_cast<uint4*>(tile + (i >> 3) * HALF_BYTES + r * 128 + (((i & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack2_f16(f0, f2), pack2_f16(f1, f3), pack2_f16(f4, f6), pack2_f16(f5, f7));
+    }
+    return exp2f((float)(e - 14)) * scale_log2e;
+}
 
 // q [T, H, D], out [T, H * D]; with splits > 1 instead scratch_o [T, H, splits, D] and scratch_ml [T, H, splits, 2] (M, l).
 template <int D>
@@ -1039,10 +1034,10 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     const int rep = H / G, TQ = ROWS / rep, P = gridDim.x;
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; x++) {
-            mbar_init(smem_u32(&bars->q_full[x]), 4);
+            mbar_init(smem_u32(&bars->q_full[x]), SOFT_WARPS / 2);
             mbar_init(smem_u32(&bars->q_empty[x]), 1);
             mbar_init(smem_u32(&bars->s_full[x]), 1);
-            mbar_init(smem_u32(&bars->p_ready[x]), 4);
+            mbar_init(smem_u32(&bars->p_ready[x]), SOFT_WARPS / 2);
             mbar_init(smem_u32(&bars->pv_done[x]), 1);
         }
         for (int s = 0; s < KV_STAGES; s++) {
@@ -1055,7 +1050,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         bars->gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 4) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -1066,82 +1061,93 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     gfb_pdl_launch();
     gfb_pdl_wait();
 
-    // Registers per thread: 72 + 40 + 200 + 200 for the four warpgroups, 512 together, which is what 512 threads of 128 came with.
     PromptItem it;
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        // ---- converters: a warp has 32 keys of the 128, half of one page; a lane 16 bytes of a row at a time
+    if (warp >= SOFT_WARPS && warp < MMA_WARP) {
+        // ---- converters.  A unit is 32 keys of a block's K, or of its V; the block's eight units, K first, go round the warps.  A lane has 16 bytes of a row.
         constexpr int CH = D / 16, RPI = 32 / CH, LOADS = 32 / RPI;      // 16-byte chunks of a row, rows per load of a warp, loads
-        const int row0 = warp * 32 + lane / CH, c = lane % CH;
-        int gj = 0;                                                      // key blocks so far
+        const int sub = lane / CH, c = lane % CH;
+        // lanes of the second 64 dims write their two halves in the other order, so that the eight lanes of a row meet eight bank groups
+        const int swap = (c >> 2) & 1, k0 = 2 * (c & 3) + swap;
+        int g0 = 0;                                                      // key blocks ahead of the item
         bool ok = true;
         for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
             if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
             const int* pt = kv.page_table + (size_t)it.slot * kv.max_pages;
-            const int last_page = it.last_pos / PAGE;
-            for (int j = 0; j < it.n && ok; j++, gj++) {
-                const int s = gj % KV_STAGES, sc = gj % SC_STAGES;
-                const uint32_t empty = ((uint32_t)(gj / KV_STAGES) & 1u) ^ 1u;
-                const int pi = (it.blk0 + j) * 2 + (warp >> 1);
-                int page = -1;
-                if (pi <= last_page) {
-                    page = pi < kv.max_pages ? pt[pi] : -1;
-                    if (page < 0 || page >= kv.n_pages) {
-                        if (lane == 0) gfb_report(status, GFB_ERR_PAGE_TABLE, it.slot, pi);
-                        page = -1;
-                    }
-                }
-                const size_t first = ((size_t)max(page, 0) * G + it.g) * PAGE + (warp & 1) * 32;      // the warp's first row in the pools
-                auto fetch = [&](const int8_t* pool, uint4 (&v)[LOADS]) {
+            const int last_page = it.last_pos / PAGE, first_unit = 8 * g0, end = first_unit + 8 * it.n;
+            int U = first_unit + (warp - SOFT_WARPS + 3 * first_unit + 3 - first_unit % 3) % 3;      // the warp's first unit of the item: U mod 3 is the warp
+            // the page of a unit's keys; -1: there is none
+            auto page_of = [&](int u) -> int {
+                const int pi = (it.blk0 + ((u - first_unit) >> 3)) * 2 + ((u >> 1) & 1);
+                if (u >= end || pi > last_page) return -1;
+                const int page = pi < kv.max_pages ? pt[pi] : -1;
+                if (page >= 0 && page < kv.n_pages) return page;
+                if (lane == 0) gfb_report(status, GFB_ERR_PAGE_TABLE, it.slot, pi);
+                return -1;
+            };
+            auto row_of = [&](int u, int page) -> size_t { return ((size_t)max(page, 0) * G + it.g) * PAGE + (u & 1) * 32; };     // its first row in the pools
+            auto fetch = [&](int u, int page, uint4 (&v)[LOADS]) {
+                const int8_t* src = ((u & 4) ? kv.v_pool : kv.k_pool) + (row_of(u, page) + sub) * D + c * 16;
 #pragma unroll
-                    for (int i = 0; i < LOADS; i++)
-                        v[i] = page >= 0 ? *reinterpret_cast<const uint4*>(pool + (first + i * RPI + lane / CH) * D + c * 16) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                };
-                auto store = [&](uint8_t* tile, const uint4 (&v)[LOADS]) {
-#pragma unroll
-                    for (int i = 0; i < LOADS; i++) {
-                        const int r = row0 + i * RPI;
-                        uint8_t* line = tile + (c >> 2) * HALF_BYTES + r * 128;
-                        const uint4 a = make_uint4(pair(v[i].x), pair(v[i].x >> 8), pair(v[i].y), pair(v[i].y >> 8));
-                        const uint4 d = make_uint4(pair(v[i].z), pair(v[i].z >> 8), pair(v[i].w), pair(v[i].w >> 8));
-                        // lanes of the second 64 dims write their two halves in the other order, so that the eight lanes of a row meet eight bank groups
-                        const int swap = (c >> 2) & 1, k0 = 2 * (c & 3);
-                        *reinterpret_cast<uint4*>(line + (((k0 + swap) ^ (r & 7)) << 4)) = swap ? d : a;
-                        *reinterpret_cast<uint4*>(line + (((k0 + 1 - swap) ^ (r & 7)) << 4)) = swap ? a : d;
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor cores read it
-                    __syncwarp();
-                };
-                uint4 v[LOADS];
-                fetch(kv.k_pool, v);
-                const int key = (it.blk0 + j) * KEYS + warp * 32 + lane;
+                for (int i = 0; i < LOADS; i++) v[i] = page >= 0 ? *reinterpret_cast<const uint4*>(src + i * RPI * D) : make_uint4(0u, 0u, 0u, 0u);
+            };
+            int page = page_of(U), next = page_of(U + CONV_WARPS);
+            uint4 v[LOADS];
+            fetch(U, page, v);
+#pragma unroll 1
+            for (; U < end; U += CONV_WARPS) {
+                const int gj = U >> 3, s = gj & (KV_STAGES - 1), sc = gj & (SC_STAGES - 1), group = U & 3;
+                const bool is_v = U & 4;
+                const int key = (it.blk0 + gj - g0) * KEYS + group * 32 + lane;
                 const bool here = page >= 0 && key <= it.last_pos;
-                const float k_scale = here ? kv.k_scale[first + lane] : 0.f, v_scale = here ? kv.v_scale[first + lane] : 0.f;
-                ok = mbar_wait_warp(smem_u32(&bars->k_empty[s]), empty, gave_up, status, 401);
-                if (!ok) break;
-                scales[sc].k[warp * 32 + lane] = k_scale;
-                scales[sc].v[warp * 32 + lane] = v_scale;
-                const float lv = fmaxf(log2f(v_scale), PROMPT_LEAST_LOG);
-                const float most = gfb_warp_max(here ? lv : -ABSENT), least = -gfb_warp_max(here ? -lv : -ABSENT);
-                if (lane == 0) {
-                    scales[sc].most[warp] = most;
-                    scales[sc].least[warp] = least;
+                float k_scale = 0.f, v_scale = 0.f;
+                if (!is_v && here) {
+                    const size_t row = row_of(U, page) + lane;
+                    k_scale = kv.k_scale[row];
+                    v_scale = kv.v_scale[row];
                 }
-                store(smem + S::K + s * TILE, v);
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&bars->sc_full[sc]));
-                    mbar_arrive(smem_u32(&bars->k_full[s]));
-                }
-                fetch(kv.v_pool, v);
-                ok = mbar_wait_warp(smem_u32(&bars->v_empty[s]), empty, gave_up, status, 402);
+                const int after = page_of(U + 2 * CONV_WARPS);
+                ok = mbar_wait_warp(smem_u32(is_v ? &bars->v_empty[s] : &bars->k_empty[s]), ((uint32_t)(gj / KV_STAGES) & 1u) ^ 1u, gave_up, status, 401);
                 if (!ok) break;
-                store(smem + S::V + s * TILE, v);
-                if (lane == 0) mbar_arrive(smem_u32(&bars->v_full[s]));
+                uint4 lo[LOADS], hi[LOADS];
+#pragma unroll
+                for (int i = 0; i < LOADS; i++) {
+                    const uint32_t x = swap ? v[i].z : v[i].x, y = swap ? v[i].w : v[i].y, z = swap ? v[i].x : v[i].z, w = swap ? v[i].y : v[i].w;
+                    lo[i] = make_uint4(x, x >> 8, y, y >> 8);
+                    hi[i] = make_uint4(z, z >> 8, w, w >> 8);
+                }
+                uint8_t* line = smem + (is_v ? S::V : S::K) + s * TILE + (c >> 2) * HALF_BYTES + (group * 32 + sub) * 128;
+#pragma unroll
+                for (int i = 0; i < LOADS; i++) {
+                    const int r7 = (sub + i * RPI) & 7;
+                    *reinterpret_cast<uint4*>(line + i * RPI * 128 + ((k0 ^ r7) << 4)) = make_uint4(pair(lo[i].x), pair(lo[i].y), pair(lo[i].z), pair(lo[i].w));
+                    *reinterpret_cast<uint4*>(line + i * RPI * 128 + ((k0 ^ 1 ^ r7) << 4)) = make_uint4(pair(hi[i].x), pair(hi[i].y), pair(hi[i].z), pair(hi[i].w));
+                }
+                fetch(U + CONV_WARPS, next, v);                          // in flight during what is left of this unit and the wait for the next one's place
+                if (!is_v) {
+                    const float lv = fmaxf(log2f(v_scale), PROMPT_LEAST_LOG);
+                    scales[sc].k[group * 32 + lane] = k_scale;
+                    scales[sc].v[group * 32 + lane] = v_scale;
+                    scales[sc].log_v[group * 32 + lane] = lv;
+                    const float most = gfb_warp_max(here ? lv : -ABSENT);
+                    const float least = -gfb_warp_max(!here ? -ABSENT : (__float_as_uint(v_scale) & 0x7f800000u) == 0x7f800000u ? ABSENT : -lv);
+                    if (lane == 0) {
+                        scales[sc].most[group] = most;
+                        scales[sc].least[group] = least;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // the tensor cores read it
+                __syncwarp();
+                if (lane == 0) {
+                    if (!is_v) mbar_arrive(smem_u32(&bars->sc_full[sc]));
+                    mbar_arrive(smem_u32(is_v ? &bars->v_full[s] : &bars->k_full[s]));
+                }
+                page = next;
+                next = after;
             }
+            g0 += it.n;
         }
-    } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 4 && lane == 0) {
+    } else if (warp == MMA_WARP) {
+        if (lane == 0) {
             constexpr uint32_t idesc_s = idesc_f16(ROWS, KEYS, 0), idesc_o = idesc_f16(ROWS, D, 1);
             uint32_t n_pv[2] = {0, 0}, n_item = 0;                       // products W V issued per tile, items with keys
             int g0 = 0;                                                  // key blocks ahead of the item
@@ -1188,9 +1194,9 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll
-                            for (int kk = 0; kk < 8; kk++)               // 16 keys per MMA: 8 columns of W, 2 KB of V
-                                umma_ts(tmem + 256 + 128 * x, tmem + 128 * x + kk * 8, desc_mnmajor(base + S::V + s * TILE + kk * 2048), idesc_o,
-                                        (mine[x] | (uint32_t)kk) != 0);
+                            for (int kk = 0; kk < 8; kk++)               // 16 keys per MMA: 8 columns of W (of the second 64 keys over their own scores), 2 KB of V
+                                umma_ts(tmem + 256 + 128 * x, tmem + 128 * x + (kk >> 2) * 64 + (kk & 3) * 8, desc_mnmajor(base + S::V + s * TILE + kk * 2048),
+                                        idesc_o, (mine[x] | (uint32_t)kk) != 0);
                             umma_commit(smem_u32(&bars->pv_done[x]));
                             n_pv[x]++;
                             mine[x]++;
@@ -1211,125 +1217,141 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-        const int x = (warp - 8) >> 2, w4 = warp & 3, r = w4 * 32 + lane, tq = r / rep;      // tile, the warp's 32 lanes of tensor memory, row, its token
-        const uint32_t lanes = tmem + ((uint32_t)(w4 * 32) << 16), col_s = lanes + 128 * x, col_o = lanes + 256 + 128 * x;
-        uint8_t* tile = smem + x * TILE;
-        PromptRow<D> row;
-        uint32_t n_item = 0;                                             // items with keys so far
-        auto ask = [&](const PromptItem& i) -> bool {                    // the item's queries into shared memory
-            if (!mbar_wait_warp(smem_u32(&bars->q_empty[x]), (n_item++ & 1u) ^ 1u, gave_up, status, 411)) return false;
-            const bool mine = tq < i.nq[x];
-            row.put_query(tile, r, mine ? q + ((size_t)(i.t0 + x * TQ + tq) * H + i.g * rep + (r - tq * rep)) * D : nullptr, scale_log2e);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars->q_full[x]));
-            return true;
-        };
+        // ---- softmax.  A wait that runs out voids the results (the status says so); the warps go on to meet at the barriers of two.
+        const int x = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3;      // tile, which 64 keys, which 32 lanes of tensor memory
+        const int r = w4 * 32 + lane, tq = r / rep;                      // the thread's row and its token
+        const uint32_t lanes = tmem + ((uint32_t)(w4 * 32) << 16), col_s = lanes + 128 * x + 64 * half, col_o = lanes + 256 + 128 * x + (D / 2) * half;
+        float* mine_at = reinterpret_cast<float*>(smem + S::ROWS_AT) + (x * 2 + half) * ROWS + r;
+        const float* other_at = reinterpret_cast<const float*>(smem + S::ROWS_AT) + (x * 2 + (half ^ 1)) * ROWS + r;
+        auto meet = [&]() { asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(1 + x * 4 + w4) : "memory"); };     // the two warps of 32 rows
         int g0 = 0;
-        uint32_t n_done = 0;                                             // this tile's blocks so far
+        uint32_t n_done = 0, n_item = 0;                                 // this tile's blocks and items with keys so far
         bool ok = true;
-        for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
+        for (int pass = 0; snake_item(pass, blockIdx.x, P) < n_items; pass++) {
             if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
-            if (it.n > 0 && !ask(it)) break;
             const bool row_ok = tq < it.nq[x];
+            const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
+            float unit = 0.f;
+            if (it.n > 0) {
+                ok = ok && mbar_wait_warp(smem_u32(&bars->q_empty[x]), (n_item & 1u) ^ 1u, gave_up, status, 411);
+                n_item++;
+                unit = put_query<D>(smem + x * TILE, r, row_ok ? q + at * D : nullptr, scale_log2e, half * (D / 2), D / 2);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&bars->q_full[x]));
+            }
             const int row_pos = it.pos0[x] + tq, row_lo = window > 0 ? max(0, row_pos - window + 1) : 0;
             const int last_lo = window > 0 ? max(0, it.pos0[x] + max(it.nq[x], 1) - window) : 0;
             float M = NONE, l = 0.f;
             uint32_t here = 0;                                           // blocks of this item
-            for (int j = 0; j < it.n && ok; j++) {
+#pragma unroll 1
+            for (int j = 0; j < it.n; j++) {
                 if (!it.active(x, j)) continue;
-                const int key0 = (it.blk0 + j) * KEYS;
-                const Scales& sc = scales[(g0 + j) % SC_STAGES];
-                ok = mbar_wait_warp(smem_u32(&bars->sc_full[(g0 + j) % SC_STAGES]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
+                const int key0 = (it.blk0 + j) * KEYS, mine0 = key0 + 64 * half, st = (g0 + j) % SC_STAGES;
+                const Scales& sc = scales[st];
+                ok = ok && mbar_wait_warp(smem_u32(&bars->sc_full[st]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
                      && mbar_wait_warp(smem_u32(&bars->s_full[x]), n_done & 1u, gave_up, status, 408);
-                if (!ok) break;
+                if (!ok) { meet(); continue; }
                 tc_fence_after();
                 const bool need_mask = key0 + KEYS - 1 > it.pos0[x] || key0 < last_lo;
-                float v[4][32];
-                tmem_ld_row128(col_s, v);
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 k = *reinterpret_cast<const float4*>(sc.k + c * 32 + i);
-                        apart(mul2(both(v[c][i], v[c][i + 1]), both(k.x, k.y)), v[c][i], v[c][i + 1]);
-                        apart(mul2(both(v[c][i + 2], v[c][i + 3]), both(k.z, k.w)), v[c][i + 2], v[c][i + 3]);
-                    }
-                if (need_mask) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int kj = key0 + c * 32 + i;
-                            if (!(kj <= row_pos && kj >= row_lo)) v[c][i] = -INFINITY;
-                        }
-                }
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (sc.most[c] == -ABSENT) {                         // none of these 32 keys exists (uniform, and rare)
-#pragma unroll
-                        for (int i = 0; i < 32; i++) v[c][i] = -INFINITY;
-                    }
-                float mx = -INFINITY;
                 const float4 most4 = *reinterpret_cast<const float4*>(sc.most), least4 = *reinterpret_cast<const float4*>(sc.least);
                 const float most = fmaxf(fmaxf(most4.x, most4.y), fmaxf(most4.z, most4.w)), least = fminf(fminf(least4.x, least4.y), fminf(least4.z, least4.w));
+                const bool plain = most - least <= WIDE_LOG && fminf(fminf(most4.x, most4.y), fminf(most4.z, most4.w)) != -ABSENT;      // uniform
+                const float *ks = sc.k + 64 * half, *vs = sc.v + 64 * half;
                 float y;                                                 // at least the largest of score + log2 of the value's scale
-                if (most - least <= WIDE_LOG) {                          // uniform
-                    float mx4[4];
+                float v[2][32];
+                if (plain) {
+                    uint32_t raw[2][32];
+                    tmem_ld32_issue(col_s, raw[0]);
+                    tmem_ld32_issue(col_s + 32, raw[1]);
+                    float mx = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        mx4[c] = fmaxf(v[c][0], v[c][1]);
+                    for (int c = 0; c < 2; c++) {
+                        tmem_ld_wait32(raw[c]);
 #pragma unroll
-                        for (int i = 2; i < 32; i += 2) mx4[c] = max3(mx4[c], v[c][i], v[c][i + 1]);
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 k = *reinterpret_cast<const float4*>(ks + c * 32 + i);
+                            apart(mul2(both(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), both(k.x, k.y)), v[c][i], v[c][i + 1]);
+                            apart(mul2(both(__uint_as_float(raw[c][i + 2]), __uint_as_float(raw[c][i + 3])), both(k.z, k.w)), v[c][i + 2], v[c][i + 3]);
+                        }
                     }
-                    mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    y = fmaf(mx, row.unit, most);
+                    if (need_mask) {
+                        const int top = row_pos - mine0, low = row_lo - mine0;
+#pragma unroll
+                        for (int c = 0; c < 2; c++)
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (c * 32 + i > top || c * 32 + i < low) v[c][i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) mx = max3(mx, v[c][i], v[c][i + 1]);
+                    y = fmaf(mx, unit, most);
                 } else {
                     y = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int i = 0; i < 32; i++) y = fmaxf(y, fmaf(v[c][i], row.unit, fmaxf(log2f(sc.v[c * 32 + i]), PROMPT_LEAST_LOG)));
-                }
-                const float M_new = y > M + (15.f - LIFT) ? y : M;
-                const float corr = power2(M - M_new);
-                const uint64_t unit2 = both(row.unit, row.unit), off2 = both(LIFT - M_new, LIFT - M_new);
-                uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 vs = *reinterpret_cast<const float4*>(sc.v + c * 32 + i);
-                        float t0, t1, t2, t3;
-                        apart(fma2(both(v[c][i], v[c][i + 1]), unit2, off2), t0, t1);
-                        apart(fma2(both(v[c][i + 2], v[c][i + 3]), unit2, off2), t2, t3);
-                        const uint64_t p01 = both(power2(t0), power2(t1)), p23 = both(power2(t2), power2(t3));
-                        sum[0] = add2(sum[0], p01);
-                        sum[1] = add2(sum[1], p23);
-                        float w0, w1, w2, w3;
-                        apart(mul2(p01, both(vs.x, vs.y)), w0, w1);
-                        apart(mul2(p23, both(vs.z, vs.w)), w2, w3);
-                        if (need_mask) {                                 // an unseen key's value scale can be anything
-                            const int kj = key0 + c * 32 + i;
-                            if (!(kj <= row_pos && kj >= row_lo)) w0 = 0.f;
-                            if (!(kj + 1 <= row_pos && kj + 1 >= row_lo)) w1 = 0.f;
-                            if (!(kj + 2 <= row_pos && kj + 2 >= row_lo)) w2 = 0.f;
-                            if (!(kj + 3 <= row_pos && kj + 3 >= row_lo)) w3 = 0.f;
-                        }
-                        pk[i >> 1] = pack2_f16(w0, w1);
-                        pk[(i >> 1) + 1] = pack2_f16(w2, w3);
+#pragma unroll 1
+                    for (int i = 0; i < 64; i++) {
+                        const int kj = mine0 + i;
+                        const float s = tmem_ld1(col_s + i) * ks[i];
+                        if (kj <= row_pos && kj >= row_lo && sc.most[2 * half + (i >> 5)] != -ABSENT) y = fmaxf(y, fmaf(s, unit, sc.log_v[64 * half + i]));
                     }
-                    tmem_st16(col_s + c * 16, pk);
+                }
+                *mine_at = y;
+                meet();
+                y = fmaxf(y, *other_at);
+                const float M_new = y > M + (15.f - LIFT) ? y : M, corr = power2(M - M_new), off = LIFT - M_new;
+                float sum;
+                if (plain) {
+                    const uint64_t unit2 = both(unit, unit), off2 = both(off, off);
+                    uint64_t sums[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(vs + c * 32 + i);
+                            float t0, t1, t2, t3, w0, w1, w2, w3;
+                            apart(fma2(both(v[c][i], v[c][i + 1]), unit2, off2), t0, t1);
+                            apart(fma2(both(v[c][i + 2], v[c][i + 3]), unit2, off2), t2, t3);
+                            const uint64_t p01 = both(power2(t0), power2(t1)), p23 = both(power2(t2), power2(t3));
+                            sums[0] = add2(sums[0], p01);
+                            sums[1] = add2(sums[1], p23);
+                            apart(mul2(p01, both(f.x, f.y)), w0, w1);
+                            apart(mul2(p23, both(f.z, f.w)), w2, w3);
+                            pk[i >> 1] = pack2_f16(w0, w1);
+                            pk[(i >> 1) + 1] = pack2_f16(w2, w3);
+                        }
+                        tmem_st16(col_s + c * 16, pk);
+                    }
+                    float s0, s1, s2, s3;
+                    apart(sums[0], s0, s1);
+                    apart(sums[1], s2, s3);
+                    sum = (s0 + s1) + (s2 + s3);
+                } else {
+                    sum = 0.f;
+#pragma unroll 1
+                    for (int i = 0; i < 64; i += 2) {
+                        float w[2];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const int kj = mine0 + i + u;
+                            const float s = tmem_ld1(col_s + i + u) * ks[i + u];
+                            const bool seen = kj <= row_pos && kj >= row_lo && sc.most[2 * half + ((i + u) >> 5)] != -ABSENT;
+                            const float p = seen ? power2(fmaf(s, unit, off)) : 0.f;
+                            sum += p;
+                            w[u] = seen ? p * vs[i + u] : 0.f;           // an unseen key's value scale can be anything
+                        }
+                        tmem_st1(col_s + (i >> 1), pack2_f16(w[0], w[1]));
+                        tmem_wait_st();
+                    }
                 }
                 // O follows the reference, rarely (S of this block was issued behind the tile's previous W V, so that phase is over)
                 if (here > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
                     ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
-                    if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; c++) {
+                    for (int c = 0; c < D / 64; c++) {
                         float o[32];
                         tmem_ld32(col_o + c * 32, o);
 #pragma unroll
@@ -1340,23 +1362,25 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars->p_ready[x]));
-                float s0, s1, s2, s3;
-                apart(sum[0], s0, s1);
-                apart(sum[1], s2, s3);
-                l = l * corr + ((s0 + s1) + (s2 + s3));
+                if (lane == 0 && ok) mbar_arrive(smem_u32(&bars->p_ready[x]));
+                l = fmaf(l, corr, sum);
                 M = M_new;
                 n_done++;
                 here++;
             }
-            if (ok && here > 0) ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
+            meet();                                                      // the other half has read this one's last maximum
+            *mine_at = l;
+            meet();
+            l = half ? *other_at + l : l + *other_at;
+            meet();
+            if (here > 0) ok = ok && mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
             if (ok) {
                 tc_fence_after();
-                const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
-                const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                if (splits > 1 && row_ok) *reinterpret_cast<float2*>(scratch_ml + (at * splits + it.z) * 2) = make_float2(here > 0 ? M : NONE, here > 0 ? l : 0.f);
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                if (splits > 1 && row_ok && half == 0)
+                    *reinterpret_cast<float2*>(scratch_ml + (at * splits + it.z) * 2) = make_float2(here > 0 ? M : NONE, here > 0 ? l : 0.f);
 #pragma unroll 1
-                for (int c = 0; c < D / 32; c++) {
+                for (int c = 0; c < D / 64; c++) {
                     if (here == 0 && splits > 1) break;                  // nothing of this row in this part: its (M, l) say so
                     float o[32];
                     if (here > 0) tmem_ld32(col_o + c * 32, o);
@@ -1365,14 +1389,15 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                         for (int i = 0; i < 32; i++) o[i] = 0.f;
                     }
                     if (!row_ok) continue;
+                    const int dim = half * (D / 2) + c * 32;
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {                    // dims 0, 2, 1, 3 of every four
                         if (splits > 1) {
-                            float* dst = scratch_o + (at * splits + it.z) * D + c * 32 + i;
+                            float* dst = scratch_o + (at * splits + it.z) * D + dim + i;
                             *reinterpret_cast<float4*>(dst) = make_float4(o[i], o[i + 2], o[i + 1], o[i + 3]);
                             *reinterpret_cast<float4*>(dst + 4) = make_float4(o[i + 4], o[i + 6], o[i + 5], o[i + 7]);
                         } else {
-                            *reinterpret_cast<uint4*>(out + at * D + c * 32 + i) =
+                            *reinterpret_cast<uint4*>(out + at * D + dim + i) =
                                 make_uint4(pack2(o[i] * inv, o[i + 2] * inv), pack2(o[i + 1] * inv, o[i + 3] * inv),
                                            pack2(o[i + 4] * inv, o[i + 6] * inv), pack2(o[i + 5] * inv, o[i + 7] * inv));
                         }
@@ -1390,7 +1415,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         const unsigned long long t0 = global_ns();
         while (global_ns() - t0 < 50000ull) __nanosleep(1000);
     }
-    if (warp == 4) {
+    if (warp == MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
