@@ -1218,8 +1218,8 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         }
     } else {
         // ---- softmax.  A wait that runs out voids the results (the status says so); the warps go on to meet at the barriers of two.
-        const int x = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3;      // tile, which 64 keys, which 32 lanes of tensor memory
-        const int r = w4 * 32 + lane, tq = r / rep;                      // the thread's row and its token
+        const int x = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3;  // tile, which 64 keys, which 32 lanes of tensor memory
+        const int r = w4 * 32 + lane;                                    // the thread's row
         const uint32_t lanes = tmem + ((uint32_t)(w4 * 32) << 16), col_s = lanes + 128 * x + 64 * half, col_o = lanes + 256 + 128 * x + (D / 2) * half;
         float* mine_at = reinterpret_cast<float*>(smem + S::ROWS_AT) + (x * 2 + half) * ROWS + r;
         const float* other_at = reinterpret_cast<const float*>(smem + S::ROWS_AT) + (x * 2 + (half ^ 1)) * ROWS + r;
@@ -1229,125 +1229,145 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         bool ok = true;
         for (int pass = 0; snake_item(pass, blockIdx.x, P) < n_items; pass++) {
             if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
-            const bool row_ok = tq < it.nq[x];
-            const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
             float unit = 0.f;
             if (it.n > 0) {
+                const int tq = r / rep;
+                const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
                 ok = ok && mbar_wait_warp(smem_u32(&bars->q_empty[x]), (n_item & 1u) ^ 1u, gave_up, status, 411);
                 n_item++;
-                unit = put_query<D>(smem + x * TILE, r, row_ok ? q + at * D : nullptr, scale_log2e, half * (D / 2), D / 2);
+                unit = put_query<D>(smem + x * TILE, r, tq < it.nq[x] ? q + at * D : nullptr, scale_log2e, half * (D / 2), D / 2);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars->q_full[x]));
             }
-            const int row_pos = it.pos0[x] + tq, row_lo = window > 0 ? max(0, row_pos - window + 1) : 0;
-            const int last_lo = window > 0 ? max(0, it.pos0[x] + max(it.nq[x], 1) - window) : 0;
+            // the tile's blocks [j, end) of the item's; of those [.., plain0) and [plain1, ..) have keys that some row does not see.  top, low: the last and the
+            // first key the row sees, counted from the thread's first key of block j
+            int j = max(0, it.lo[x] - it.blk0), top, low, plain0 = 0, plain1;
+            const int end = min(it.n, it.hi[x] - it.blk0), was = (int)n_done;
+            {
+                const int row_pos = it.pos0[x] + r / rep, key0 = (it.blk0 + j) * KEYS + 64 * half;
+                top = row_pos - key0;
+                low = (window > 0 ? max(0, row_pos - window + 1) : 0) - key0;
+                if (window > 0) plain0 = (max(0, it.pos0[x] + max(it.nq[x], 1) - window) + KEYS - 1) / KEYS - it.blk0;
+                plain1 = (it.pos0[x] + 1) / KEYS - it.blk0;
+            }
+            const int item_n = it.n;
             float M = NONE, l = 0.f;
-            uint32_t here = 0;                                           // blocks of this item
 #pragma unroll 1
-            for (int j = 0; j < it.n; j++) {
-                if (!it.active(x, j)) continue;
-                const int key0 = (it.blk0 + j) * KEYS, mine0 = key0 + 64 * half, st = (g0 + j) % SC_STAGES;
-                const Scales& sc = scales[st];
-                ok = ok && mbar_wait_warp(smem_u32(&bars->sc_full[st]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
+            for (; j < end; j++, top -= KEYS, low -= KEYS) {
+                const Scales& sc = scales[(g0 + j) & (SC_STAGES - 1)];
+                ok = ok && mbar_wait_warp(smem_u32(&bars->sc_full[(g0 + j) & (SC_STAGES - 1)]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
                      && mbar_wait_warp(smem_u32(&bars->s_full[x]), n_done & 1u, gave_up, status, 408);
                 if (!ok) { meet(); continue; }
                 tc_fence_after();
-                const bool need_mask = key0 + KEYS - 1 > it.pos0[x] || key0 < last_lo;
-                const float4 most4 = *reinterpret_cast<const float4*>(sc.most), least4 = *reinterpret_cast<const float4*>(sc.least);
-                const float most = fmaxf(fmaxf(most4.x, most4.y), fmaxf(most4.z, most4.w)), least = fminf(fminf(least4.x, least4.y), fminf(least4.z, least4.w));
-                const bool plain = most - least <= WIDE_LOG && fminf(fminf(most4.x, most4.y), fminf(most4.z, most4.w)) != -ABSENT;      // uniform
-                const float *ks = sc.k + 64 * half, *vs = sc.v + 64 * half;
+                const bool need_mask = j < plain0 || j >= plain1;
+                float most;
+                bool plain;                                              // uniform
+                {
+                    const float4 m4 = *reinterpret_cast<const float4*>(sc.most), l4 = *reinterpret_cast<const float4*>(sc.least);
+                    most = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+                    plain = most - fminf(fminf(l4.x, l4.y), fminf(l4.z, l4.w)) <= WIDE_LOG && fminf(fminf(m4.x, m4.y), fminf(m4.z, m4.w)) != -ABSENT;
+                }
                 float y;                                                 // at least the largest of score + log2 of the value's scale
-                float v[2][32];
-                if (plain) {
-                    uint32_t raw[2][32];
-                    tmem_ld32_issue(col_s, raw[0]);
-                    tmem_ld32_issue(col_s + 32, raw[1]);
-                    float mx = -INFINITY;
+                // 32 of the thread's scores times their keys' scales, what the row does not see at -infinity.  They are fetched for the maximum and once more
+                // for the weights: 64 of them in registers cost more in spills than 16 products and 8 loads do.
+                auto scores = [&](int c, uint64_t (&v)[16]) {
+                    uint32_t raw[32];
+                    tmem_ld32_issue(col_s + 32 * c, raw);
+                    const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(sc.k + 64 * half + 32 * c);
+                    tmem_ld_wait32(raw);
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        tmem_ld_wait32(raw[c]);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 k = *reinterpret_cast<const float4*>(ks + c * 32 + i);
-                            apart(mul2(both(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), both(k.x, k.y)), v[c][i], v[c][i + 1]);
-                            apart(mul2(both(__uint_as_float(raw[c][i + 2]), __uint_as_float(raw[c][i + 3])), both(k.z, k.w)), v[c][i + 2], v[c][i + 3]);
-                        }
+                    for (int i = 0; i < 16; i += 2) {
+                        const ulonglong2 k = ks[i / 2];
+                        v[i] = mul2(both(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), k.x);
+                        v[i + 1] = mul2(both(__uint_as_float(raw[2 * i + 2]), __uint_as_float(raw[2 * i + 3])), k.y);
                     }
                     if (need_mask) {
-                        const int top = row_pos - mine0, low = row_lo - mine0;
+                        const int t = top - 32 * c, f = low - 32 * c;
 #pragma unroll
-                        for (int c = 0; c < 2; c++)
-#pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (c * 32 + i > top || c * 32 + i < low) v[c][i] = -INFINITY;
+                        for (int i = 0; i < 16; i++) {
+                            float s0, s1;
+                            apart(v[i], s0, s1);
+                            if (2 * i > t || 2 * i < f) s0 = -INFINITY;
+                            if (2 * i + 1 > t || 2 * i + 1 < f) s1 = -INFINITY;
+                            v[i] = both(s0, s1);
+                        }
                     }
+                };
+                if (plain) {
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int c = 0; c < 2; c++) {
+                        uint64_t v[16];
+                        scores(c, v);
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) mx = max3(mx, v[c][i], v[c][i + 1]);
-                    y = fmaf(mx, unit, most);
+                        for (int i = 0; i < 16; i++) {
+                            float s0, s1;
+                            apart(v[i], s0, s1);
+                            mx[i & 3] = max3(mx[i & 3], s0, s1);
+                        }
+                    }
+                    y = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), unit, most);
                 } else {
                     y = -INFINITY;
 #pragma unroll 1
                     for (int i = 0; i < 64; i++) {
-                        const int kj = mine0 + i;
-                        const float s = tmem_ld1(col_s + i) * ks[i];
-                        if (kj <= row_pos && kj >= row_lo && sc.most[2 * half + (i >> 5)] != -ABSENT) y = fmaxf(y, fmaf(s, unit, sc.log_v[64 * half + i]));
+                        const float s = tmem_ld1(col_s + i) * sc.k[64 * half + i];
+                        if (i <= top && i >= low && sc.most[2 * half + (i >> 5)] != -ABSENT) y = fmaxf(y, fmaf(s, unit, sc.log_v[64 * half + i]));
                     }
                 }
                 *mine_at = y;
                 meet();
                 y = fmaxf(y, *other_at);
                 const float M_new = y > M + (15.f - LIFT) ? y : M, corr = power2(M - M_new), off = LIFT - M_new;
-                float sum;
+                M = M_new;
                 if (plain) {
                     const uint64_t unit2 = both(unit, unit), off2 = both(off, off);
                     uint64_t sums[2] = {0ull, 0ull};
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < 2; c++) {
+                        uint64_t v[16];
+                        scores(c, v);
+                        const ulonglong2* vs = reinterpret_cast<const ulonglong2*>(sc.v + 64 * half + 32 * c);
                         uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(vs + c * 32 + i);
-                            float t0, t1, t2, t3, w0, w1, w2, w3;
-                            apart(fma2(both(v[c][i], v[c][i + 1]), unit2, off2), t0, t1);
-                            apart(fma2(both(v[c][i + 2], v[c][i + 3]), unit2, off2), t2, t3);
-                            const uint64_t p01 = both(power2(t0), power2(t1)), p23 = both(power2(t2), power2(t3));
-                            sums[0] = add2(sums[0], p01);
-                            sums[1] = add2(sums[1], p23);
-                            apart(mul2(p01, both(f.x, f.y)), w0, w1);
-                            apart(mul2(p23, both(f.z, f.w)), w2, w3);
-                            pk[i >> 1] = pack2_f16(w0, w1);
-                            pk[(i >> 1) + 1] = pack2_f16(w2, w3);
+                        for (int i = 0; i < 16; i += 2) {
+                            const ulonglong2 f = vs[i / 2];
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                float t0, t1;
+                                apart(fma2(v[i + u], unit2, off2), t0, t1);
+                                const uint64_t p = both(power2(t0), power2(t1));
+                                sums[u] = add2(sums[u], p);
+                                apart(mul2(p, u ? f.y : f.x), t0, t1);
+                                pk[i + u] = pack2_f16(t0, t1);
+                            }
                         }
                         tmem_st16(col_s + c * 16, pk);
                     }
                     float s0, s1, s2, s3;
                     apart(sums[0], s0, s1);
                     apart(sums[1], s2, s3);
-                    sum = (s0 + s1) + (s2 + s3);
+                    l = fmaf(l, corr, (s0 + s1) + (s2 + s3));
                 } else {
-                    sum = 0.f;
+                    l *= corr;
 #pragma unroll 1
                     for (int i = 0; i < 64; i += 2) {
                         float w[2];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const int kj = mine0 + i + u;
-                            const float s = tmem_ld1(col_s + i + u) * ks[i + u];
-                            const bool seen = kj <= row_pos && kj >= row_lo && sc.most[2 * half + ((i + u) >> 5)] != -ABSENT;
+                            const float s = tmem_ld1(col_s + i + u) * sc.k[64 * half + i + u];
+                            const bool seen = i + u <= top && i + u >= low && sc.most[2 * half + ((i + u) >> 5)] != -ABSENT;
                             const float p = seen ? power2(fmaf(s, unit, off)) : 0.f;
-                            sum += p;
-                            w[u] = seen ? p * vs[i + u] : 0.f;           // an unseen key's value scale can be anything
+                            l += p;
+                            w[u] = seen ? p * sc.v[64 * half + i + u] : 0.f;             // an unseen key's value scale can be anything
                         }
                         tmem_st1(col_s + (i >> 1), pack2_f16(w[0], w[1]));
                         tmem_wait_st();
                     }
                 }
                 // O follows the reference, rarely (S of this block was issued behind the tile's previous W V, so that phase is over)
-                if (here > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                if (was != (int)n_done && __any_sync(0xffffffffu, corr != 1.f)) {
                     ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
                     tc_fence_after();
 #pragma unroll 1
@@ -1363,27 +1383,29 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0 && ok) mbar_arrive(smem_u32(&bars->p_ready[x]));
-                l = fmaf(l, corr, sum);
-                M = M_new;
                 n_done++;
-                here++;
             }
+            const bool some = was != (int)n_done;                        // the part has keys of this tile
             meet();                                                      // the other half has read this one's last maximum
             *mine_at = l;
             meet();
             l = half ? *other_at + l : l + *other_at;
             meet();
-            if (here > 0) ok = ok && mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
+            if (some) ok = ok && mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
             if (ok) {
                 tc_fence_after();
+                it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window);
+                const int tq = r / rep;
+                const bool row_ok = tq < it.nq[x];
+                const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 if (splits > 1 && row_ok && half == 0)
-                    *reinterpret_cast<float2*>(scratch_ml + (at * splits + it.z) * 2) = make_float2(here > 0 ? M : NONE, here > 0 ? l : 0.f);
+                    *reinterpret_cast<float2*>(scratch_ml + (at * splits + it.z) * 2) = make_float2(some ? M : NONE, some ? l : 0.f);
 #pragma unroll 1
                 for (int c = 0; c < D / 64; c++) {
-                    if (here == 0 && splits > 1) break;                  // nothing of this row in this part: its (M, l) say so
+                    if (!some && splits > 1) break;                      // nothing of this row in this part: its (M, l) say so
                     float o[32];
-                    if (here > 0) tmem_ld32(col_o + c * 32, o);
+                    if (some) tmem_ld32(col_o + c * 32, o);
                     else {
 #pragma unroll
                         for (int i = 0; i < 32; i++) o[i] = 0.f;
@@ -1405,7 +1427,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 }
                 tc_fence_before();
             }
-            g0 += it.n;
+            g0 += item_n;
         }
     }
 
