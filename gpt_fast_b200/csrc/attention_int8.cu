@@ -783,24 +783,24 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // A work item is two tiles of 128 rows, a row being (token, head of the group): 2 TQ consecutive tokens of one sequence and key head, TQ = 128 / (heads per
 // group), against the item's keys, or one of `splits` equal parts of them where items are few.  Blocks are persistent, one per SM.  Per 128 keys:
 //
-//   converters (3 warps)    the integers of K and V from the cache through registers into shared memory as float16 (`pair`, exact), with the 128-byte swizzle
-//                           the tensor cores read; the scales beside them
+//   converters (7 warps)    K and V from the cache through registers into shared memory as float16, with the 128-byte swizzle the tensor cores read: integers
+//                           (`pair`) times their row's scale over a power of two that the 128 rows share, k_ref and v_ref
 //   MMA (one thread)        S = Q K^T (128 x 128, A and B from shared memory) and O += W V (W from tensor memory, V as it lies, [key][dim]); the pipe
 //                           alternates between the two tiles, so one's softmax runs under the other's products
-//   softmax (8 warps per tile, two threads per row, 64 keys each)   s = S ks unit;  p = 2^(s - M + LIFT), l += p;  W = p vs as float16, over the first half of
-//                           the thread's own scores
+//   softmax (8 warps per tile, two threads per row, 64 keys each)   s = S unit k_ref;  W = 2^(s + log2 v_ref - M + LIFT) as float16, over the first half of the
+//                           thread's own scores;  l += W / v_ref
 //
-// The arithmetic is the single-token kernel's: queries as float16 times a power of two per row, W rounded once, M the reference of weights times scales, which
-// follows their maximum in steps of 2^3 or more.  Here the sum has the same reference (p stays below 2^105 for scales from 2^-90 up).  M counts the largest
-// scale of the 128 keys for each of them; where the scales of 128 keys differ by more than 2^8, or one is not finite, a slower way works it out key by key.
+// Here scales are multiplied in ahead of the products, where a key's is needed once and not once per query: the number an integer and its scale stand for
+// is rounded to float16, half a step being 2^-11 of it, an eighth of what a bfloat16 cache has.  (With the scales applied to scores and weights, exactly, the
+// softmax warps took 2.3 times the instructions, two thirds of their loads from shared memory among them, and the step 476 us.)  The scale itself
+// enters as two float16 numbers, so its own rounding does not add up over a row.  Queries are float16 times a power of two per row, as in the single-token
+// kernel; M, the reference of weights with v_ref, follows their maximum in steps of 2^3 or more, and a weight below 2^-37 of the largest is lost.
+// A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
-//
-// What bounds it: the softmax warps' instructions.  (One thread per row, 128 scores in registers, everything unrolled: 1,198 us for 512 tokens behind 32,001; the
-// MMA thread waited for its instructions to come into the cache, 400 cycles per MMA.)
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
-constexpr int SOFT_WARPS = 16, CONV_WARPS = 3, MMA_WARP = SOFT_WARPS + CONV_WARPS, PROMPT_THREADS = 32 * (MMA_WARP + 1);     // five warps per quarter of an SM: 96 registers each
-constexpr float PROMPT_LEAST_LOG = -90.f, WIDE_LOG = 8.f, ABSENT = 1e30f;
+constexpr int SOFT_WARPS = 16, CONV_WARPS = 7, CONV_UNITS = 8, MMA_WARP = SOFT_WARPS + CONV_WARPS, PROMPT_THREADS = 32 * (MMA_WARP + 1);     // six warps per quarter of an SM: 80 registers each
+constexpr int LEAST_EXPONENT = 37, MOST_EXPONENT = 217;      // of k_ref and v_ref, in a float's bits: 2^-90 to 2^90, so that weights over v_ref stay finite
 
 struct PromptBars {
     unsigned long long q_full[2], q_empty[2];
@@ -810,14 +810,22 @@ struct PromptBars {
     uint32_t tmem_base;
     int gave_up;
 };
-struct Scales {
-    float k[KEYS], v[KEYS], log_v[KEYS];     // log2 of the values' scales, at least PROMPT_LEAST_LOG
-    float most[4], least[4];                 // of them, per 32 keys (least: -ABSENT where a scale is not finite; most: -ABSENT where there is no key)
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+// two float16 numbers x times the number hi + lo
+__device__ __forceinline__ uint32_t times(uint32_t x, uint32_t hi, uint32_t lo) {
+    uint32_t y;
+    asm("{\n\t.reg .b32 t;\n\tmul.rn.f16x2 t, %1, %3;\n\tfma.rn.f16x2 %0, %1, %2, t;\n\t}" : "=r"(y) : "r"(x), "r"(hi), "r"(lo));
+    return y;
+}
+// What the softmax warps have to know of 128 keys.
+struct Refs {
+    float k_ref, log_v_ref, inv_v_ref, unused;
+    int missing[4];                          // per 32 keys: the page table has no page for them
 };
 template <int D>
 struct PromptSmem {
     static constexpr int TILE = (D / 64) * HALF_BYTES;
-    static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, ROWS_AT = SC + SC_STAGES * (int)sizeof(Scales);
+    static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, ROWS_AT = SC + SC_STAGES * (int)sizeof(Refs);
     static constexpr int BARS = ROWS_AT + 2 * 2 * ROWS * 4;
     static constexpr int BYTES = 1024 + BARS + (int)sizeof(PromptBars);
 };
@@ -907,16 +915,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-// one column: a number per lane
-__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(v) : "memory");
-}
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
-    uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r) :: "memory");
-    return __uint_as_float(r);
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // two 32-bit numbers per instruction
 __device__ __forceinline__ uint64_t both(float a, float b) {
@@ -925,11 +923,6 @@ __device__ __forceinline__ uint64_t both(float a, float b) {
     return r;
 }
 __device__ __forceinline__ void apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -1027,7 +1020,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     extern __shared__ __align__(16) uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-    Scales* scales = reinterpret_cast<Scales*>(smem + S::SC);
+    Refs* refs = reinterpret_cast<Refs*>(smem + S::SC);
     PromptBars* bars = reinterpret_cast<PromptBars*>(smem + S::BARS);
     volatile int* gave_up = &bars->gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1065,75 +1058,102 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         // ---- converters.  A unit is 32 keys of a block's K, or of its V; the block's eight units, K first, go round the warps.  A lane has 16 bytes of a row.
         constexpr int CH = D / 16, RPI = 32 / CH, LOADS = 32 / RPI;      // 16-byte chunks of a row, rows per load of a warp, loads
-        const int sub = lane / CH, c = lane % CH;
-        // lanes of the second 64 dims write their two halves in the other order, so that the eight lanes of a row meet eight bank groups
-        const int swap = (c >> 2) & 1, k0 = 2 * (c & 3) + swap;
+        // which row of a load's and which chunk: every eight lanes have four chunks of the same 64 dims of two neighbouring rows, whose 16-byte pieces meet
+        // eight bank groups
+        const int sub = CH == 8 ? ((lane >> 2) & 1) | ((lane >> 4) << 1) : lane >> 2, c = CH == 8 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3;
         int g0 = 0;                                                      // key blocks ahead of the item
         bool ok = true;
         for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
             if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
             const int* pt = kv.page_table + (size_t)it.slot * kv.max_pages;
-            const int last_page = it.last_pos / PAGE, first_unit = 8 * g0, end = first_unit + 8 * it.n;
-            int U = first_unit + (warp - SOFT_WARPS + 3 * first_unit + 3 - first_unit % 3) % 3;      // the warp's first unit of the item: U mod 3 is the warp
-            // the page of a unit's keys; -1: there is none
-            auto page_of = [&](int u) -> int {
-                const int pi = (it.blk0 + ((u - first_unit) >> 3)) * 2 + ((u >> 1) & 1);
-                if (u >= end || pi > last_page) return -1;
-                const int page = pi < kv.max_pages ? pt[pi] : -1;
-                if (page >= 0 && page < kv.n_pages) return page;
-                if (lane == 0) gfb_report(status, GFB_ERR_PAGE_TABLE, it.slot, pi);
-                return -1;
+            const int last_page = it.last_pos / PAGE, first_unit = CONV_UNITS * g0, end = first_unit + CONV_UNITS * it.n;
+            int U = first_unit + (warp - SOFT_WARPS + CONV_WARPS - first_unit % CONV_WARPS) % CONV_WARPS;      // the warp's first unit of the item
+            // the pages of a unit's block; -1: not needed or not there
+            auto pages_of = [&](int u) -> int2 {
+                const int pi = (it.blk0 + ((u - first_unit) >> 3)) * 2;
+                int2 p = make_int2(-1, -1);
+                if (u < end) {
+                    if (pi <= last_page && pi < kv.max_pages) p.x = pt[pi];
+                    if (pi + 1 <= last_page && pi + 1 < kv.max_pages) p.y = pt[pi + 1];
+                    if (p.x >= kv.n_pages) p.x = -1;
+                    if (p.y >= kv.n_pages) p.y = -1;
+                }
+                return p;
             };
-            auto row_of = [&](int u, int page) -> size_t { return ((size_t)max(page, 0) * G + it.g) * PAGE + (u & 1) * 32; };     // its first row in the pools
-            auto fetch = [&](int u, int page, uint4 (&v)[LOADS]) {
-                const int8_t* src = ((u & 4) ? kv.v_pool : kv.k_pool) + (row_of(u, page) + sub) * D + c * 16;
+            auto row_of = [&](int page) -> size_t { return ((size_t)max(page, 0) * G + it.g) * PAGE; };         // a page's first row in the pools
+            auto fetch = [&](int u, int2 p, uint4 (&v)[LOADS]) {
+                const int page = (u & 2) ? p.y : p.x;
+                const int8_t* src = ((u & 4) ? kv.v_pool : kv.k_pool) + (row_of(page) + (u & 1) * 32 + sub) * D + c * 16;
 #pragma unroll
                 for (int i = 0; i < LOADS; i++) v[i] = page >= 0 ? *reinterpret_cast<const uint4*>(src + i * RPI * D) : make_uint4(0u, 0u, 0u, 0u);
             };
-            int page = page_of(U), next = page_of(U + CONV_WARPS);
+            // scales of the 128 keys, four per lane: keys lane, lane + 32, ...
+            auto fetch_scales = [&](int2 p, float (&ks)[4], float (&vs)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int page = i < 2 ? p.x : p.y;
+                    const size_t row = row_of(page) + (i & 1) * 32 + lane;
+                    ks[i] = page >= 0 ? kv.k_scale[row] : 0.f;
+                    vs[i] = page >= 0 ? kv.v_scale[row] : 0.f;
+                }
+            };
+            int2 page = pages_of(U), next = pages_of(U + CONV_WARPS);
             uint4 v[LOADS];
+            float ks[4], vs[4];
             fetch(U, page, v);
+            fetch_scales(page, ks, vs);
 #pragma unroll 1
             for (; U < end; U += CONV_WARPS) {
                 const int gj = U >> 3, s = gj & (KV_STAGES - 1), sc = gj & (SC_STAGES - 1), group = U & 3;
                 const bool is_v = U & 4;
-                const int key = (it.blk0 + gj - g0) * KEYS + group * 32 + lane;
-                const bool here = page >= 0 && key <= it.last_pos;
-                float k_scale = 0.f, v_scale = 0.f;
-                if (!is_v && here) {
-                    const size_t row = row_of(U, page) + lane;
-                    k_scale = kv.k_scale[row];
-                    v_scale = kv.v_scale[row];
+                // the powers of two above the largest finite scales of the block's keys, and this lane's key's scale over its own
+                const int key0 = (it.blk0 + gj - g0) * KEYS + lane;
+                uint32_t kt = 0, vt = 0;
+                float mine = 0.f;
+                bool odd = false;                                        // a scale that is not finite
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool here = key0 + 32 * i <= it.last_pos;
+                    const uint32_t kb = __float_as_uint(ks[i]) & 0x7fffffffu, vb = __float_as_uint(vs[i]) & 0x7fffffffu;
+                    if (here && kb < 0x7f800000u) kt = max(kt, kb);
+                    if (here && vb < 0x7f800000u) vt = max(vt, vb);
+                    if (i == group) {
+                        mine = here ? (is_v ? vs[i] : ks[i]) : 0.f;
+                        odd = here && (kb >= 0x7f800000u || vb >= 0x7f800000u);
+                    }
                 }
-                const int after = page_of(U + 2 * CONV_WARPS);
+                const int ke = min(max((int)(warp_max_bits(kt) >> 23) + 1, LEAST_EXPONENT), MOST_EXPONENT);
+                const int ve = min(max((int)(warp_max_bits(vt) >> 23) + 1, LEAST_EXPONENT), MOST_EXPONENT);
+                const float over = mine * __uint_as_float((uint32_t)(254 - (is_v ? ve : ke)) << 23);
+                const __half hi = __float2half_rn(over), lo = __float2half_rn(over - __half2float(hi));
+                uint32_t factor = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+                if (odd) factor = is_v ? 0u : 0x7fff7fffu;
+                const int2 after = pages_of(U + 2 * CONV_WARPS);
                 ok = mbar_wait_warp(smem_u32(is_v ? &bars->v_empty[s] : &bars->k_empty[s]), ((uint32_t)(gj / KV_STAGES) & 1u) ^ 1u, gave_up, status, 401);
                 if (!ok) break;
-                uint4 lo[LOADS], hi[LOADS];
-#pragma unroll
-                for (int i = 0; i < LOADS; i++) {
-                    const uint32_t x = swap ? v[i].z : v[i].x, y = swap ? v[i].w : v[i].y, z = swap ? v[i].x : v[i].z, w = swap ? v[i].y : v[i].w;
-                    lo[i] = make_uint4(x, x >> 8, y, y >> 8);
-                    hi[i] = make_uint4(z, z >> 8, w, w >> 8);
-                }
                 uint8_t* line = smem + (is_v ? S::V : S::K) + s * TILE + (c >> 2) * HALF_BYTES + (group * 32 + sub) * 128;
+                const int even = ((2 * (c & 3)) ^ (sub & 7)) << 4, odd_row = RPI == 4 ? even ^ 64 : even;      // (rows 4 further exchange pieces 4 further)
 #pragma unroll
                 for (int i = 0; i < LOADS; i++) {
-                    const int r7 = (sub + i * RPI) & 7;
-                    *reinterpret_cast<uint4*>(line + i * RPI * 128 + ((k0 ^ r7) << 4)) = make_uint4(pair(lo[i].x), pair(lo[i].y), pair(lo[i].z), pair(lo[i].w));
-                    *reinterpret_cast<uint4*>(line + i * RPI * 128 + ((k0 ^ 1 ^ r7) << 4)) = make_uint4(pair(hi[i].x), pair(hi[i].y), pair(hi[i].z), pair(hi[i].w));
+                    const int piece = (i & 1) ? odd_row : even;
+                    const uint32_t f = __shfl_sync(0xffffffffu, factor, sub + i * RPI);
+                    const uint32_t hi2 = __byte_perm(f, f, 0x1010), lo2 = __byte_perm(f, f, 0x3232);
+                    *reinterpret_cast<uint4*>(line + i * RPI * 128 + piece) = make_uint4(times(pair(v[i].x), hi2, lo2), times(pair(v[i].x >> 8), hi2, lo2),
+                                                                                         times(pair(v[i].y), hi2, lo2), times(pair(v[i].y >> 8), hi2, lo2));
+                    *reinterpret_cast<uint4*>(line + i * RPI * 128 + (piece ^ 16)) = make_uint4(times(pair(v[i].z), hi2, lo2), times(pair(v[i].z >> 8), hi2, lo2),
+                                                                                                times(pair(v[i].w), hi2, lo2), times(pair(v[i].w >> 8), hi2, lo2));
                 }
                 fetch(U + CONV_WARPS, next, v);                          // in flight during what is left of this unit and the wait for the next one's place
-                if (!is_v) {
-                    const float lv = fmaxf(log2f(v_scale), PROMPT_LEAST_LOG);
-                    scales[sc].k[group * 32 + lane] = k_scale;
-                    scales[sc].v[group * 32 + lane] = v_scale;
-                    scales[sc].log_v[group * 32 + lane] = lv;
-                    const float most = gfb_warp_max(here ? lv : -ABSENT);
-                    const float least = -gfb_warp_max(!here ? -ABSENT : (__float_as_uint(v_scale) & 0x7f800000u) == 0x7f800000u ? ABSENT : -lv);
-                    if (lane == 0) {
-                        scales[sc].most[group] = most;
-                        scales[sc].least[group] = least;
+                fetch_scales(next, ks, vs);
+                if (!is_v && lane == 0) {
+                    const int mine_page = (group & 2) ? page.y : page.x, index = (it.blk0 + gj - g0) * 2 + (group >> 1);
+                    if (group == 0) {
+                        refs[sc].k_ref = __uint_as_float((uint32_t)ke << 23);
+                        refs[sc].log_v_ref = (float)(ve - 127);
+                        refs[sc].inv_v_ref = __uint_as_float((uint32_t)(254 - ve) << 23);
                     }
+                    refs[sc].missing[group] = mine_page < 0 && index <= last_page;
+                    if (mine_page < 0 && index <= last_page) gfb_report(status, GFB_ERR_PAGE_TABLE, it.slot, index);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // the tensor cores read it
                 __syncwarp();
@@ -1255,117 +1275,60 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             float M = NONE, l = 0.f;
 #pragma unroll 1
             for (; j < end; j++, top -= KEYS, low -= KEYS) {
-                const Scales& sc = scales[(g0 + j) & (SC_STAGES - 1)];
+                const Refs& ref = refs[(g0 + j) & (SC_STAGES - 1)];
                 ok = ok && mbar_wait_warp(smem_u32(&bars->sc_full[(g0 + j) & (SC_STAGES - 1)]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
                      && mbar_wait_warp(smem_u32(&bars->s_full[x]), n_done & 1u, gave_up, status, 408);
                 if (!ok) { meet(); continue; }
                 tc_fence_after();
-                const bool need_mask = j < plain0 || j >= plain1;
-                float most;
-                bool plain;                                              // uniform
-                {
-                    const float4 m4 = *reinterpret_cast<const float4*>(sc.most), l4 = *reinterpret_cast<const float4*>(sc.least);
-                    most = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
-                    plain = most - fminf(fminf(l4.x, l4.y), fminf(l4.z, l4.w)) <= WIDE_LOG && fminf(fminf(m4.x, m4.y), fminf(m4.z, m4.w)) != -ABSENT;
-                }
-                float y;                                                 // at least the largest of score + log2 of the value's scale
-                // 32 of the thread's scores times their keys' scales, what the row does not see at -infinity.  They are fetched for the maximum and once more
-                // for the weights: 64 of them in registers cost more in spills than 16 products and 8 loads do.
-                auto scores = [&](int c, uint64_t (&v)[16]) {
-                    uint32_t raw[32];
-                    tmem_ld32_issue(col_s + 32 * c, raw);
-                    const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(sc.k + 64 * half + 32 * c);
-                    tmem_ld_wait32(raw);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const ulonglong2 k = ks[i / 2];
-                        v[i] = mul2(both(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), k.x);
-                        v[i + 1] = mul2(both(__uint_as_float(raw[2 * i + 2]), __uint_as_float(raw[2 * i + 3])), k.y);
-                    }
+                const int gone = ref.missing[2 * half] | (ref.missing[2 * half + 1] << 1);       // 32 keys without a page: rare
+                const bool need_mask = j < plain0 || j >= plain1 || gone;
+                const float by = unit * ref.k_ref;
+                // 32 of the thread's scores, what the row does not see at -infinity.  They are fetched for the maximum and once more for the weights, since 64 of
+                // them do not stay in registers.
+                auto scores = [&](int c, uint32_t (&v)[32]) {
+                    tmem_ld32_issue(col_s + 32 * c, v);
+                    tmem_ld_wait32(v);
                     if (need_mask) {
-                        const int t = top - 32 * c, f = low - 32 * c;
+                        const int t = (gone >> c & 1) ? -1 : top - 32 * c, f = low - 32 * c;
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float s0, s1;
-                            apart(v[i], s0, s1);
-                            if (2 * i > t || 2 * i < f) s0 = -INFINITY;
-                            if (2 * i + 1 > t || 2 * i + 1 < f) s1 = -INFINITY;
-                            v[i] = both(s0, s1);
-                        }
+                        for (int i = 0; i < 32; i++)
+                            if (i > t || i < f) v[i] = 0xff800000u;
                     }
                 };
-                if (plain) {
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-                    for (int c = 0; c < 2; c++) {
-                        uint64_t v[16];
-                        scores(c, v);
+                for (int c = 0; c < 2; c++) {
+                    uint32_t v[32];
+                    scores(c, v);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float s0, s1;
-                            apart(v[i], s0, s1);
-                            mx[i & 3] = max3(mx[i & 3], s0, s1);
-                        }
-                    }
-                    y = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), unit, most);
-                } else {
-                    y = -INFINITY;
-#pragma unroll 1
-                    for (int i = 0; i < 64; i++) {
-                        const float s = tmem_ld1(col_s + i) * sc.k[64 * half + i];
-                        if (i <= top && i >= low && sc.most[2 * half + (i >> 5)] != -ABSENT) y = fmaxf(y, fmaf(s, unit, sc.log_v[64 * half + i]));
-                    }
+                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                 }
+                float y = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), by, ref.log_v_ref);
                 *mine_at = y;
                 meet();
                 y = fmaxf(y, *other_at);
-                const float M_new = y > M + (15.f - LIFT) ? y : M, corr = power2(M - M_new), off = LIFT - M_new;
+                const float M_new = y > M + (15.f - LIFT) ? y : M, corr = power2(M - M_new), off = ref.log_v_ref + LIFT - M_new;
                 M = M_new;
-                if (plain) {
-                    const uint64_t unit2 = both(unit, unit), off2 = both(off, off);
-                    uint64_t sums[2] = {0ull, 0ull};
+                const uint64_t by2 = both(by, by), off2 = both(off, off);
+                uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll 1
-                    for (int c = 0; c < 2; c++) {
-                        uint64_t v[16];
-                        scores(c, v);
-                        const ulonglong2* vs = reinterpret_cast<const ulonglong2*>(sc.v + 64 * half + 32 * c);
-                        uint32_t pk[16];
+                for (int c = 0; c < 2; c++) {
+                    uint32_t v[32], pk[16];
+                    scores(c, v);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const ulonglong2 f = vs[i / 2];
-#pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                float t0, t1;
-                                apart(fma2(v[i + u], unit2, off2), t0, t1);
-                                const uint64_t p = both(power2(t0), power2(t1));
-                                sums[u] = add2(sums[u], p);
-                                apart(mul2(p, u ? f.y : f.x), t0, t1);
-                                pk[i + u] = pack2_f16(t0, t1);
-                            }
-                        }
-                        tmem_st16(col_s + c * 16, pk);
+                    for (int i = 0; i < 32; i += 2) {
+                        float t0, t1;
+                        apart(fma2(both(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), by2, off2), t0, t1);
+                        const float w0 = power2(t0), w1 = power2(t1);
+                        sums[(i >> 1) & 1] = add2(sums[(i >> 1) & 1], both(w0, w1));
+                        pk[i >> 1] = pack2_f16(w0, w1);
                     }
-                    float s0, s1, s2, s3;
-                    apart(sums[0], s0, s1);
-                    apart(sums[1], s2, s3);
-                    l = fmaf(l, corr, (s0 + s1) + (s2 + s3));
-                } else {
-                    l *= corr;
-#pragma unroll 1
-                    for (int i = 0; i < 64; i += 2) {
-                        float w[2];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const float s = tmem_ld1(col_s + i + u) * sc.k[64 * half + i + u];
-                            const bool seen = i + u <= top && i + u >= low && sc.most[2 * half + ((i + u) >> 5)] != -ABSENT;
-                            const float p = seen ? power2(fmaf(s, unit, off)) : 0.f;
-                            l += p;
-                            w[u] = seen ? p * sc.v[64 * half + i + u] : 0.f;             // an unseen key's value scale can be anything
-                        }
-                        tmem_st1(col_s + (i >> 1), pack2_f16(w[0], w[1]));
-                        tmem_wait_st();
-                    }
+                    tmem_st16(col_s + c * 16, pk);
                 }
+                float s0, s1, s2, s3;
+                apart(sums[0], s0, s1);
+                apart(sums[1], s2, s3);
+                l = fmaf(l, corr, ((s0 + s1) + (s2 + s3)) * ref.inv_v_ref);
                 // O follows the reference, rarely (S of this block was issued behind the tile's previous W V, so that phase is over)
                 if (was != (int)n_done && __any_sync(0xffffffffu, corr != 1.f)) {
                     ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
