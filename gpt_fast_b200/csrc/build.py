@@ -49,7 +49,7 @@ LIBRARIES = {
     "gemm_int8": (["gemm_int8.cu"], [], []),
     "attention_int8": (["attention_int8.cu"], [], []),
 }
-HEADERS = ["common.cuh", "attn_decode_noalloc.h"]
+HEADERS = ["common.cuh", "attn_decode_noalloc.h", "int8_rows.cuh"]
 
 _loaded = {}
 _lock = threading.Lock()

@@ -1,5 +1,5 @@
 // Products of 8-bit integers on the 5th-generation tensor cores: y[m, n] = a_scale[m] w_scale[n] sum_k A[m, k] W[n, k] for rows of integers
-// with a scale each (quantize.cu).
+// with a scale each (int8_rows.cuh).
 //
 // The sum is a 32-bit integer in tensor memory (tcgen05.mma kind::i8), so it has no rounding and no order: however K is split and whatever batch a row
 // comes in, its result is the same bits.  |sum| <= 127^2 K stays below 2^31 for K up to 133,144.  Behind it everything is 32-bit floating point: the integer
@@ -17,7 +17,7 @@
 //
 // Weights are taken to be complete before the kernel ahead of this one starts: the ring is filled with them ahead of the wait for it.  quantize_rows, which
 // makes them, lets no kernel start before it has ended.
-#include "common.cuh"
+#include "int8_rows.cuh"
 
 #include <cuda.h>
 
@@ -766,4 +766,20 @@ GFB_API int gfb_gemm_int8(const void* A, const float* a_scale, int lda, const vo
     if (epi == EPI_GELU || epi == EPI_GELU_TANH || epi == EPI_SILU || epi == EPI_RELU2) GO(KIND_UNARY);
 #undef GO
     return gfb_fail("gfb_gemm_int8: unknown epilogue %d", epi);
+}
+
+// The same with a [M, K] of bfloat16 or float32 (a_dt) that is quantised on the way: scratch of M (pitch + 4) bytes, pitch = K rounded up to 16.
+GFB_API int gfb_linear_int8(const void* a, int a_dt, void* scratch, const void* W, const float* w_scale, int ldw, void* out, int out_dt, int M, int N, int K, int epi,
+                            int bn, int splits, int stages, int* status, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || K > 133144) return gfb_fail("gfb_linear_int8: rows of %d numbers (1 to 133,144, beyond which a sum may leave 32 bits)", K);
+    const int pitch = (K + 15) / 16 * 16;
+    int8_t* q = (int8_t*)scratch;
+    float* scale = (float*)(q + (size_t)M * pitch);
+    cudaError_t e;
+    if (a_dt == GFB_BF16) e = quantize_rows_launch((const __nv_bfloat16*)a, q, scale, M, K, pitch, 1, stream);
+    else if (a_dt == GFB_F32) e = quantize_rows_launch((const float*)a, q, scale, M, K, pitch, 1, stream);
+    else return gfb_fail("gfb_linear_int8: unknown type %d", a_dt);
+    if (gfb_check(e, "gfb_linear_int8")) return 1;
+    return gfb_gemm_int8(q, scale, pitch, W, w_scale, ldw, out, out_dt, M, N, K, epi, bn, splits, stages, status, stream);
 }

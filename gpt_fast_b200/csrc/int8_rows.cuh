@@ -1,0 +1,138 @@
+// Rows of 8-bit integers with one scale each: what the 8-bit products multiply and the 8-bit cache holds.
+//
+// A row x becomes scale = m / 127, m = max |x_i|, and the integers q_i nearest to 127 x_i / m (ties to even), so that q_i scale is within
+// scale / 2 of x_i and |q_i| <= 127.  The integer is the one exact arithmetic gives for the 32-bit numbers x_i: a first 32-bit quotient is right unless it
+// lies within 1e-4 of a tie, and those few are decided by comparing 254 |x_i| with an odd multiple of m in 64 bits, where both are exact.
+// So the same numbers give the same integers in every kernel here, whatever order its code computes in.
+// A row of zeros has scale 0.  A row that holds a NaN or an infinity has scale NaN (and integers 0): it stands for NaN as a whole.
+#pragma once
+#include "common.cuh"
+
+namespace {
+
+// How a row's numbers become integers; `bits`: the largest |x_i| as its 32-bit pattern, which orders like the number and puts infinity and NaN on top.
+struct RowScale {
+    float most, lift, inv, scale;
+    bool live;                                          // finite and not all zeros
+    __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+        most = __uint_as_float(bits);
+        live = bits != 0u && bits < 0x7f800000u;
+        lift = most < 0x1p-60f ? 0x1p64f : 1.f;         // keeps the reciprocal of a tiny maximum finite
+        inv = live ? __fdiv_rn(127.f, most * lift) : 0.f;
+        scale = bits < 0x7f800000u ? __fdiv_rn(most, 127.f) : __uint_as_float(0x7fc00000u);
+    }
+    __device__ __forceinline__ int of(float x) const {
+        if (!live) return 0;
+        const float r = __fmul_rn(__fmul_rn(x, lift), inv);
+        float k = rintf(r);
+        if (fabsf(r - k) > 0.4999f) {                   // next to a tie, about one number in 5,000
+            const float a = fabsf(r), f = floorf(a);
+            const double twice = 254.0 * (double)fabsf(x), tie = (2.0 * (double)f + 1.0) * (double)most;
+            k = (twice > tie || (twice == tie && ((int)f & 1))) ? f + 1.f : f;
+            k = copysignf(k, x);
+        }
+        return (int)k;
+    }
+    // four of them in the bytes of a word
+    __device__ __forceinline__ uint32_t of4(float a, float b, float c, float d) const {
+        const uint32_t ab = __byte_perm((uint32_t)of(a), (uint32_t)of(b), 0x0040), cd = __byte_perm((uint32_t)of(c), (uint32_t)of(d), 0x0040);
+        return __byte_perm(ab, cd, 0x5410);
+    }
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
+    v = warp_max_bits(v);
+    __syncthreads();
+    if (lane == 0) scratch[warp] = v;
+    __syncthreads();
+    return warp_max_bits(lane < n ? scratch[lane] : 0u);
+}
+
+// eight neighbouring numbers from an address that is a multiple of 16 bytes
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+
+constexpr int ROW_VECTORS = 4;               // vectors of eight numbers that a thread keeps
+
+// q [R, pitch] and scale [R] of x [R, K], the columns from K to the pitch zeros.  One block per row, K a multiple of 8, rows aligned: one pass, the row in
+// registers.  It is bound by memory (8,192 rows of 4,096 bfloat16 numbers ROWS_US us, ROWS_TBS TB/s) and, where rows are few, by latency, hence
+// a thread per vector then.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+quantize_rows_vec_kernel(const T* x, int8_t* q, float* scale, int K, int pitch, int early) {
+    __shared__ uint32_t scratch[32];
+    if (early) gfb_pdl_launch();
+    gfb_pdl_wait();
+    const T* row = x + (size_t)blockIdx.x * K;
+    const int n = K >> 3;
+    float v[ROW_VECTORS][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < n) load8(row + 8 * i, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++)
+        if (threadIdx.x + k * blockDim.x < n) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = max(m, abs_bits(v[k][e]));
+        }
+    const RowScale rs(block_max_bits(m, scratch));
+    int8_t* out = q + (size_t)blockIdx.x * pitch;
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < n) *reinterpret_cast<uint2*>(out + 8 * i) = make_uint2(rs.of4(v[k][0], v[k][1], v[k][2], v[k][3]), rs.of4(v[k][4], v[k][5], v[k][6], v[k][7]));
+    }
+    if (threadIdx.x == 0) {
+        scale[blockIdx.x] = rs.scale;
+        if (pitch > K) *reinterpret_cast<uint2*>(out + K) = make_uint2(0u, 0u);      // (a pitch of whole 16 bytes is at most 8 more)
+    }
+}
+
+// The same for any K and alignment, reading the row twice.
+template <typename T>
+__global__ void __launch_bounds__(512)
+quantize_rows_kernel(const T* x, int8_t* q, float* scale, int K, int pitch, int early) {
+    __shared__ uint32_t scratch[32];
+    if (early) gfb_pdl_launch();
+    gfb_pdl_wait();
+    const T* row = x + (size_t)blockIdx.x * K;
+    uint32_t m = 0;
+    for (int i = threadIdx.x; i < K; i += blockDim.x) m = max(m, abs_bits(gfb_to_f32(row[i])));
+    const RowScale rs(block_max_bits(m, scratch));
+    int8_t* out = q + (size_t)blockIdx.x * pitch;
+    for (int i = threadIdx.x; i < pitch; i += blockDim.x) out[i] = i < K ? (int8_t)rs.of(gfb_to_f32(row[i])) : (int8_t)0;
+    if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
+}
+
+// Threads of a block for rows of n vectors: one vector each where rows are few and wait for one another's launches, as many as a thread holds otherwise.
+inline int row_threads(int R, int n) {
+    const int each = R <= 296 && n <= 1024 ? 1 : ROW_VECTORS;
+    const int t = ((n + each - 1) / each + 31) / 32 * 32;
+    return t < 64 ? 64 : t > 1024 ? 1024 : t;
+}
+
+// early: the next kernel may start while this one runs and waits for it before it reads the rows.  A product asks for its weights ahead of that wait, so rows
+// that may become weights are made with early = 0: nothing starts before they are complete.
+template <typename T>
+cudaError_t quantize_rows_launch(const T* x, int8_t* q, float* scale, int R, int K, int pitch, int early, cudaStream_t stream) {
+    const int n = K / 8, t = row_threads(R, n);
+    if (K % 8 == 0 && n <= ROW_VECTORS * t && pitch - K <= 8 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)q & 15) == 0)
+        return gfb_launch(quantize_rows_vec_kernel<T>, dim3(R), dim3(t), 0, stream, x, q, scale, K, pitch, early);
+    return gfb_launch(quantize_rows_kernel<T>, dim3(R), dim3(K >= 2048 ? 512 : 256), 0, stream, x, q, scale, K, pitch, early);
+}
+
+}  // namespace

@@ -1,73 +1,96 @@
-// Rows of 8-bit integers with one scale each: what the 8-bit products multiply and the 8-bit cache holds.
-//
-// A row x becomes scale = m / 127, m = max |x_i|, and the integers q_i nearest to 127 x_i / m (ties to even), so that q_i scale is within
-// scale / 2 of x_i and |q_i| <= 127.  The integer is the one exact arithmetic gives for the 32-bit numbers x_i: a first 32-bit quotient is right unless it
-// lies within 1e-4 of a tie, and those few are decided by comparing 254 |x_i| with an odd multiple of m in 64 bits, where both are exact.
-// So the same numbers give the same integers in every kernel here, whatever order its code computes in.
-// A row of zeros has scale 0.  A row that holds a NaN or an infinity has scale NaN (and integers 0): it stands for NaN as a whole.
-#include "common.cuh"
+// Making 8-bit integers (int8_rows.cuh says how): rows for the 8-bit products, the norm that quantises its output, and the cache of 8-bit integers, written and read
+// back.  All of it is bound by memory, and by latency in a decode step.
+#include "int8_rows.cuh"
 
 GFB_DEFINE_LAST_ERROR()
 
 namespace {
 
-// How a row's numbers become integers; `bits`: the largest |x_i| as its 32-bit pattern, which orders like the number and puts infinity and NaN on top.
-struct RowScale {
-    float most, lift, inv, scale;
-    bool live;                                          // finite and not all zeros
-    __device__ __forceinline__ explicit RowScale(uint32_t bits) {
-        most = __uint_as_float(bits);
-        live = bits != 0u && bits < 0x7f800000u;
-        lift = most < 0x1p-60f ? 0x1p64f : 1.f;         // keeps the reciprocal of a tiny maximum finite
-        inv = live ? __fdiv_rn(127.f, most * lift) : 0.f;
-        scale = bits < 0x7f800000u ? __fdiv_rn(most, 127.f) : __uint_as_float(0x7fc00000u);
-    }
-    __device__ __forceinline__ int of(float x) const {
-        if (!live) return 0;
-        const float r = __fmul_rn(__fmul_rn(x, lift), inv);
-        float k = rintf(r);
-        if (fabsf(r - k) > 0.4999f) {                   // next to a tie, about one number in 5,000
-            const float a = fabsf(r), f = floorf(a);
-            const double twice = 254.0 * (double)fabsf(x), tie = (2.0 * (double)f + 1.0) * (double)most;
-            k = (twice > tie || (twice == tie && ((int)f & 1))) ? f + 1.f : f;
-            k = copysignf(k, x);
-        }
-        return (int)k;
-    }
-};
-
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
-    v = warp_max_bits(v);
-    __syncthreads();
-    if (lane == 0) scratch[warp] = v;
-    __syncthreads();
-    return warp_max_bits(lane < n ? scratch[lane] : 0u);
-}
-
-// q [R, pitch] and scale [R] of x [R, K]; the columns from K to the pitch are zeros.  One block per row.
-template <typename T>
-__global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* x, int8_t* q, float* scale, int K, int pitch, int early) {
+// Rows of h = x * rsqrt(mean(x^2) + eps) * w in 32 bits, x float32 [T, D] with pending partial sums and picked rows as in gfb_rmsnorm.  One block per row, the row
+// in registers (D a multiple of 8, rows aligned); the weights are fetched ahead of the wait for the kernel before.
+template <typename TW>
+__global__ void __launch_bounds__(1024)
+rmsnorm_quantize_vec_kernel(float* x, const float* pending, int S, size_t slice, const TW* w, int8_t* q, float* scale, const int* rows, int D, int pitch, float eps) {
+    __shared__ float fscratch[32];
     __shared__ uint32_t scratch[32];
-    if (early) gfb_pdl_launch();
+    gfb_pdl_launch();
+    const int r = blockIdx.x, n = D >> 3;
+    uint4 wk[ROW_VECTORS][sizeof(TW) / 2];
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++) {
+        const int i = threadIdx.x + k * blockDim.x;
+#pragma unroll
+        for (int u = 0; u < (int)sizeof(TW) / 2; u++)
+            if (i < n) wk[k][u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(w) + (size_t)i * 8 * sizeof(TW) + 16 * u);
+    }
     gfb_pdl_wait();
-    const T* row = x + (size_t)blockIdx.x * K;
+    float* row = x + (size_t)(rows ? rows[r] : r) * D;
+    float v[ROW_VECTORS][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < n) load8(row + 8 * i, v[k]);
+    }
+    if (pending != nullptr) {
+        const float* p = pending + (row - x);
+        for (int s = 0; s < S; s++, p += slice) {
+            float a[ROW_VECTORS][8];
+#pragma unroll
+            for (int k = 0; k < ROW_VECTORS; k++) {
+                const int i = threadIdx.x + k * blockDim.x;
+                if (i < n) load8(p + 8 * i, a[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < ROW_VECTORS; k++)
+                if (threadIdx.x + k * blockDim.x < n) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[k][e] += a[k][e];
+                }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < n) {
+            if (pending != nullptr) {
+                *reinterpret_cast<float4*>(row + 8 * i) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+                *reinterpret_cast<float4*>(row + 8 * i + 4) = make_float4(v[k][4], v[k][5], v[k][6], v[k][7]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) ss = fmaf(v[k][e], v[k][e], ss);
+        }
+    }
+    const float rstd = rsqrtf(gfb_block_sum(ss, fscratch) / (float)D + eps);
     uint32_t m = 0;
-    for (int i = threadIdx.x; i < K; i += blockDim.x) m = max(m, abs_bits(gfb_to_f32(row[i])));
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++)
+        if (threadIdx.x + k * blockDim.x < n) {
+            float f[8];
+            load8(reinterpret_cast<const TW*>(&wk[k][0]), f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[k][e] = v[k][e] * rstd * f[e];
+                m = max(m, abs_bits(v[k][e]));
+            }
+        }
     const RowScale rs(block_max_bits(m, scratch));
-    int8_t* out = q + (size_t)blockIdx.x * pitch;
-    for (int i = threadIdx.x; i < pitch; i += blockDim.x) out[i] = i < K ? (int8_t)rs.of(gfb_to_f32(row[i])) : (int8_t)0;
-    if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
+    int8_t* out = q + (size_t)r * pitch;
+#pragma unroll
+    for (int k = 0; k < ROW_VECTORS; k++) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < n) *reinterpret_cast<uint2*>(out + 8 * i) = make_uint2(rs.of4(v[k][0], v[k][1], v[k][2], v[k][3]), rs.of4(v[k][4], v[k][5], v[k][6], v[k][7]));
+    }
+    if (threadIdx.x == 0) {
+        scale[r] = rs.scale;
+        if (pitch > D) *reinterpret_cast<uint2*>(out + D) = make_uint2(0u, 0u);
+    }
 }
 
-// The same of h = x * rsqrt(mean(x^2) + eps) * w in 32 bits, x float32 [T, D] with pending partial sums and picked rows as in gfb_rmsnorm.
+// The same for any D and alignment.
 template <typename TW>
 __global__ void __launch_bounds__(256)
-rmsnorm_quantize_kernel(float* x, const float* pending, int S, size_t slice, const TW* w,
-                        int8_t* q, float* scale, const int* rows, int D, int pitch, float eps) {
+rmsnorm_quantize_kernel(float* x, const float* pending, int S, size_t slice, const TW* w, int8_t* q, float* scale, const int* rows, int D, int pitch, float eps) {
     __shared__ float fscratch[32];
     __shared__ uint32_t scratch[32];
     gfb_pdl_launch();
@@ -107,8 +130,15 @@ __device__ __forceinline__ long long cache_row(const int* page_table, int max_pa
     return page < 0 || page >= n_pages ? -1 : (long long)page * G * page_size + (pos - pi * page_size);
 }
 
+// (x0, x1) turned by the angle of (cos, sin), every product and sum rounded by itself
+__device__ __forceinline__ void turn(float& x0, float& x1, float c, float s) {
+    const float y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s)), y1 = __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, s));
+    x0 = y0;
+    x1 = y1;
+}
+
 // Rotate q and k by the token's position, q to q_out, k and v quantised per (token, head) to the token's place in the cache.
-// One warp per head of a token; the rotation rounds each product and sum by itself.
+// One warp per head of a token, any even d and alignment; the rotation rounds each product and sum by itself.
 template <typename T>
 __global__ void __launch_bounds__(128)
 rope_append_int8_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const float* table, int table_len,
@@ -144,9 +174,7 @@ rope_append_int8_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const flo
             float x0 = gfb_to_f32(src[i0]), x1 = gfb_to_f32(src[i1]);
             if (rot && ok) {
                 const float c = table[((size_t)pos * half + i) * 2], sn = table[((size_t)pos * half + i) * 2 + 1];
-                const float y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn)), y1 = __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, sn));
-                x0 = y0;
-                x1 = y1;
+                turn(x0, x1, c, sn);
             }
             if (head < H) {
                 if (pass) continue;
@@ -162,36 +190,145 @@ rope_append_int8_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const flo
     }
 }
 
-// What the cache holds at the places of the step's tokens: k_out, v_out [T, G, d].  One block per token.
+// The same for heads of 64 and 128, aligned: one block per token, its place found once, one warp per head at a time, a lane D / 32 neighbouring numbers (D / 64 of
+// either half where pairs are halves) in one load; the loads of up to HEADS_AT_ONCE heads are in flight together.
+constexpr int APPEND_WARPS = 8, HEADS_AT_ONCE = 3;
+
+template <typename T, int N> struct alignas(N * sizeof(T)) Few { T v[N]; };
+
+// a lane's numbers to their places: side by side, or half of them here and half HALF further
+template <typename T, int N>
+__device__ __forceinline__ void put(T* dst, const Few<T, N>& o, int half, int pairing) {
+    if (pairing != 1) { *reinterpret_cast<Few<T, N>*>(dst) = o; return; }
+    Few<T, N / 2> a, b;
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) { a.v[i] = o.v[i]; b.v[i] = o.v[i + N / 2]; }
+    *reinterpret_cast<Few<T, N / 2>*>(dst) = a;
+    *reinterpret_cast<Few<T, N / 2>*>(dst + half) = b;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * APPEND_WARPS)
+rope_append_int8_vec_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const float* table, int table_len, int H, int G, int pairing, int append, int* status) {
+    constexpr int E = D / 32, HALF = D / 2;                              // numbers per lane
+    gfb_pdl_launch();
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int s = b.tok_seq[t], slot = b.slots[s], q_off = t - b.cu_seqlens[s];
+    gfb_pdl_wait();
+    const int pos = b.lengths[slot] + q_off;
+    bool ok = pos >= 0 && pos < table_len;
+    long long row = 0;
+    if (ok && append) {
+        row = cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, pos);
+        ok = row >= 0;
+    }
+    if (!ok && threadIdx.x == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, pos);
+    // where this lane's numbers are: E neighbours, or E / 2 neighbours of either half; pair i of them is (x[i0], x[i1])
+    const int at = pairing == 1 ? lane * (E / 2) : lane * E;
+    float cs[E / 2][2];
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) {
+        const float2 c = ok ? *reinterpret_cast<const float2*>(table + ((size_t)pos * HALF + lane * (E / 2) + i) * 2) : make_float2(0.f, 0.f);
+        cs[i][0] = c.x;
+        cs[i][1] = c.y;
+    }
+    const int heads = H + (append ? 2 * G : 0);
+    const T* src = qkv + (size_t)t * (H + 2 * G) * D;
+    for (int h0 = warp; h0 < heads; h0 += APPEND_WARPS * HEADS_AT_ONCE) {
+        Few<T, E / 2> raw[HEADS_AT_ONCE][2];
+#pragma unroll
+        for (int u = 0; u < HEADS_AT_ONCE; u++) {
+            const int head = h0 + u * APPEND_WARPS;
+            if (head >= heads) continue;
+            const T* p = src + (size_t)head * D;
+            if (pairing == 1) {                                          // values come the same way, as pairs (i, i + HALF) that are not rotated
+                raw[u][0] = *reinterpret_cast<const Few<T, E / 2>*>(p + at);
+                raw[u][1] = *reinterpret_cast<const Few<T, E / 2>*>(p + HALF + at);
+            } else {
+                const Few<T, E> both = *reinterpret_cast<const Few<T, E>*>(p + at);
+#pragma unroll
+                for (int i = 0; i < E; i++) raw[u][i / (E / 2)].v[i % (E / 2)] = both.v[i];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < HEADS_AT_ONCE; u++) {
+            const int head = h0 + u * APPEND_WARPS;
+            if (head >= heads) continue;
+            float x[E];
+#pragma unroll
+            for (int i = 0; i < E; i++) x[i] = gfb_to_f32(raw[u][i / (E / 2)].v[i % (E / 2)]);
+            if (head < H + G) {
+                if (pairing == 1) {
+#pragma unroll
+                    for (int i = 0; i < E / 2; i++) turn(x[i], x[i + E / 2], cs[i][0], cs[i][1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < E / 2; i++) turn(x[2 * i], x[2 * i + 1], cs[i][0], cs[i][1]);
+                }
+            }
+            if (head < H) {
+                Few<T, E> o;
+#pragma unroll
+                for (int i = 0; i < E; i++) o.v[i] = gfb_from_f32<T>(ok ? x[i] : 0.f);      // q stays defined so that later kernels read no garbage
+                put(q_out + ((size_t)t * H + head) * D + at, o, HALF, pairing);
+                continue;
+            }
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < E; i++) m = max(m, abs_bits(x[i]));
+            const RowScale rs(warp_max_bits(m));
+            if (!ok) continue;
+            const bool key = head < H + G;
+            const size_t place = (size_t)row + (size_t)(head - (key ? H : H + G)) * kv.page_size;
+            if (lane == 0) (key ? kv.k_scale : kv.v_scale)[place] = rs.scale;
+            Few<int8_t, E> o;
+#pragma unroll
+            for (int i = 0; i < E; i++) o.v[i] = (int8_t)rs.of(x[i]);
+            put((key ? kv.k_pool : kv.v_pool) + place * D + at, o, HALF, pairing);
+        }
+    }
+}
+
+// What the cache holds at the places of the step's tokens: k_out, v_out [T, G, d].  Eight numbers per thread where d allows it (wide), else one.
+template <typename TO>
+__device__ __forceinline__ void put8(TO* dst, uint2 q, float s) {
+    Few<TO, 8> o;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o.v[i] = gfb_from_f32<TO>(__fmul_rn((float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))), s));
+    *reinterpret_cast<Few<TO, 8>*>(dst) = o;
+}
+
 template <typename TO>
 __global__ void __launch_bounds__(256)
-read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d, int* status) {
+read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d, int wide, int* status) {
     gfb_pdl_launch();
-    gfb_pdl_wait();
     const int t = blockIdx.x;
-    const int s = b.tok_seq[t], slot = b.slots[s], pos = b.lengths[slot] + (t - b.cu_seqlens[s]);
+    const int s = b.tok_seq[t], slot = b.slots[s], q_off = t - b.cu_seqlens[s];
+    gfb_pdl_wait();
+    const int pos = b.lengths[slot] + q_off;
     const long long row = cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, pos);
     if (row < 0 && threadIdx.x == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, pos);
-    for (int i = threadIdx.x; i < G * d; i += blockDim.x) {
-        const int g = i / d;
-        const size_t at = (size_t)max(row, 0ll) + (size_t)g * kv.page_size;
-        const size_t e = at * d + (i - g * d);
-        const size_t o = (size_t)t * G * d + i;
-        k_out[o] = gfb_from_f32<TO>(row < 0 ? 0.f : __fmul_rn((float)kv.k_pool[e], kv.k_scale[at]));
-        v_out[o] = gfb_from_f32<TO>(row < 0 ? 0.f : __fmul_rn((float)kv.v_pool[e], kv.v_scale[at]));
+    const int step = wide ? 8 : 1, n = G * d / step;
+    for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
+        const bool key = i < n;
+        const int j = (key ? i : i - n) * step, g = j / d;
+        const size_t at = (size_t)(row < 0 ? 0 : row) + (size_t)g * kv.page_size, e = at * d + (j - g * d);
+        TO* dst = (key ? k_out : v_out) + (size_t)t * G * d + j;
+        const int8_t* pool = key ? kv.k_pool : kv.v_pool;
+        const float sc = row < 0 ? 0.f : (key ? kv.k_scale : kv.v_scale)[at];
+        if (wide) put8(dst, row < 0 ? make_uint2(0u, 0u) : *reinterpret_cast<const uint2*>(pool + e), sc);
+        else *dst = gfb_from_f32<TO>(row < 0 ? 0.f : __fmul_rn((float)pool[e], sc));
     }
 }
 
 }  // namespace
 
-// early: the next kernel may start while this one runs and waits for it before it reads the rows.  A product asks for its weights ahead of that wait, so rows
-// that may become weights are made with early = 0: nothing starts before they are complete.
 GFB_API int gfb_quantize_rows(const void* x, int dt, void* q, float* scale, int R, int K, int pitch, int early, cudaStream_t stream) {
     if (R <= 0) return 0;
     if (K <= 0 || pitch < K) return gfb_fail("gfb_quantize_rows: rows of %d numbers with a pitch of %d", K, pitch);
     cudaError_t e;
-    if (dt == GFB_BF16) e = gfb_launch(quantize_rows_kernel<__nv_bfloat16>, dim3(R), dim3(256), 0, stream, (const __nv_bfloat16*)x, (int8_t*)q, scale, K, pitch, early);
-    else if (dt == GFB_F32) e = gfb_launch(quantize_rows_kernel<float>, dim3(R), dim3(256), 0, stream, (const float*)x, (int8_t*)q, scale, K, pitch, early);
+    if (dt == GFB_BF16) e = quantize_rows_launch((const __nv_bfloat16*)x, (int8_t*)q, scale, R, K, pitch, early, stream);
+    else if (dt == GFB_F32) e = quantize_rows_launch((const float*)x, (int8_t*)q, scale, R, K, pitch, early, stream);
     else return gfb_fail("gfb_quantize_rows: unknown type %d", dt);
     return gfb_check(e, "gfb_quantize_rows");
 }
@@ -202,9 +339,14 @@ GFB_API int gfb_rmsnorm_quantize(float* x, const float* pending, int S, long sli
     if (D <= 0 || pitch < D) return gfb_fail("gfb_rmsnorm_quantize: rows of %d numbers with a pitch of %d", D, pitch);
     if (pending != nullptr && rows != nullptr) return gfb_fail("gfb_rmsnorm_quantize: pending partial sums cannot be combined with a row gather");
     cudaError_t e;
-    if (w_dt == GFB_BF16) e = gfb_launch(rmsnorm_quantize_kernel<__nv_bfloat16>, dim3(R), dim3(256), 0, stream, x, pending, S, (size_t)slice, (const __nv_bfloat16*)w, (int8_t*)q, scale, rows, D, pitch, eps);
-    else if (w_dt == GFB_F32) e = gfb_launch(rmsnorm_quantize_kernel<float>, dim3(R), dim3(256), 0, stream, x, pending, S, (size_t)slice, (const float*)w, (int8_t*)q, scale, rows, D, pitch, eps);
+    const int n = D / 8, t = row_threads(R, n);
+    const bool vec = D % 8 == 0 && n <= ROW_VECTORS * t && pitch - D <= 8 && (((uintptr_t)x | (uintptr_t)pending | (uintptr_t)w | (uintptr_t)q) & 15) == 0 && slice % 4 == 0;
+#define GO(TW) e = vec ? gfb_launch(rmsnorm_quantize_vec_kernel<TW>, dim3(R), dim3(t), 0, stream, x, pending, S, (size_t)slice, (const TW*)w, (int8_t*)q, scale, rows, D, pitch, eps) \
+                       : gfb_launch(rmsnorm_quantize_kernel<TW>, dim3(R), dim3(256), 0, stream, x, pending, S, (size_t)slice, (const TW*)w, (int8_t*)q, scale, rows, D, pitch, eps)
+    if (w_dt == GFB_BF16) GO(__nv_bfloat16);
+    else if (w_dt == GFB_F32) GO(float);
     else return gfb_fail("gfb_rmsnorm_quantize: unknown type %d", w_dt);
+#undef GO
     return gfb_check(e, "gfb_rmsnorm_quantize");
 }
 
@@ -217,6 +359,17 @@ GFB_API int gfb_rope_append_int8(const void* qkv, void* q_out, int dt, void* k_p
     if (d % 2) return gfb_fail("gfb_rope_append_int8: head_dim %d is odd", d);
     Int8KV kv{(int8_t*)k_pool, (int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages};
     GfbBatch b{cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens};
+    if ((d == 64 || d == 128) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)table) & 15) == 0) {
+        cudaError_t ve;
+#define GO(T, D) ve = gfb_launch(rope_append_int8_vec_kernel<T, D>, dim3(n_tokens), dim3(32 * APPEND_WARPS), 0, stream, (const T*)qkv, (T*)q_out, kv, b, table, table_len, H, G, pairing, append, status)
+        if (dt == GFB_BF16 && d == 128) GO(__nv_bfloat16, 128);
+        else if (dt == GFB_BF16) GO(__nv_bfloat16, 64);
+        else if (dt == GFB_F32 && d == 128) GO(float, 128);
+        else if (dt == GFB_F32) GO(float, 64);
+        else return gfb_fail("gfb_rope_append_int8: unknown type %d", dt);
+#undef GO
+        return gfb_check(ve, "gfb_rope_append_int8");
+    }
     dim3 grid(n_tokens, (H + (append ? 2 * G : 0) + 3) / 4);
     if (grid.y > 65535) return gfb_fail("gfb_rope_append_int8: %d heads exceed the grid", H + 2 * G);
     cudaError_t e;
@@ -233,9 +386,10 @@ GFB_API int gfb_read_cache_int8(void* k_pool, void* v_pool, float* k_scale, floa
     if (n_tokens <= 0) return 0;
     Int8KV kv{(int8_t*)k_pool, (int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages};
     GfbBatch b{cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens};
+    const int wide = d % 8 == 0 && (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 31) == 0;
     cudaError_t e;
-    if (dt == GFB_BF16) e = gfb_launch(read_cache_int8_kernel<__nv_bfloat16>, dim3(n_tokens), dim3(256), 0, stream, kv, b, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, G, d, status);
-    else if (dt == GFB_F32) e = gfb_launch(read_cache_int8_kernel<float>, dim3(n_tokens), dim3(256), 0, stream, kv, b, (float*)k_out, (float*)v_out, G, d, status);
+    if (dt == GFB_BF16) e = gfb_launch(read_cache_int8_kernel<__nv_bfloat16>, dim3(n_tokens), dim3(256), 0, stream, kv, b, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, G, d, wide, status);
+    else if (dt == GFB_F32) e = gfb_launch(read_cache_int8_kernel<float>, dim3(n_tokens), dim3(256), 0, stream, kv, b, (float*)k_out, (float*)v_out, G, d, wide, status);
     else return gfb_fail("gfb_read_cache_int8: unknown type %d", dt);
     return gfb_check(e, "gfb_read_cache_int8");
 }

@@ -1358,14 +1358,13 @@ class CudaKernels:
             _fail(f"{name}: rows of {r.cols} numbers need a pitch that is a multiple of 16, got {tuple(r.q.shape)}")
         _need(r.scale, torch.float32, (shape[0],), f"scales of {name}")
 
-    def quantize_rows(self, x, out, weights=True):
-        """weights=False: rows that no product takes as its weights, so that the kernel behind may start early."""
+    def quantize_rows(self, x, out):
         if x.dim() != 2:
             _fail(f"rows to quantise are [R, K], got {tuple(x.shape)}")
         _need(x, name="rows")
         self._need_rows(out, x.shape, "quantised rows")
         self._need_here(x, out.q)
-        self._call("quantize", "gfb_quantize_rows", _ptr(x), _dt(x), _ptr(out.q), _ptr(out.scale), x.shape[0], x.shape[1], out.q.shape[1], 0 if weights else 1, _stream())
+        self._call("quantize", "gfb_quantize_rows", _ptr(x), _dt(x), _ptr(out.q), _ptr(out.scale), x.shape[0], x.shape[1], out.q.shape[1], 0, _stream())
 
     def rmsnorm_int8(self, x, weight, eps, out, rows=None, pending=None):
         T, D = x.shape
@@ -1404,15 +1403,6 @@ class CudaKernels:
         if mode == "add" and out.dtype != torch.float32:
             _fail("the residual sum is kept in float32")
         self._need_here(w.q, out)
-        if not isinstance(a, Int8Rows):
-            _need(a, name="activation")
-            from . import int8_rows
-            rows = int8_rows(M, K, a.device)
-            self.quantize_rows(a, rows, weights=False)
-            a = rows
-        else:
-            self._need_rows(a, (M, K), "activation")
-            self._need_here(a.q)
         key = (M, N, K, mode, "int8")
         plan = self._plans.get(key)
         if plan is None:
@@ -1420,6 +1410,14 @@ class CudaKernels:
                 self._plans.clear()
             plan = self._plans[key] = int8_plan(M, N, K, mode, self.sm_count)
         self._label = f"linear int8 {N}x{K} {mode}"
+        if not isinstance(a, Int8Rows):
+            _need(a, name="activation")
+            self._need_here(a)
+            scratch = torch.empty(M * (-(-K // 16) * 16 + 4), dtype=torch.int8, device=a.device)
+            return self._call("gemm_int8", "gfb_linear_int8", _ptr(a), _dt(a), _ptr(scratch), _ptr(w.q), _ptr(w.scale), w.q.shape[1], _ptr(out), _dt(out),
+                              M, N, K, _EPI[mode], *plan, _ptr(self.status), _stream())
+        self._need_rows(a, (M, K), "activation")
+        self._need_here(a.q)
         self._call("gemm_int8", "gfb_gemm_int8", _ptr(a.q), _ptr(a.scale), a.q.shape[1], _ptr(w.q), _ptr(w.scale), w.q.shape[1], _ptr(out), _dt(out),
                    M, N, K, _EPI[mode], *plan, _ptr(self.status), _stream())
 
