@@ -447,8 +447,8 @@ def linear(a, w, out, mode: str = "store", defer: bool = False):
 
 def int8_rows(n_rows: int, cols: int, device) -> Int8Rows:
     """Room for `n_rows` quantised rows of `cols` numbers, not yet written."""
-    return Int8Rows(torch.empty((n_rows, -(-cols // 16) * 16), dtype=torch.int8, device=device),
-                    torch.empty(n_rows, dtype=torch.float32, device=device), cols)
+    scale = torch.empty(n_rows, dtype=torch.float32, device=device)
+    return Int8Rows(scale.new_empty((n_rows, -(-cols // 16) * 16), dtype=torch.int8), scale, cols)
 
 
 def quantize_rows(x, out: Optional[Int8Rows] = None) -> Int8Rows:

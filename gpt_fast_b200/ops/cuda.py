@@ -1339,40 +1339,53 @@ class CudaKernels:
                    _ptr(scratch), _ptr(batch.status), _ptr(lengths_early), int(batch.max_kv_len), _stream())
         return True
 
-    # -- sampling --------------------------------------------------------------------------
     # -- 8-bit integers: rows with a scale each, their products, a cache of them -----------------------------
+    # A decode step's calls cost the host more than the device: one comparison of each kind per tensor, and the explanations only where one fails.
     @staticmethod
-    def _need_here(*tensors):
+    def _need_here(here, *tensors):
         """The kernels run on the current device's current stream; their tensors have to be there."""
-        here = _device()
         for t in tensors:
-            if t.device.index != here:
+            if t.get_device() != here:
                 _fail(f"a tensor is on {t.device}, the current device is cuda:{here}")
 
-    @staticmethod
-    def _need_rows(r: Int8Rows, shape, name):
-        if r.shape != shape:
-            _fail(f"{name} must be {tuple(shape)} in 8-bit rows, got {tuple(r.shape)}")
-        _need(r.q, torch.int8, name=name)
-        if r.q.dim() != 2 or r.q.shape[1] < r.cols or r.q.shape[1] % 16:
-            _fail(f"{name}: rows of {r.cols} numbers need a pitch that is a multiple of 16, got {tuple(r.q.shape)}")
-        _need(r.scale, torch.float32, (shape[0],), f"scales of {name}")
+    def _need_fast(self, t, dtype, shape, name, here):
+        if t.dtype is dtype and t.shape == shape and t.get_device() == here and t.is_contiguous():
+            return
+        _need(t, dtype, shape, name)
+        self._need_here(here, t)
+
+    def _need_rows(self, r: Int8Rows, n, cols, name, here):
+        q, scale = r.q, r.scale
+        s = q.shape
+        if (q.dtype is torch.int8 and len(s) == 2 and s[0] == n and r.cols == cols and s[1] >= cols and s[1] % 16 == 0 and q.get_device() == here
+                and q.is_contiguous() and scale.dtype is torch.float32 and scale.shape == (n,) and scale.get_device() == here and scale.is_contiguous()):
+            return s[1]
+        if r.shape != (n, cols):
+            _fail(f"{name} must be {(n, cols)} in 8-bit rows, got {tuple(r.shape)}")
+        _need(q, torch.int8, name=name)
+        if q.dim() != 2 or s[1] < cols or s[1] % 16:
+            _fail(f"{name}: rows of {cols} numbers need a pitch that is a multiple of 16, got {tuple(s)}")
+        _need(scale, torch.float32, (n,), f"scales of {name}")
+        self._need_here(here, q, scale)
+        return s[1]
 
     def quantize_rows(self, x, out):
+        here = _device()
         if x.dim() != 2:
             _fail(f"rows to quantise are [R, K], got {tuple(x.shape)}")
+        R, K = x.shape
         _need(x, name="rows")
-        self._need_rows(out, x.shape, "quantised rows")
-        self._need_here(x, out.q)
-        self._call("quantize", "gfb_quantize_rows", _ptr(x), _dt(x), _ptr(out.q), _ptr(out.scale), x.shape[0], x.shape[1], out.q.shape[1], 0, _stream())
+        pitch = self._need_rows(out, R, K, "quantised rows", here)
+        self._need_here(here, x)
+        self._call("quantize", "gfb_quantize_rows", x.data_ptr(), _dt(x), out.q.data_ptr(), out.scale.data_ptr(), R, K, pitch, 0, _stream())
 
     def rmsnorm_int8(self, x, weight, eps, out, rows=None, pending=None):
+        here = _device()
         T, D = x.shape
         R = out.q.shape[0]
-        _need(x, torch.float32, name="norm input")
-        _need(weight, shape=(D,), name="norm weight")
-        self._need_rows(out, (R, D), "norm output")
-        self._need_here(x, out.q, weight)
+        self._need_fast(x, torch.float32, (T, D), "norm input", here)
+        self._need_fast(weight, weight.dtype, (D,), "norm weight", here)
+        pitch = self._need_rows(out, R, D, "norm output", here)
         if rows is not None:
             _need(rows, torch.int32, (R,), "rows")
             if pending is not None:
@@ -1384,96 +1397,117 @@ class CudaKernels:
         if pending is not None:
             S = pending.shape[0]
             _need(pending, torch.float32, (S, T, D), "pending partial sums")
-        self._call("quantize", "gfb_rmsnorm_quantize", _ptr(x), _ptr(pending), S, T * D, _ptr(weight), _dt(weight), _ptr(out.q), _ptr(out.scale),
-                   _ptr(rows), R, D, out.q.shape[1], eps, _stream())
+        self._call("quantize", "gfb_rmsnorm_quantize", x.data_ptr(), _ptr(pending), S, T * D, weight.data_ptr(), _dt(weight), out.q.data_ptr(),
+                   out.scale.data_ptr(), _ptr(rows), R, D, pitch, eps, _stream())
 
     MAX_INT8_K = 133144                    # 127^2 times this is the largest sum that 32 bits hold for sure
 
     def linear_int8(self, a, w, out, mode="store"):
-        M, K = a.shape
-        N = w.q.shape[0]
-        if mode not in _EPI:
+        here = _device()
+        rows = isinstance(a, Int8Rows)
+        M, K = (a.q.shape[0], a.cols) if rows else a.shape
+        wq = w.q
+        N = wq.shape[0]
+        epi = _EPI.get(mode)
+        if epi is None:
             _fail(f"unknown mode '{mode}'")
         if K > self.MAX_INT8_K:
             _fail(f"rows of {K} 8-bit numbers: from {self.MAX_INT8_K + 1} on a sum may leave 32 bits")
-        self._need_rows(w, (N, K), "weight")
-        if mode == "swiglu" and N % 2:
-            _fail(f"SwiGLU needs pairs of gate and up rows, got {N} rows")
-        _need(out, shape=(M, N // 2 if mode == "swiglu" else N), name="product output")
-        if mode == "add" and out.dtype != torch.float32:
+        w_pitch = self._need_rows(w, N, K, "weight", here)
+        No = N
+        if mode == "swiglu":
+            if N % 2:
+                _fail(f"SwiGLU needs pairs of gate and up rows, got {N} rows")
+            No = N // 2
+        out_dt = _dt(out)
+        self._need_fast(out, out.dtype, (M, No), "product output", here)
+        if epi == 1 and out_dt != 0:
             _fail("the residual sum is kept in float32")
-        self._need_here(w.q, out)
         key = (M, N, K, mode, "int8")
         plan = self._plans.get(key)
         if plan is None:
             if len(self._plans) > 4096:
                 self._plans.clear()
             plan = self._plans[key] = int8_plan(M, N, K, mode, self.sm_count)
-        self._label = f"linear int8 {N}x{K} {mode}"
-        if not isinstance(a, Int8Rows):
-            _need(a, name="activation")
-            self._need_here(a)
-            scratch = torch.empty(M * (-(-K // 16) * 16 + 4), dtype=torch.int8, device=a.device)
-            return self._call("gemm_int8", "gfb_linear_int8", _ptr(a), _dt(a), _ptr(scratch), _ptr(w.q), _ptr(w.scale), w.q.shape[1], _ptr(out), _dt(out),
-                              M, N, K, _EPI[mode], *plan, _ptr(self.status), _stream())
-        self._need_rows(a, (M, K), "activation")
-        self._need_here(a.q)
-        self._call("gemm_int8", "gfb_gemm_int8", _ptr(a.q), _ptr(a.scale), a.q.shape[1], _ptr(w.q), _ptr(w.scale), w.q.shape[1], _ptr(out), _dt(out),
-                   M, N, K, _EPI[mode], *plan, _ptr(self.status), _stream())
+        if self.trace is not None:
+            self._label = f"linear int8 {N}x{K} {mode}"
+        if not rows:
+            self._need_fast(a, a.dtype, (M, K), "activation", here)
+            scratch = wq.new_empty(M * (-(-K // 16) * 16 + 4))
+            return self._call("gemm_int8", "gfb_linear_int8", a.data_ptr(), _dt(a), scratch.data_ptr(), wq.data_ptr(), w.scale.data_ptr(), w_pitch,
+                              out.data_ptr(), out_dt, M, N, K, epi, *plan, self.status.data_ptr(), _stream())
+        a_pitch = self._need_rows(a, M, K, "activation", here)
+        self._call("gemm_int8", "gfb_gemm_int8", a.q.data_ptr(), a.scale.data_ptr(), a_pitch, wq.data_ptr(), w.scale.data_ptr(), w_pitch,
+                   out.data_ptr(), out_dt, M, N, K, epi, *plan, self.status.data_ptr(), _stream())
 
-    def _int8_kv_args(self, kv: Int8KV, n_kv, head_dim):
-        P = kv.k_pool.shape[0]
-        for pool, scale, name in ((kv.k_pool, kv.k_scale, "key"), (kv.v_pool, kv.v_scale, "value")):
-            _need(pool, torch.int8, (P, n_kv, kv.page_size, head_dim), f"{name} pool")
-            if scale is None:
-                _fail(f"a pool of 8-bit {name}s needs its scales")
-            _need(scale, torch.float32, (P, n_kv, kv.page_size), f"scales of the {name} pool")
-        _need(kv.page_table, torch.int32, name="page table")
-        return (_ptr(kv.k_pool), _ptr(kv.v_pool), _ptr(kv.k_scale), _ptr(kv.v_scale), _ptr(kv.page_table), kv.page_table.shape[1], kv.page_size, P)
+    def _int8_kv_args(self, kv: Int8KV, n_kv, head_dim, here):
+        k, v, ks, vs, table, page = kv.k_pool, kv.v_pool, kv.k_scale, kv.v_scale, kv.page_table, kv.page_size
+        if ks is None or vs is None:
+            _fail("pools of 8-bit keys and values need their scales")
+        P = k.shape[0]
+        shape = (P, n_kv, page, head_dim)
+        self._need_fast(k, torch.int8, shape, "key pool", here)
+        self._need_fast(v, torch.int8, shape, "value pool", here)
+        self._need_fast(ks, torch.float32, shape[:3], "scales of the key pool", here)
+        self._need_fast(vs, torch.float32, shape[:3], "scales of the value pool", here)
+        slots, longest = table.shape
+        self._need_fast(table, torch.int32, (slots, longest), "page table", here)
+        return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), longest, page, P)
 
     def rope_append_int8(self, qkv, q_out, kv, batch, table, n_head, n_kv, head_dim, pairing, append):
+        here = _device()
         T = batch.n_tokens
-        _need(qkv, shape=(T, (n_head + 2 * n_kv) * head_dim), name="qkv")
-        _need(q_out, qkv.dtype, (T, n_head, head_dim), "q_out")
-        _need(table, torch.float32, (table.shape[0], head_dim // 2, 2), "rotary table")
+        self._need_fast(qkv, qkv.dtype, (T, (n_head + 2 * n_kv) * head_dim), "qkv", here)
+        self._need_fast(q_out, qkv.dtype, (T, n_head, head_dim), "q_out", here)
+        P = table.shape[0]
+        self._need_fast(table, torch.float32, (P, head_dim // 2, 2), "rotary table", here)
         if pairing not in _PAIRING:
             _fail(f"unknown rotary pairing '{pairing}'")
-        self._need_here(qkv, q_out, kv.k_pool, table)
-        self._call("quantize", "gfb_rope_append_int8", _ptr(qkv), _ptr(q_out), _dt(qkv), *self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch),
-                   _ptr(table), table.shape[0], n_head, n_kv, head_dim, _PAIRING[pairing], 1 if append else 0, _ptr(batch.status), _stream())
+        self._call("quantize", "gfb_rope_append_int8", qkv.data_ptr(), q_out.data_ptr(), _dt(qkv), *self._int8_kv_args(kv, n_kv, head_dim, here),
+                   *self._batch_args(batch), table.data_ptr(), P, n_head, n_kv, head_dim, _PAIRING[pairing], 1 if append else 0, batch.status.data_ptr(), _stream())
 
     def read_cache_int8(self, kv, batch, k_out, v_out):
+        here = _device()
         T = batch.n_tokens
         n_kv, head_dim = kv.k_pool.shape[1], kv.k_pool.shape[3]
-        _need(k_out, shape=(T, n_kv, head_dim), name="keys")
-        _need(v_out, k_out.dtype, (T, n_kv, head_dim), "values")
-        self._need_here(kv.k_pool, k_out, v_out)
-        self._call("quantize", "gfb_read_cache_int8", *self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch), _ptr(k_out), _ptr(v_out),
-                   _dt(k_out), n_kv, head_dim, _ptr(batch.status), _stream())
+        self._need_fast(k_out, k_out.dtype, (T, n_kv, head_dim), "keys", here)
+        self._need_fast(v_out, k_out.dtype, (T, n_kv, head_dim), "values", here)
+        self._call("quantize", "gfb_read_cache_int8", *self._int8_kv_args(kv, n_kv, head_dim, here), *self._batch_args(batch), k_out.data_ptr(),
+                   v_out.data_ptr(), _dt(k_out), n_kv, head_dim, batch.status.data_ptr(), _stream())
 
     def attention_int8(self, q, kv, batch, out, n_head, n_kv, head_dim, scale, window=None):
+        here = _device()
         T = batch.n_tokens
         if n_kv < 1 or n_head % n_kv:
             _fail(f"{n_head} query heads do not divide into {n_kv} key/value heads")
         if window is not None and window < 1:
             _fail(f"a window of {window} positions")
-        _need(q, shape=(T, n_head, head_dim), name="q")
-        _need(out, q.dtype, (T, n_head * head_dim), "attention output")
-        self._need_here(q, out, kv.k_pool)
-        args = (*self._int8_kv_args(kv, n_kv, head_dim), *self._batch_args(batch), n_head, n_kv, head_dim, scale, window or 0)
-        if q.dtype == torch.bfloat16 and batch.max_q_len == 1 and head_dim in (64, 128) and kv.page_size == 64 and n_head // n_kv <= 8:
-            reach = batch.max_kv_len if not window else min(batch.max_kv_len, window + kv.page_size)
-            splits, blocks = int8_shares(-(-reach // kv.page_size) * kv.page_size, kv.page_size, T * n_kv, self.sm_count)
-            if T > 4096:                          # whose pages the shares kernel does not count
-                splits, blocks = 1, 0
-            scratch = torch.empty(2 * blocks * (n_head // n_kv) * (head_dim + 2) + T + 1, dtype=torch.float32, device=q.device) if blocks else None
-            return self._call("attention_int8", "gfb_attention_int8_decode", _ptr(q), _ptr(out), *args, splits, blocks, _ptr(scratch), _ptr(batch.status), _stream())
-        if q.dtype == torch.bfloat16 and head_dim in (64, 128) and kv.page_size == 64 and n_head // n_kv <= 128 and scale > 0:
-            pairs, splits = int8_parts(T, batch.n_seqs, batch.max_kv_len if not window else min(batch.max_kv_len, window + 256), n_head // n_kv, n_kv, self.sm_count)
-            scratch = torch.empty(T * n_head * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-            return self._call("attention_int8", "gfb_attention_int8_prompt", _ptr(q), _ptr(out), *args, pairs, splits, _ptr(scratch), _ptr(batch.status), _stream())
-        self._call("attention_int8", "gfb_attention_int8_generic", _ptr(q), _ptr(out), _dt(q), *args, _ptr(batch.status), _stream())
+        dtype, page, rep, reach = q.dtype, kv.page_size, n_head // n_kv, batch.max_kv_len
+        self._need_fast(q, dtype, (T, n_head, head_dim), "q", here)
+        self._need_fast(out, dtype, (T, n_head * head_dim), "attention output", here)
+        args = (*self._int8_kv_args(kv, n_kv, head_dim, here), *self._batch_args(batch), n_head, n_kv, head_dim, scale, window or 0)
+        if dtype is torch.bfloat16 and page == 64 and (head_dim == 128 or head_dim == 64):
+            if batch.max_q_len == 1 and rep <= 8:
+                if window:
+                    reach = min(reach, window + page)
+                splits, blocks = int8_shares(-(-reach // page) * page, page, T * n_kv, self.sm_count)
+                scratch = None
+                if T > 4096:                      # (whose pages the kernel of equal shares does not count)
+                    splits, blocks = 1, 0
+                elif blocks:
+                    scratch = torch.empty(2 * blocks * rep * (head_dim + 2) + T + 1, dtype=torch.float32, device=q.device)
+                return self._call("attention_int8", "gfb_attention_int8_decode", q.data_ptr(), out.data_ptr(), *args, splits, blocks, _ptr(scratch),
+                                  batch.status.data_ptr(), _stream())
+            if rep <= 128 and scale > 0:
+                if window:
+                    reach = min(reach, window + 256)
+                pairs, splits = int8_parts(T, batch.n_seqs, reach, rep, n_kv, self.sm_count)
+                scratch = torch.empty(T * n_head * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+                return self._call("attention_int8", "gfb_attention_int8_prompt", q.data_ptr(), out.data_ptr(), *args, pairs, splits, _ptr(scratch),
+                                  batch.status.data_ptr(), _stream())
+        self._call("attention_int8", "gfb_attention_int8_generic", q.data_ptr(), out.data_ptr(), _dt(q), *args, batch.status.data_ptr(), _stream())
 
+    # -- sampling --------------------------------------------------------------------------
     def argmax(self, logits, out):
         B, V = logits.shape
         _need(logits, torch.float32, name="logits")
