@@ -12,13 +12,16 @@ its own.  A mixer that asks for fixed-size state gets a [n_slots, *shape] tensor
 per entry, zeroed when a slot is handed out.  Slots and pages go back to their
 free lists when a sequence ends and are used again without clearing: nothing
 reads beyond a slot's length.
+
+With kv_dtype='int8' keys and values are 8-bit integers and every cached row (token, head) has a 32-bit scale for its key and one for its
+value: 2 d + 8 bytes per token and head instead of 4 d in bfloat16.
 """
 from dataclasses import dataclass
 from typing import Dict, Iterable, List, Optional, Sequence
 
 import torch
 
-from ..ops.types import PagedKV
+from ..ops.types import Int8KV, PagedKV
 from .needs import CacheNeeds, KVNeed, StateNeed
 from .slots import CacheFull, FreeList
 
@@ -33,18 +36,31 @@ class EntryView:
 
 
 class _KVGroup:
-    def __init__(self, need: KVNeed, entries: List[int], n_pages, n_slots, max_pages, page_size, dtype, device):
+    def __init__(self, need: KVNeed, entries: List[int], n_pages, n_slots, max_pages, page_size, dtype, device, int8=False):
+        if int8 and (not need.values or need.v_head_dim not in (None, need.head_dim)):
+            raise ValueError("a cache of 8-bit integers has values of the keys' size")
         self.need, self.entries = need, entries
         self.index = {e: i for i, e in enumerate(entries)}
         shape = (len(entries), n_pages, need.n_kv, page_size, need.head_dim)
+        if int8:
+            dtype = torch.int8
         self.k_pool = torch.zeros(shape, dtype=dtype, device=device)
         v_dim = (need.v_head_dim or need.head_dim) if need.values else 0
         self.v_pool = torch.zeros(shape[:-1] + (v_dim,), dtype=dtype, device=device)
+        self.k_scale, self.v_scale = (torch.zeros(shape[:-1], dtype=torch.float32, device=device) if int8 else None for _ in range(2))
         self.pages = FreeList(n_pages, "page")
         self.table_host = torch.full((n_slots, max_pages), -1, dtype=torch.int32)
         self.table = self.table_host.to(device)
         self.slot_pages: Dict[int, List[int]] = {}
         self.dirty = set()
+
+    def view(self, i: int, page_size: int) -> PagedKV:
+        if self.k_scale is None:
+            return PagedKV(self.k_pool[i], self.v_pool[i], self.table, page_size)
+        return Int8KV(self.k_pool[i], self.v_pool[i], self.table, page_size, k_scale=self.k_scale[i], v_scale=self.v_scale[i])
+
+    def storage(self):
+        return [t for t in (self.k_pool, self.v_pool, self.k_scale, self.v_scale) if t is not None]
 
 
 class _StateGroup:
@@ -57,12 +73,15 @@ class _StateGroup:
 class Cache:
     def __init__(self, needs: Dict[int, CacheNeeds], dtype: torch.dtype, device, *, max_tokens: int,
                  max_seqs: Optional[int] = None, max_seq_len: Optional[int] = None,
-                 page_size: int = DEFAULT_PAGE_SIZE):
+                 page_size: int = DEFAULT_PAGE_SIZE, kv_dtype: Optional[str] = None):
         """needs: cache entry id -> what its mixer asks for.
         max_tokens: the most tokens live sequences hold at once, each sequence
           rounded up to whole pages.
         max_seqs: the most live sequences (default: one per page).
-        max_seq_len: the longest one sequence may get (default: all pages)."""
+        max_seq_len: the longest one sequence may get (default: all pages).
+        kv_dtype: 'int8', or None for keys and values in `dtype`."""
+        if kv_dtype not in (None, "int8"):
+            raise ValueError(f"keys and values are cached in the model's type or as 'int8', not '{kv_dtype}'")
         if page_size <= 0 or max_tokens <= 0:
             raise ValueError("page_size and max_tokens must be positive")
         self.page_size = page_size
@@ -86,7 +105,8 @@ class Cache:
                 by_kv.setdefault(n.kv, []).append(entry)
             if n.state is not None:
                 by_state.setdefault(n.state, []).append(entry)
-        self.kv_groups = [_KVGroup(need, entries, self.n_pages, self.n_slots, self.max_pages, page_size, dtype, device)
+        self.kv_groups = [_KVGroup(need, entries, self.n_pages, self.n_slots, self.max_pages, page_size, dtype, device,
+                                   int8=kv_dtype == "int8")
                           for need, entries in by_kv.items()]
         self.state_groups = [_StateGroup(need, entries, self.n_slots, device) for need, entries in by_state.items()]
         self._views: Dict[int, EntryView] = {}
@@ -94,8 +114,7 @@ class Cache:
             v = EntryView()
             for g in self.kv_groups:
                 if entry in g.index:
-                    i = g.index[entry]
-                    v.kv = PagedKV(g.k_pool[i], g.v_pool[i], g.table, page_size)
+                    v.kv = g.view(g.index[entry], page_size)
             for g in self.state_groups:
                 if entry in g.index:
                     v.state = g.data[g.index[entry]]
@@ -174,9 +193,8 @@ class Cache:
         return min((g.pages.n_free for g in self.kv_groups), default=self.n_pages)
 
     def bytes(self) -> int:
-        n = sum((g.k_pool.numel() + g.v_pool.numel()) * g.k_pool.element_size() for g in self.kv_groups)
+        n = sum(t.numel() * t.element_size() for g in self.kv_groups for t in g.storage())
         return n + sum(g.data.numel() * g.data.element_size() for g in self.state_groups)
 
     def kv_bytes_per_token(self) -> int:
-        return sum(len(g.entries) * g.need.n_kv * (g.need.head_dim + g.v_pool.shape[-1]) * g.k_pool.element_size()
-                   for g in self.kv_groups)
+        return sum(t[:, 0, :, 0].numel() * t.element_size() for g in self.kv_groups for t in g.storage())

@@ -134,7 +134,7 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity)
     return ok;
 }
 // Wait for the phase with `parity` to complete; false when the block gives up or time runs out.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int which) {
+__device__ __forceinline__ bool lane_waits(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int which) {
     if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long t0 = global_ns();
     for (;;) {
@@ -149,8 +149,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 // The same for a whole warp: one answer for all its lanes, which meet again at the aligned instructions behind it.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int which) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up, status, which));
+__device__ __forceinline__ bool warp_waits(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int which) {
+    return __all_sync(0xffffffffu, lane_waits(bar, parity, gave_up, status, which));
 }
 __device__ __forceinline__ uint64_t l2_evict_first_policy() {
     uint64_t pol;
@@ -415,7 +415,7 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             for (int i = 0; i < n; i++) {
                 const int st = i % NS, page = next;
                 next = i + 1 < n && p0 + i + 1 < kv.max_pages ? pt[p0 + i + 1] : -1;
-                if (i >= NS && !mbar_wait(bar0 + 16 * st + 8, ((i / NS) & 1) ^ 1, gave_up, status, 301)) break;
+                if (i >= NS && !lane_waits(bar0 + 16 * st + 8, ((i / NS) & 1) ^ 1, gave_up, status, 301)) break;
                 fetch_page<D>(&map_k, &map_v, kv, G, g, page, slot, p0 + i, tiles + st * S::STAGE, tiles + S::SCALES + st * 2 * PAGE * 4, bar0 + 16 * st, dead + st,
                               pol, status);
             }
@@ -428,7 +428,7 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         int st = 0, j0 = p0 * PAGE;
         uint32_t ph = 0;
         for (int i = 0; i < n; i++, j0 += PAGE) {
-            if (!mbar_wait_warp(bar0 + 16 * st, ph, gave_up, status, 300)) break;
+            if (!warp_waits(bar0 + 16 * st, ph, gave_up, status, 300)) break;
             rows.page_at(tiles + st * S::STAGE, off, scales + st * 2 * PAGE + warp * 16 + g4, j0, j0 + warp * 16 + g4, lo, pos, dead[st] != 0);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar0 + 16 * st + 8);
@@ -638,7 +638,7 @@ attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     for (int i = 0; i < n; i++) {
                         const int page = next;
                         next = i + 1 < n && p0 + i + 1 < kv.max_pages ? pt[p0 + i + 1] : -1;
-                        if (again && !mbar_wait(bar0 + 16 * st + 8, ph ^ 1u, gave_up, status, 303)) break;
+                        if (again && !lane_waits(bar0 + 16 * st + 8, ph ^ 1u, gave_up, status, 303)) break;
                         fetch_page<D>(&map_k, &map_v, kv, G, g, page, seen.slot, p0 + i, tiles + st * S::STAGE, tiles + S::SCALES + st * 2 * PAGE * 4, bar0 + 16 * st,
                                       dead + st, pol, status);
                         if (++st == NS) { st = 0; ph ^= 1u; again = true; }
@@ -651,7 +651,7 @@ attention_int8_shares_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 int j0 = (seen.first + p) * PAGE, last = st;
                 for (int i = 0; i < n; i++, j0 += PAGE) {
                     last = st;
-                    if (mbar_wait_warp(bar0 + 16 * st, ph, gave_up, status, 302)) {
+                    if (warp_waits(bar0 + 16 * st, ph, gave_up, status, 302)) {
                         rows.page_at(tiles + st * S::STAGE, off, scales + st * 2 * PAGE + warp * 16 + g4, j0, j0 + warp * 16 + g4, seen.lo, seen.pos, dead[st] != 0);
                         __syncwarp();
                         if (lane == 0 && i + 1 < n) mbar_arrive(bar0 + 16 * st + 8);
@@ -1129,7 +1129,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 uint32_t factor = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
                 if (odd) factor = is_v ? 0u : 0x7fff7fffu;
                 const int2 after = pages_of(U + 2 * CONV_WARPS);
-                ok = mbar_wait_warp(smem_u32(is_v ? &bars->v_empty[s] : &bars->k_empty[s]), ((uint32_t)(gj / KV_STAGES) & 1u) ^ 1u, gave_up, status, 401);
+                ok = warp_waits(smem_u32(is_v ? &bars->v_empty[s] : &bars->k_empty[s]), ((uint32_t)(gj / KV_STAGES) & 1u) ^ 1u, gave_up, status, 401);
                 if (!ok) break;
                 uint8_t* line = smem + (is_v ? S::V : S::K) + s * TILE + (c >> 2) * HALF_BYTES + (group * 32 + sub) * 128;
                 const int even = ((2 * (c & 3)) ^ (sub & 7)) << 4, odd_row = RPI == 4 ? even ^ 64 : even;      // (rows 4 further exchange pieces 4 further)
@@ -1174,7 +1174,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             bool ok = true;
             for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
                 if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window) || it.n == 0) continue;
-                for (int x = 0; x < 2 && ok; x++) ok = mbar_wait(smem_u32(&bars->q_full[x]), n_item & 1u, gave_up, status, 403);
+                for (int x = 0; x < 2 && ok; x++) ok = lane_waits(smem_u32(&bars->q_full[x]), n_item & 1u, gave_up, status, 403);
                 n_item++;
                 uint32_t mine[2] = {0, 0};                               // of this item
                 auto issue_s = [&](int x, int j) {
@@ -1187,7 +1187,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                     umma_commit(smem_u32(&bars->s_full[x]));
                 };
                 auto k_ready = [&](int j) {
-                    return mbar_wait(smem_u32(&bars->k_full[(g0 + j) % KV_STAGES]), (uint32_t)((g0 + j) / KV_STAGES) & 1u, gave_up, status, 404);
+                    return lane_waits(smem_u32(&bars->k_full[(g0 + j) % KV_STAGES]), (uint32_t)((g0 + j) / KV_STAGES) & 1u, gave_up, status, 404);
                 };
                 auto scores_issued = [&](int j) {                        // K of block j is free when they are done, and behind the last block Q is
                     umma_commit(smem_u32(&bars->k_empty[(g0 + j) % KV_STAGES]));
@@ -1206,11 +1206,11 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 for (int j = 0; j < it.n && ok; j++) {
                     const int s = (g0 + j) % KV_STAGES;
                     bool k_next = false;                                 // whether K of block j + 1 has been waited for
-                    ok = mbar_wait(smem_u32(&bars->v_full[s]), (uint32_t)((g0 + j) / KV_STAGES) & 1u, gave_up, status, 405);
+                    ok = lane_waits(smem_u32(&bars->v_full[s]), (uint32_t)((g0 + j) / KV_STAGES) & 1u, gave_up, status, 405);
 #pragma unroll
                     for (int x = 0; x < 2 && ok; x++) {
                         if (it.active(x, j)) {
-                            ok = mbar_wait(smem_u32(&bars->p_ready[x]), n_pv[x] & 1u, gave_up, status, 406);
+                            ok = lane_waits(smem_u32(&bars->p_ready[x]), n_pv[x] & 1u, gave_up, status, 406);
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll
@@ -1253,7 +1253,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             if (it.n > 0) {
                 const int tq = r / rep;
                 const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
-                ok = ok && mbar_wait_warp(smem_u32(&bars->q_empty[x]), (n_item & 1u) ^ 1u, gave_up, status, 411);
+                ok = ok && warp_waits(smem_u32(&bars->q_empty[x]), (n_item & 1u) ^ 1u, gave_up, status, 411);
                 n_item++;
                 unit = put_query<D>(smem + x * TILE, r, tq < it.nq[x] ? q + at * D : nullptr, scale_log2e, half * (D / 2), D / 2);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1276,8 +1276,8 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
 #pragma unroll 1
             for (; j < end; j++, top -= KEYS, low -= KEYS) {
                 const Refs& ref = refs[(g0 + j) & (SC_STAGES - 1)];
-                ok = ok && mbar_wait_warp(smem_u32(&bars->sc_full[(g0 + j) & (SC_STAGES - 1)]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
-                     && mbar_wait_warp(smem_u32(&bars->s_full[x]), n_done & 1u, gave_up, status, 408);
+                ok = ok && warp_waits(smem_u32(&bars->sc_full[(g0 + j) & (SC_STAGES - 1)]), (uint32_t)((g0 + j) / SC_STAGES) & 1u, gave_up, status, 407)
+                     && warp_waits(smem_u32(&bars->s_full[x]), n_done & 1u, gave_up, status, 408);
                 if (!ok) { meet(); continue; }
                 tc_fence_after();
                 const int gone = ref.missing[2 * half] | (ref.missing[2 * half + 1] << 1);       // 32 keys without a page: rare
@@ -1331,7 +1331,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 l = fmaf(l, corr, ((s0 + s1) + (s2 + s3)) * ref.inv_v_ref);
                 // O follows the reference, rarely (S of this block was issued behind the tile's previous W V, so that phase is over)
                 if (was != (int)n_done && __any_sync(0xffffffffu, corr != 1.f)) {
-                    ok = mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
+                    ok = warp_waits(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D / 64; c++) {
@@ -1354,7 +1354,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             meet();
             l = half ? *other_at + l : l + *other_at;
             meet();
-            if (some) ok = ok && mbar_wait_warp(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
+            if (some) ok = ok && warp_waits(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
             if (ok) {
                 tc_fence_after();
                 it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window);

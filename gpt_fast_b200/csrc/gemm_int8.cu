@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity)
     return ok;
 }
 // Wait for the phase with `parity` to complete; false when the block aborts or time runs out.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int which) {
+__device__ __forceinline__ bool lane_waits(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int which) {
     if (mbar_try_wait(bar, parity)) return true;
     unsigned long long t0 = global_ns();
     for (;;) {
@@ -80,8 +80,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 // The same for a whole warp: one answer for all its lanes.  Where a wait runs out lanes can differ (one sees the abort flag, another its barrier), and
 // a warp that parted there would never meet again at the aligned instructions behind it.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int which) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, which));
+__device__ __forceinline__ bool warp_waits(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int which) {
+    return __all_sync(0xffffffffu, lane_waits(bar, parity, abort_flag, status, which));
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -295,7 +295,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             for (int i = n_pre; i < nkb; i++) {
                 const int s = i % stages;
                 const uint32_t ph = (uint32_t)(i / stages) & 1u;
-                if (!mbar_wait(smem_u32(&bars->empty[s]), ph ^ 1u, abort_flag, status, 1)) break;
+                if (!lane_waits(smem_u32(&bars->empty[s]), ph ^ 1u, abort_flag, status, 1)) break;
                 const uint32_t full = smem_u32(&bars->full[s]);
                 mbar_expect_tx(full, X_TILE_BYTES + Y_TILE_BYTES);
                 tma_load_2d_hint(xs + s * X_TILE_BYTES, &map_w, (kb0 + i) * BK, row0, full, pol);
@@ -309,7 +309,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             for (int i = 0; i < nkb && ok; i++) {
                 const int s = i % stages;
                 const uint32_t ph = (uint32_t)(i / stages) & 1u;
-                ok = mbar_wait(smem_u32(&bars->full[s]), ph, abort_flag, status, 2);
+                ok = lane_waits(smem_u32(&bars->full[s]), ph, abort_flag, status, 2);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t da = umma_smem_desc(xs + s * X_TILE_BYTES);
@@ -324,7 +324,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     } else {
         // The tile goes through shared memory (the ring is free by then): [tokens][128 rows], so that a warp finishes a token's 128 rows side by side.
         const int q = warp & 3;                             // tensor-memory lanes 32q .. 32q+31 belong to this warp
-        const bool ok = mbar_wait_warp(smem_u32(&bars->accum), 0, abort_flag, status, 3);
+        const bool ok = warp_waits(smem_u32(&bars->accum), 0, abort_flag, status, 3);
         tc_fence_after();
         uint32_t* tile = reinterpret_cast<uint32_t*>(aligned);
         if (ok) {
@@ -554,7 +554,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             for (int it = 0; it < total; it++) {
                 const uint32_t full = smem_u32(&bars->full[s]) & PEER_MASK;        // the leader's barrier
                 if (it >= n_pre) {
-                    if (!mbar_wait(smem_u32(&bars->empty[s]), ph ^ 1u, abort_flag, status, 1)) break;
+                    if (!lane_waits(smem_u32(&bars->empty[s]), ph ^ 1u, abort_flag, status, 1)) break;
                     if (leader) mbar_expect_tx(smem_u32(&bars->full[s]), 2 * PAIR_STAGE_BYTES);
                     tma_load_2d_pair(ys + s * X_TILE_BYTES, &map_w, kb * BK, wrow0, full);
                 }
@@ -576,12 +576,12 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             bool ok = true;
             for (int ti = 0; ti < my_tiles && ok; ti++) {
                 const int ab = ti & 1;
-                ok = mbar_wait(smem_u32(&bars->acc_empty[ab]), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag, status, 4);
+                ok = lane_waits(smem_u32(&bars->acc_empty[ab]), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag, status, 4);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t acc = tmem + (uint32_t)(ab * 256);
                 for (int kb = 0; kb < nkb; kb++) {
-                    ok = mbar_wait(smem_u32(&bars->full[s]), ph, abort_flag, status, 2);
+                    ok = lane_waits(smem_u32(&bars->full[s]), ph, abort_flag, status, 2);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t da = umma_smem_desc(xs + s * X_TILE_BYTES);
@@ -603,7 +603,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             const int row0 = (tile % row_tiles) * 256 + (int)rank * 128 + q * 32, col0 = (tile / row_tiles) * 256;
             const int rows = min(32, M - row0);
             const float sm = lane < rows ? a_scale[row0 + lane] : 0.f;
-            if (!mbar_wait_warp(smem_u32(&bars->acc_full[ab]), (uint32_t)(ti >> 1) & 1u, abort_flag, status, 3)) break;
+            if (!warp_waits(smem_u32(&bars->acc_full[ab]), (uint32_t)(ti >> 1) & 1u, abort_flag, status, 3)) break;
             tc_fence_after();
             const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * 256);
 #pragma unroll 1

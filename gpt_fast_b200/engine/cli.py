@@ -55,6 +55,8 @@ def build_parser():
     p.add_argument("--random_weights", action="store_true", help="Seeded random weights instead of a checkpoint")
     p.add_argument("--seed", type=int, default=1234, help="Seed of sampling (and of random weights/prompts)")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--weight_dtype", choices=["int8"], default=None, help="Weights of mixers and feed-forwards as 8-bit integers, quantised on load")
+    p.add_argument("--cache_dtype", choices=["int8"], default=None, help="Keys and values cached as 8-bit integers")
     p.add_argument("--stop_token", type=int, action="append", default=None, help="Stop token id (repeatable)")
     p.add_argument("--no_cuda_graph", action="store_true", help="Run decode steps without a CUDA graph")
     p.add_argument("--max_seq", type=int, default=None,
@@ -102,11 +104,12 @@ def main(argv=None) -> int:
             source = a.model_name or (str(a.checkpoint_path) if a.checkpoint_path else None)
             if source is None:
                 return _fail("--random_weights needs --model_name or a folder with config.json")
-            model = gf.load(source, dtype=a.dtype, device=a.device, random_weights=True, seed=a.seed)
+            model = gf.load(source, dtype=a.dtype, device=a.device, random_weights=True, seed=a.seed, weight_dtype=a.weight_dtype,
+                            cache_dtype=a.cache_dtype)
         else:
             if a.checkpoint_path is None or not a.checkpoint_path.is_dir():
                 return _fail(f"--checkpoint_path must be a model folder, got {a.checkpoint_path}")
-            model = gf.load(str(a.checkpoint_path), dtype=a.dtype, device=a.device)
+            model = gf.load(str(a.checkpoint_path), dtype=a.dtype, device=a.device, weight_dtype=a.weight_dtype, cache_dtype=a.cache_dtype)
     except (gf.ConfigError, gf.WeightError, FileNotFoundError) as e:
         return _fail(f"cannot load the model: {e}")
     torch.cuda.synchronize()
@@ -144,8 +147,7 @@ def main(argv=None) -> int:
                             max_seqs=batch, max_seq_len=max_seq)
 
     model_size = model.weight_bytes()
-    itemsize = 2 if a.dtype == "bfloat16" else 4
-    params = model_size // itemsize
+    params = model.weight_count()
     hbm_peak, peak_source = _hbm_peak(a.hbm_peak_gbs)
     kv_per_token = cache.kv_bytes_per_token()
     tokens_per_sec = []

@@ -15,12 +15,15 @@ from .model import Transformer, compute_dtype
 
 
 def load(source: Union[str, os.PathLike, dict], dtype="bfloat16", device="cuda", *, random_weights: bool = False,
-         seed: int = 0, n_layers: Optional[int] = None, progress=None) -> Transformer:
+         seed: int = 0, n_layers: Optional[int] = None, progress=None, weight_dtype: Optional[str] = None,
+         cache_dtype: Optional[str] = None) -> Transformer:
     """source: a model folder (config.json + safetensors), or, with
     random_weights=True, a folder with only config.json, a config dict, or the
     name of a named size (`config.registry.named_configs()`).
     n_layers: build only the first n layers (for measurements on less memory;
-    only with random weights)."""
+    only with random weights).
+    weight_dtype='int8': the weights of mixers and feed-forwards as 8-bit integers with a scale per output (quantised here, from the
+    checkpoint's numbers in `dtype`); cache_dtype='int8': keys and values cached as 8-bit integers with a scale per token and head."""
     if isinstance(source, dict):
         cfg, folder = dict(source), None
     elif os.path.isdir(os.fspath(source)):
@@ -40,7 +43,7 @@ def load(source: Union[str, os.PathLike, dict], dtype="bfloat16", device="cuda",
     spec = arch.build_spec(args, *extra)
     plan = arch.weight_plan(args, *extra)
     dt = compute_dtype(dtype)
-    model = Transformer(spec, dt, device)
+    model = Transformer(spec, dt, device, weight_dtype, cache_dtype)
     if random_weights:
         dev = torch.device(device)
         ckpt = RandomCheckpoint(plan, seed, gen_device=dev if dev.type == "cuda" else "cpu")

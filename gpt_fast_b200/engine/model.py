@@ -13,8 +13,9 @@ import torch
 
 from .. import ops
 from ..cache import Cache, CacheNeeds, EntryView
+from ..config.args import ConfigError
 from ..config.spec import ModelSpec, PartSpec
-from ..ops.types import BatchMeta
+from ..ops.types import BatchMeta, Int8Rows
 from ..parts.residual import Residual
 from ..parts.streams import Streams
 from ..parts import EMBEDDINGS, JUNCTIONS, NORMS, POSITIONS, build_block, build_part
@@ -35,9 +36,21 @@ def compute_dtype(dtype) -> torch.dtype:
     return COMPUTE_DTYPES[dtype]
 
 
+def _int8_or_none(value, what):
+    if value not in (None, "int8"):
+        raise ValueError(f"{what} '{value}': 'int8', or None for the model's own type")
+    return value
+
+
 class Transformer:
-    def __init__(self, spec: ModelSpec, dtype=torch.bfloat16, device="cuda"):
+    def __init__(self, spec: ModelSpec, dtype=torch.bfloat16, device="cuda", weight_dtype: Optional[str] = None,
+                 cache_dtype: Optional[str] = None):
+        """weight_dtype='int8': the matrices of mixers and feed-forwards are 8-bit integers with a scale per output, quantised as they are
+        loaded; their products quantise the activations per token.  Embedding, norms and the output product keep the model's type.
+        cache_dtype='int8': keys and values are cached as 8-bit integers with a scale per token and head.
+        A model with a part that has no such form is refused."""
         spec.validate()
+        self.weight_dtype, self.cache_dtype = _int8_or_none(weight_dtype, "weight_dtype"), _int8_or_none(cache_dtype, "cache_dtype")
         self.spec = spec
         self.dtype = compute_dtype(dtype)
         self.device = torch.device(device)
@@ -59,6 +72,13 @@ class Transformer:
         self.positions = [obj for _, obj in positions]
         if any(getattr(b, "takes_streams", False) != bool(spec.streams) for b in self.blocks):
             raise ValueError("a model with several residual streams is made of blocks that take streams, any other model of blocks that do not")
+        for i, b in enumerate(self.blocks):
+            for role, part in b.parts().items():
+                kind = b.roles.get(role)
+                if self.weight_dtype and kind in ("mixer", "feed_forward") and not hasattr(part, "quantize"):
+                    raise ConfigError(f"layer {i}: the {role} ({type(part).__name__}) has no form with 8-bit weights")
+                if self.cache_dtype and kind == "mixer" and not getattr(part, "int8_cache", part.cache_needs().kv is None):
+                    raise ConfigError(f"layer {i}: the {role} ({type(part).__name__}, with its options) cannot read keys and values of 8-bit integers")
         self.final_norm = build_part(NORMS, spec.final_norm, dtype=self.dtype)
         self.embedding = None if spec.embedding is None else build_part(EMBEDDINGS, spec.embedding, dtype=self.dtype)
         self.junctions = [build_part(JUNCTIONS, ps, dtype=self.dtype) for ps in spec.junctions]
@@ -112,12 +132,16 @@ class Transformer:
         for i, b in enumerate(self.blocks):
             for pname, part in b.parts().items():
                 part.load(sub(f"layers.{i}.{pname}."))
+                if self.weight_dtype and b.roles.get(pname) in ("mixer", "feed_forward"):
+                    part.quantize()
                 if hasattr(part, "bind_token_table"):
                     part.bind_token_table(self.token_table)
 
     def export_params(self) -> Dict[str, torch.Tensor]:
         """Every parameter under the name and in the layout of `param_specs` (the inverse of `load_params`);
         each part gives its own back through `export()`."""
+        if self.weight_dtype:
+            raise ValueError("a model whose weights were quantised has its parameters no more")
         out = {"embed.weight": self.embed_weight, "head.weight": self.head_weight}
         for name, t in self.final_norm.export().items():
             out[f"final_norm.{name}"] = t
@@ -147,13 +171,21 @@ class Transformer:
 
     def weight_bytes(self, with_embedding=False) -> int:
         """Bytes of the parameters a decode step streams (every matrix once)."""
-        seen, total = set(), 0
+        return self._weights(with_embedding)[0]
 
-        def add(t):
-            nonlocal total
+    def weight_count(self) -> int:
+        """The numbers among those parameters (the scales of 8-bit rows are not counted)."""
+        return self._weights()[1]
+
+    def _weights(self, with_embedding=False):
+        seen, total, count = set(), 0, 0
+
+        def add(t, numbers=None):
+            nonlocal total, count
             if t is not None and t.data_ptr() not in seen:
                 seen.add(t.data_ptr())
                 total += t.numel() * t.element_size()
+                count += t.numel() if numbers is None else numbers
         add(self.head_weight)
         if self.token_table is not None:
             seen.add(self.token_table.data_ptr())          # a row per token, not the table
@@ -164,6 +196,9 @@ class Transformer:
                 for v in vars(part).values():
                     if isinstance(v, torch.Tensor):
                         add(v)
+                    elif isinstance(v, Int8Rows):
+                        add(v.q, v.q.shape[0] * v.cols)
+                        add(v.scale, 0)
         for part in self.junctions:
             for v in vars(part).values():
                 if isinstance(v, torch.Tensor):
@@ -171,7 +206,7 @@ class Transformer:
         for v in vars(self.final_norm).values():
             if isinstance(v, torch.Tensor):
                 add(v)
-        return total
+        return total, count
 
     # ---- cache ---------------------------------------------------------------------
     def cache_needs(self) -> Dict[int, CacheNeeds]:
@@ -191,6 +226,8 @@ class Transformer:
         elif limit and max_seq_len > limit:
             raise ValueError(f"max_seq_len {max_seq_len} exceeds the model's longest sequence {limit}")
         kw = {} if page_size is None else {"page_size": page_size}
+        if self.cache_dtype:
+            kw["kv_dtype"] = self.cache_dtype
         cache = Cache(self.cache_needs(), self.dtype, self.device, max_tokens=max_tokens, max_seqs=max_seqs,
                       max_seq_len=max_seq_len, **kw)
         for p in self.positions:

@@ -14,7 +14,8 @@ sees the model's configuration.  Eight kinds, one registry each:
     JUNCTIONS      forward(x, x0, turn): what happens to the stream ahead of a layer run that the schedule marks
 
 Every part also has `param_specs()` (name -> weights.loader.ParamSpec) and
-`load(tensors)`.  Mixers and feed-forwards ADD their result into `residual`, the
+`load(tensors)`; one with matrices that may be 8-bit integers has `quantize()`, called behind `load`, and a mixer whose keys and
+values may be cached so says `int8_cache = True`.  Mixers and feed-forwards ADD their result into `residual`, the
 step's residual stream (`parts.residual.Residual`, float32):
 `residual.add_linear(a, w)` folds the sum into the product's kernel (or defers
 it to the next norm), `residual.add(y)` is for parts that cannot fuse.

@@ -114,9 +114,11 @@ class Attention:
                 raise ValueError(f"a distance bias is of kind 'slopes' or 'table', not {kind!r}")
         extras = (self.qk_norm_whole or self.conv_taps or self.distance_bias is not None or gate is not None or self.shared_kv
                   or self.values_are_keys or self.softcap is not None or self.keep_first or self.has_bias or self.sink_value is not None)
+        self.int8_weights = False
         self.plain = (position is not None and self.v_head_dim == head_dim and self.qk_norm_eps is None
                       and chunk is None and not self.has_sink and getattr(position, "head_dim", head_dim) == head_dim
                       and not extras)
+        self.int8_cache = self.plain             # whether keys and values may be cached as 8-bit integers
         self.wqkv = self.wo = self.q_norm = self.k_norm = self.sink = None
         self.conv = self.bias_table = self.slopes = self.qkv_bias = None
         # columns of the fused projection: q, then k and v (unless shared), then the gates
@@ -188,6 +190,10 @@ class Attention:
                     reach = min(reach, int(self.window))
                 pick = torch.tensor([distance_bucket(n, rows_, far) for n in range(max(reach, 1))], dtype=torch.long)
                 self.bias_table = tensors["rel"].float().cpu()[pick].contiguous().to(dev)
+
+    def quantize(self):
+        """The matrices as 8-bit integers with a scale per output; the other parameters stay as they are."""
+        self.wqkv, self.wo, self.int8_weights = ops.quantize_rows(self.wqkv), ops.quantize_rows(self.wo), True
 
     def export(self):
         """The parameters as `load` received them (the way back from the fused layout)."""

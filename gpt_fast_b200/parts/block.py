@@ -12,8 +12,10 @@ the kind of part that fills it ('mixer', 'feed_forward', 'norm': the registries 
 and hands them over as a dict; mixers also receive the layer's position encoding."""
 import torch
 
+from .. import ops
 from ..weights.loader import ParamSpec
 from . import register_block
+from .norm import RMSNorm
 from .residual import Branch, as_residual
 from .streams import StreamMix, Streams
 
@@ -48,17 +50,24 @@ class PreNormBlock:
         """What one run of this layer keeps per sequence (its mixer's keys/values or state)."""
         return self.mixer.cache_needs()
 
+    def _input(self, x, norm, sublayer, h=None):
+        """norm(x) as the sublayer reads it (in `h` where that fits): 8-bit rows for 8-bit weights, where the norm can write them."""
+        if getattr(sublayer, "int8_weights", False) and isinstance(norm, RMSNorm):
+            h = ops.int8_rows(x.x.shape[0], self.dim, x.x.device)
+        elif h is None or h.dtype != self.dtype:
+            h = torch.empty(x.x.shape[0], self.dim, dtype=self.dtype, device=x.x.device)
+        return norm.forward(x, h)
+
     def forward(self, x, batch, view, append: bool = True):
         """x: the residual stream (`parts.residual.Residual`), updated in place."""
         x = as_residual(x)
-        h = torch.empty(x.x.shape[0], self.dim, dtype=self.dtype, device=x.x.device)
-        self.mixer_norm.forward(x, h)
+        h = self._input(x, self.mixer_norm, self.mixer)
         y = x if self.mixer_scale is None else Branch(x.x.shape[0], self.dim, x.x.device)
         self.mixer.forward(h, batch, view, residual=y, append=append)
         if self.mixer_scale is not None:
             x.add_scaled(y, self.mixer_scale.weight)
         if self.feed_forward is not None:
-            self.ffn_norm.forward(x, h)
+            h = self._input(x, self.ffn_norm, self.feed_forward, h)
             y = x if self.ffn_scale is None else Branch(x.x.shape[0], self.dim, x.x.device)
             self.feed_forward.forward(h, residual=y)
             if self.ffn_scale is not None:

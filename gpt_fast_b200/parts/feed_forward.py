@@ -16,6 +16,7 @@ class SwiGLU:
     def __init__(self, dim: int, hidden: int, dtype: torch.dtype):
         self.dim, self.hidden, self.dtype = dim, hidden, dtype
         self.w13 = self.w2 = None
+        self.int8_weights = False
 
     def param_specs(self):
         return {"w1": ParamSpec((self.hidden, self.dim)), "w3": ParamSpec((self.hidden, self.dim)),
@@ -24,6 +25,10 @@ class SwiGLU:
     def load(self, tensors):
         self.w13 = torch.stack([tensors["w1"], tensors["w3"]], dim=1).reshape(2 * self.hidden, self.dim).contiguous()
         self.w2 = tensors["w2"]
+
+    def quantize(self):
+        """Both matrices as 8-bit integers with a scale per output."""
+        self.w13, self.w2, self.int8_weights = ops.quantize_rows(self.w13), ops.quantize_rows(self.w2), True
 
     def export(self):
         """The parameters as `load` received them (gate and up rows taken apart again)."""
@@ -49,12 +54,17 @@ class Dense:
             raise ValueError(f"unknown activation '{activation}'; known: {self.ACTIVATIONS}")
         self.dim, self.hidden, self.dtype, self.activation = dim, hidden, dtype, activation
         self.up = self.down = None
+        self.int8_weights = False
 
     def param_specs(self):
         return {"up": ParamSpec((self.hidden, self.dim)), "down": ParamSpec((self.dim, self.hidden))}
 
     def load(self, tensors):
         self.up, self.down = tensors["up"], tensors["down"]
+
+    def quantize(self):
+        """Both matrices as 8-bit integers with a scale per output."""
+        self.up, self.down, self.int8_weights = ops.quantize_rows(self.up), ops.quantize_rows(self.down), True
 
     def export(self):
         return {"up": self.up, "down": self.down}

@@ -4,6 +4,7 @@ all: the stream in the compute type, for sublayers that read it as it is."""
 import torch
 
 from .. import ops
+from ..ops.types import Int8Rows
 from ..weights.loader import ParamSpec
 from . import register_norm
 from .residual import Residual
@@ -51,12 +52,14 @@ class RMSNorm:
         [T, dim]) -> out [R, dim] in the compute dtype; `rows` (int32 [R]) picks
         input rows, else R = T.  Partial sums pending on the stream are added
         by the same kernel, and so are a branch with a root-mean-square norm of its own or scaled branches.  A weighted sum of
-        several streams (a `StreamRead`) is made, and the update they are owed done, by the same kernel as well."""
+        several streams (a `StreamRead`) is made, and the update they are owed done, by the same kernel as well.
+        out an `Int8Rows`: the rows are quantised by the norm's kernel; what the stream owes besides partial sums is added ahead of it."""
         if isinstance(x, StreamRead):
             x.into(out, self.weight, self.eps, rows)
         elif isinstance(x, Residual):
-            branch = _owed_rms_branch(x, rows)
-            scaled = _owed_scaled(x, rows) if branch is None else None
+            int8 = isinstance(out, Int8Rows)
+            branch = None if int8 else _owed_rms_branch(x, rows)
+            scaled = _owed_scaled(x, rows) if branch is None and not int8 else None
             if branch is not None:
                 ops.layernorm(x.x, self.weight, None, self.eps, out, None, branch=branch, rms=True)
             elif scaled is not None:
