@@ -151,14 +151,19 @@ def split_parts(K: int, splits: int) -> int:
 
 def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
     """(bn, splits, stages) of a product of 8-bit integers.  Few tokens: 128 weight rows x bn tokens per block, K split over a cluster of up to 8
-    blocks until about two blocks per SM stream weights; many tokens: 256 x 256 tiles on pairs of SMs (bn 256).  Between 129 and 512 tokens the
-    first form, with several tiles of 128 tokens, while the second would leave most pairs without a tile; and for matrices of fewer than 256 rows."""
+    blocks; many tokens: 256 x 256 tiles on pairs of SMs (bn 256).  Between 129 and 512 tokens the
+    first form, with several tiles of 128 tokens, while the second would leave most pairs without a tile; and for matrices of fewer than 256 rows.
+
+    Two blocks share an SM, but clusters of them do not fill the chip: from 7/4 blocks per SM on some start when others have ended, and a product of
+    one wave takes two (norm and product of one token, us on a B200, parts of K: 6,144 x 4,096 in 5 8.0, in 6 13.9; 5,120 x 5,120 in 6 8.2, in 7
+    14.8).  So as many parts as stay below that, none shorter than 4 stages of 128 numbers (2 for up to 16 tokens, whose sums are joined
+    faster: 2,048 x 2,048 in 4 6.1, in 8 5.6; with 64 tokens 7.4 and over 7.6)."""
     tiles = -(-M // 256) * -(-N // 256)
     if M > 128 and N >= 256 and (M > 512 or mode == "swiglu" or tiles >= sm_count // 2):
         return 256, 1, 6
     bn = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
     blocks = -(-N // 128) * -(-M // bn)
-    splits = max(1, min(8, -(-K // 128) // 4, 2 * sm_count // max(1, blocks)))
+    splits = max(1, min(8, -(-K // 128) // (2 if M <= 16 else 4), 7 * sm_count // (4 * max(1, blocks))))
     return bn, splits, max(2, min(8, 102400 // (16384 + bn * 128)))
 
 
