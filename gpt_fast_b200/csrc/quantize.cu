@@ -190,117 +190,108 @@ rope_append_int8_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const flo
     }
 }
 
-// The same for heads of 64 and 128, aligned: one block per token, its place found once, one warp per head at a time, a lane D / 32 neighbouring numbers (D / 64 of
-// either half where pairs are halves) in one load; the loads of up to HEADS_AT_ONCE heads are in flight together.
-constexpr int APPEND_WARPS = 8, HEADS_AT_ONCE = 3;
+// The same for heads of 64 and 128, aligned: a block of four warps per token.  A lane has sixteen numbers of a head, whose pairs it turns by itself: two runs of
+// eight, side by side or at the same place of either half; D / 16 lanes make a head.  A token's row is read at once, ahead of the chain of small loads
+// that finds its place (up to HEADS_AT_ONCE heads per group of lanes), which is what memory needs to keep busy.
+constexpr int APPEND_WARPS = 4, HEADS_AT_ONCE = 3;
 
-template <typename T, int N> struct alignas(N * sizeof(T)) Few { T v[N]; };
-
-// a lane's numbers to their places: side by side, or half of them here and half HALF further
-template <typename T, int N>
-__device__ __forceinline__ void put(T* dst, const Few<T, N>& o, int half, int pairing) {
-    if (pairing != 1) { *reinterpret_cast<Few<T, N>*>(dst) = o; return; }
-    Few<T, N / 2> a, b;
-#pragma unroll
-    for (int i = 0; i < N / 2; i++) { a.v[i] = o.v[i]; b.v[i] = o.v[i + N / 2]; }
-    *reinterpret_cast<Few<T, N / 2>*>(dst) = a;
-    *reinterpret_cast<Few<T, N / 2>*>(dst + half) = b;
-}
+template <typename T, int N> struct alignas((N * sizeof(T) < 16 ? N * sizeof(T) : 16)) Few { T v[N]; };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * APPEND_WARPS)
 rope_append_int8_vec_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const float* table, int table_len, int H, int G, int pairing, int append, int* status) {
-    constexpr int E = D / 32, HALF = D / 2;                              // numbers per lane
+    constexpr int LANES = D / 16, HEADS = 32 / LANES, HALF = D / 2;      // lanes of a head, heads of a warp
     gfb_pdl_launch();
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % LANES;
     const int s = b.tok_seq[t], slot = b.slots[s], q_off = t - b.cu_seqlens[s];
-    gfb_pdl_wait();
-    const int pos = b.lengths[slot] + q_off;
-    bool ok = pos >= 0 && pos < table_len;
-    long long row = 0;
-    if (ok && append) {
-        row = cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, pos);
-        ok = row >= 0;
-    }
-    if (!ok && threadIdx.x == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, pos);
-    // where this lane's numbers are: E neighbours, or E / 2 neighbours of either half; pair i of them is (x[i0], x[i1])
-    const int at = pairing == 1 ? lane * (E / 2) : lane * E;
-    float cs[E / 2][2];
-#pragma unroll
-    for (int i = 0; i < E / 2; i++) {
-        const float2 c = ok ? *reinterpret_cast<const float2*>(table + ((size_t)pos * HALF + lane * (E / 2) + i) * 2) : make_float2(0.f, 0.f);
-        cs[i][0] = c.x;
-        cs[i][1] = c.y;
-    }
+    // pair i of this lane, of the head's pair 8 li + i, is (x[i], x[i + 8]) with pairs of halves and (x[2i], x[2i + 1]) with neighbours
+    const int at0 = pairing == 1 ? 8 * li : 16 * li, at1 = pairing == 1 ? HALF + 8 * li : 16 * li + 8;
     const int heads = H + (append ? 2 * G : 0);
     const T* src = qkv + (size_t)t * (H + 2 * G) * D;
-    for (int h0 = warp; h0 < heads; h0 += APPEND_WARPS * HEADS_AT_ONCE) {
-        Few<T, E / 2> raw[HEADS_AT_ONCE][2];
+    gfb_pdl_wait();
+    bool ok = false;
+    long long row = 0;
+    float cs[8][2];
+#pragma unroll 1
+    for (int h0 = warp * HEADS; h0 < heads; h0 += APPEND_WARPS * HEADS * HEADS_AT_ONCE) {
+        Few<T, 8> raw[HEADS_AT_ONCE][2];
 #pragma unroll
         for (int u = 0; u < HEADS_AT_ONCE; u++) {
-            const int head = h0 + u * APPEND_WARPS;
+            const int head = h0 + u * APPEND_WARPS * HEADS + lane / LANES;
             if (head >= heads) continue;
             const T* p = src + (size_t)head * D;
-            if (pairing == 1) {                                          // values come the same way, as pairs (i, i + HALF) that are not rotated
-                raw[u][0] = *reinterpret_cast<const Few<T, E / 2>*>(p + at);
-                raw[u][1] = *reinterpret_cast<const Few<T, E / 2>*>(p + HALF + at);
-            } else {
-                const Few<T, E> both = *reinterpret_cast<const Few<T, E>*>(p + at);
+            raw[u][0] = *reinterpret_cast<const Few<T, 8>*>(p + at0);
+            raw[u][1] = *reinterpret_cast<const Few<T, 8>*>(p + at1);
+        }
+        if (h0 == warp * HEADS) {
+            const int pos = b.lengths[slot] + q_off;
+            ok = pos >= 0 && pos < table_len;
+            if (ok) {
+                const float4* c = reinterpret_cast<const float4*>(table + ((size_t)pos * HALF + 8 * li) * 2);
 #pragma unroll
-                for (int i = 0; i < E; i++) raw[u][i / (E / 2)].v[i % (E / 2)] = both.v[i];
+                for (int i = 0; i < 4; i++) {
+                    const float4 v = c[i];
+                    cs[2 * i][0] = v.x; cs[2 * i][1] = v.y; cs[2 * i + 1][0] = v.z; cs[2 * i + 1][1] = v.w;
+                }
+                if (append) {
+                    row = cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, pos);
+                    ok = row >= 0;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) cs[i][0] = cs[i][1] = 0.f;
             }
+            if (!ok && threadIdx.x == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, pos);
         }
 #pragma unroll
         for (int u = 0; u < HEADS_AT_ONCE; u++) {
-            const int head = h0 + u * APPEND_WARPS;
-            if (head >= heads) continue;
-            float x[E];
+            const int first = h0 + u * APPEND_WARPS * HEADS, head = first + lane / LANES;
+            if (first >= heads) break;                                   // (the warp's)
+            float x[16];
+            uint32_t m = 0;
+            if (head < heads) {
 #pragma unroll
-            for (int i = 0; i < E; i++) x[i] = gfb_to_f32(raw[u][i / (E / 2)].v[i % (E / 2)]);
-            if (head < H + G) {
-                if (pairing == 1) {
+                for (int i = 0; i < 16; i++) x[i] = gfb_to_f32(raw[u][i >> 3].v[i & 7]);
+                if (head < H + G) {
+                    if (pairing == 1) {
 #pragma unroll
-                    for (int i = 0; i < E / 2; i++) turn(x[i], x[i + E / 2], cs[i][0], cs[i][1]);
+                        for (int i = 0; i < 8; i++) turn(x[i], x[i + 8], cs[i][0], cs[i][1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) turn(x[2 * i], x[2 * i + 1], cs[i][0], cs[i][1]);
+                    }
+                }
+                if (head < H) {
+                    T* dst = q_out + ((size_t)t * H + head) * D;
+                    Few<T, 8> o[2];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i >> 3].v[i & 7] = gfb_from_f32<T>(ok ? x[i] : 0.f);      // q stays defined so that later kernels read no garbage
+                    *reinterpret_cast<Few<T, 8>*>(dst + at0) = o[0];
+                    *reinterpret_cast<Few<T, 8>*>(dst + at1) = o[1];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < E / 2; i++) turn(x[2 * i], x[2 * i + 1], cs[i][0], cs[i][1]);
+                    for (int i = 0; i < 16; i++) m = max(m, abs_bits(x[i]));
                 }
             }
-            if (head < H) {
-                Few<T, E> o;
+            if (first + HEADS <= H) continue;                            // queries only
 #pragma unroll
-                for (int i = 0; i < E; i++) o.v[i] = gfb_from_f32<T>(ok ? x[i] : 0.f);      // q stays defined so that later kernels read no garbage
-                put(q_out + ((size_t)t * H + head) * D + at, o, HALF, pairing);
-                continue;
-            }
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < E; i++) m = max(m, abs_bits(x[i]));
-            const RowScale rs(warp_max_bits(m));
-            if (!ok) continue;
+            for (int o = LANES / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (head < H || head >= heads || !ok) continue;
+            const RowScale rs(m);
             const bool key = head < H + G;
             const size_t place = (size_t)row + (size_t)(head - (key ? H : H + G)) * kv.page_size;
-            if (lane == 0) (key ? kv.k_scale : kv.v_scale)[place] = rs.scale;
-            Few<int8_t, E> o;
-#pragma unroll
-            for (int i = 0; i < E; i++) o.v[i] = (int8_t)rs.of(x[i]);
-            put((key ? kv.k_pool : kv.v_pool) + place * D + at, o, HALF, pairing);
+            if (li == 0) (key ? kv.k_scale : kv.v_scale)[place] = rs.scale;
+            int8_t* dst = (key ? kv.k_pool : kv.v_pool) + place * D;
+            *reinterpret_cast<uint2*>(dst + at0) = make_uint2(rs.of4(x[0], x[1], x[2], x[3]), rs.of4(x[4], x[5], x[6], x[7]));
+            *reinterpret_cast<uint2*>(dst + at1) = make_uint2(rs.of4(x[8], x[9], x[10], x[11]), rs.of4(x[12], x[13], x[14], x[15]));
         }
     }
 }
 
-// What the cache holds at the places of the step's tokens: k_out, v_out [T, G, d].  Eight numbers per thread where d allows it (wide), else one.
-template <typename TO>
-__device__ __forceinline__ void put8(TO* dst, uint2 q, float s) {
-    Few<TO, 8> o;
-#pragma unroll
-    for (int i = 0; i < 8; i++) o.v[i] = gfb_from_f32<TO>(__fmul_rn((float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))), s));
-    *reinterpret_cast<Few<TO, 8>*>(dst) = o;
-}
-
-template <typename TO>
-__global__ void __launch_bounds__(256)
-read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d, int wide, int* status) {
+// What the cache holds at the places of the step's tokens: k_out, v_out [T, G, d].  A block per token; VEC (sixteen, eight or one) numbers per thread at a time.
+template <typename TO, int VEC>
+__global__ void __launch_bounds__(128)
+read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d, int* status) {
     gfb_pdl_launch();
     const int t = blockIdx.x;
     const int s = b.tok_seq[t], slot = b.slots[s], q_off = t - b.cu_seqlens[s];
@@ -308,16 +299,17 @@ read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d
     const int pos = b.lengths[slot] + q_off;
     const long long row = cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, pos);
     if (row < 0 && threadIdx.x == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, pos);
-    const int step = wide ? 8 : 1, n = G * d / step;
+    const int n = G * d / VEC;
     for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
         const bool key = i < n;
-        const int j = (key ? i : i - n) * step, g = j / d;
-        const size_t at = (size_t)(row < 0 ? 0 : row) + (size_t)g * kv.page_size, e = at * d + (j - g * d);
-        TO* dst = (key ? k_out : v_out) + (size_t)t * G * d + j;
-        const int8_t* pool = key ? kv.k_pool : kv.v_pool;
-        const float sc = row < 0 ? 0.f : (key ? kv.k_scale : kv.v_scale)[at];
-        if (wide) put8(dst, row < 0 ? make_uint2(0u, 0u) : *reinterpret_cast<const uint2*>(pool + e), sc);
-        else *dst = gfb_from_f32<TO>(row < 0 ? 0.f : __fmul_rn((float)pool[e], sc));
+        const int j = (key ? i : i - n) * VEC, g = j / d;
+        const size_t at = (size_t)(row < 0 ? 0 : row) + (size_t)g * kv.page_size;
+        const Few<int8_t, VEC> q = *reinterpret_cast<const Few<int8_t, VEC>*>((key ? kv.k_pool : kv.v_pool) + at * d + (j - g * d));
+        const float sc = (key ? kv.k_scale : kv.v_scale)[at];
+        Few<TO, VEC> o;
+#pragma unroll
+        for (int u = 0; u < VEC; u++) o.v[u] = gfb_from_f32<TO>(row < 0 ? 0.f : __fmul_rn((float)q.v[u], sc));
+        *reinterpret_cast<Few<TO, VEC>*>((key ? k_out : v_out) + (size_t)t * G * d + j) = o;
     }
 }
 
@@ -386,10 +378,14 @@ GFB_API int gfb_read_cache_int8(void* k_pool, void* v_pool, float* k_scale, floa
     if (n_tokens <= 0) return 0;
     Int8KV kv{(int8_t*)k_pool, (int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages};
     GfbBatch b{cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens};
-    const int wide = d % 8 == 0 && (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 31) == 0;
+    const int vec = (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 15) != 0 ? 1 : d % 16 == 0 ? 16 : d % 8 == 0 ? 8 : 1;
     cudaError_t e;
-    if (dt == GFB_BF16) e = gfb_launch(read_cache_int8_kernel<__nv_bfloat16>, dim3(n_tokens), dim3(256), 0, stream, kv, b, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, G, d, wide, status);
-    else if (dt == GFB_F32) e = gfb_launch(read_cache_int8_kernel<float>, dim3(n_tokens), dim3(256), 0, stream, kv, b, (float*)k_out, (float*)v_out, G, d, wide, status);
+#define GO(TO, V) e = gfb_launch(read_cache_int8_kernel<TO, V>, dim3(n_tokens), dim3(128), 0, stream, kv, b, (TO*)k_out, (TO*)v_out, G, d, status)
+#define GO3(TO) do { if (vec == 16) GO(TO, 16); else if (vec == 8) GO(TO, 8); else GO(TO, 1); } while (0)
+    if (dt == GFB_BF16) GO3(__nv_bfloat16);
+    else if (dt == GFB_F32) GO3(float);
     else return gfb_fail("gfb_read_cache_int8: unknown type %d", dt);
+#undef GO3
+#undef GO
     return gfb_check(e, "gfb_read_cache_int8");
 }
