@@ -1,8 +1,10 @@
 // Rows of 8-bit integers with one scale each: what the 8-bit products multiply and the 8-bit cache holds.
 //
 // A row x becomes scale = m / 127, m = max |x_i|, and the integers q_i nearest to 127 x_i / m (ties to even), so that q_i scale is within
-// scale / 2 of x_i and |q_i| <= 127.  The integer is the one exact arithmetic gives for the 32-bit numbers x_i: a first 32-bit quotient is right unless it
-// lies within 1e-4 of a tie, and those few are decided by comparing 254 |x_i| with an odd multiple of m in 64 bits, where both are exact.
+// scale / 2 of x_i and |q_i| <= 127.  The integer is the one exact arithmetic gives for the 32-bit numbers x_i: a 32-bit quotient is off by two roundings,
+// at most 127 x 2^-23 < 2e-5, so it is right unless it lies that near to a tie; then 254 |x_i| is compared with the odd multiple of m, each product as a 32-bit
+// number and its rest.  The two rounded products are next to each other, so that their difference is exact, and the rests are multiples of a 256th of their
+// last place, so theirs is too.
 // So the same numbers give the same integers in every kernel here, whatever order its code computes in.
 // A row of zeros has scale 0.  A row that holds a NaN or an infinity has scale NaN (and integers 0): it stands for NaN as a whole.
 #pragma once
@@ -12,31 +14,47 @@ namespace {
 
 // How a row's numbers become integers; `bits`: the largest |x_i| as its 32-bit pattern, which orders like the number and puts infinity and NaN on top.
 struct RowScale {
-    float most, lift, inv, scale;
+    float most, lift, inv, scale;                       // most, inv: of the row times lift
     bool live;                                          // finite and not all zeros
     __device__ __forceinline__ explicit RowScale(uint32_t bits) {
-        most = __uint_as_float(bits);
+        const float m = __uint_as_float(bits);
         live = bits != 0u && bits < 0x7f800000u;
-        lift = most < 0x1p-60f ? 0x1p64f : 1.f;         // keeps the reciprocal of a tiny maximum finite
-        inv = live ? __fdiv_rn(127.f, most * lift) : 0.f;
-        scale = bits < 0x7f800000u ? __fdiv_rn(most, 127.f) : __uint_as_float(0x7fc00000u);
+        lift = m < 0x1p-60f ? 0x1p64f : m > 0x1p100f ? 0x1p-30f : 1.f;      // keeps 127 / m and 254 m finite and their parts exact
+        most = __fmul_rn(m, lift);
+        inv = live ? __fdiv_rn(127.f, most) : 0.f;
+        scale = bits < 0x7f800000u ? __fdiv_rn(m, 127.f) : __uint_as_float(0x7fc00000u);
     }
-    __device__ __forceinline__ int of(float x) const {
-        if (!live) return 0;
-        const float r = __fmul_rn(__fmul_rn(x, lift), inv);
+    // x: times lift
+    __device__ __forceinline__ float nearest(float x) const {
+        const float r = __fmul_rn(x, inv);
         float k = rintf(r);
-        if (fabsf(r - k) > 0.4999f) {                   // next to a tie, about one number in 5,000
-            const float a = fabsf(r), f = floorf(a);
-            const double twice = 254.0 * (double)fabsf(x), tie = (2.0 * (double)f + 1.0) * (double)most;
-            k = (twice > tie || (twice == tie && ((int)f & 1))) ? f + 1.f : f;
-            k = copysignf(k, x);
+        if (fabsf(r - k) > 0.49998f) {
+            // 254 |x| against (2 f + 1) most: both products as a rounded one and its rest, which has few bits
+            const float f = floorf(fabsf(r)), odd = 2.f * f + 1.f;
+            const float p = __fmul_rn(254.f, fabsf(x)), t = __fmul_rn(odd, most);
+            const float over = (p - t) + (__fmaf_rn(254.f, fabsf(x), -p) - __fmaf_rn(odd, most, -t));
+            k = copysignf(over > 0.f || (over == 0.f && ((int)f & 1)) ? f + 1.f : f, x);
         }
-        return (int)k;
+        return k;
     }
-    // four of them in the bytes of a word
-    __device__ __forceinline__ uint32_t of4(float a, float b, float c, float d) const {
-        const uint32_t ab = __byte_perm((uint32_t)of(a), (uint32_t)of(b), 0x0040), cd = __byte_perm((uint32_t)of(c), (uint32_t)of(d), 0x0040);
-        return __byte_perm(ab, cd, 0x5410);
+    __device__ __forceinline__ int of(float x) const { return live ? (int)nearest(__fmul_rn(x, lift)) : 0; }
+    // Eight numbers of the row in the bytes of two words.  Adding 1.5 x 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
+    __device__ __forceinline__ uint2 of8(const float* x) const {
+        uint32_t w[8];
+        float far = lift != 1.f ? 1.f : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float r = __fmul_rn(x[i], inv), t = __fadd_rn(r, 12582912.f);
+            w[i] = __float_as_uint(t);
+            far = fmaxf(far, fabsf(__fsub_rn(r, __fsub_rn(t, 12582912.f))));
+        }
+        if (far > 0.49998f) {                           // one of them next to a tie, or a row out of the ordinary
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = (uint32_t)(int)nearest(__fmul_rn(x[i], lift));
+        }
+        const uint32_t lo = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+        const uint32_t hi = __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410);
+        return live ? make_uint2(lo, hi) : make_uint2(0u, 0u);
     }
 };
 
@@ -94,7 +112,7 @@ quantize_rows_vec_kernel(const T* x, int8_t* q, float* scale, int K, int pitch, 
 #pragma unroll
     for (int k = 0; k < ROW_VECTORS; k++) {
         const int i = threadIdx.x + k * blockDim.x;
-        if (i < n) *reinterpret_cast<uint2*>(out + 8 * i) = make_uint2(rs.of4(v[k][0], v[k][1], v[k][2], v[k][3]), rs.of4(v[k][4], v[k][5], v[k][6], v[k][7]));
+        if (i < n) *reinterpret_cast<uint2*>(out + 8 * i) = rs.of8(v[k]);
     }
     if (threadIdx.x == 0) {
         scale[blockIdx.x] = rs.scale;

@@ -79,7 +79,7 @@ rmsnorm_quantize_vec_kernel(float* x, const float* pending, int S, size_t slice,
 #pragma unroll
     for (int k = 0; k < ROW_VECTORS; k++) {
         const int i = threadIdx.x + k * blockDim.x;
-        if (i < n) *reinterpret_cast<uint2*>(out + 8 * i) = make_uint2(rs.of4(v[k][0], v[k][1], v[k][2], v[k][3]), rs.of4(v[k][4], v[k][5], v[k][6], v[k][7]));
+        if (i < n) *reinterpret_cast<uint2*>(out + 8 * i) = rs.of8(v[k]);
     }
     if (threadIdx.x == 0) {
         scale[r] = rs.scale;
@@ -190,102 +190,124 @@ rope_append_int8_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const flo
     }
 }
 
-// The same for heads of 64 and 128, aligned: a block of four warps per token.  A lane has sixteen numbers of a head, whose pairs it turns by itself: two runs of
-// eight, side by side or at the same place of either half; D / 16 lanes make a head.  A token's row is read at once, ahead of the chain of small loads
-// that finds its place (up to HEADS_AT_ONCE heads per group of lanes), which is what memory needs to keep busy.
+// The same for heads of 64 and 128, aligned.  A lane has sixteen numbers of a head, whose pairs it turns by itself: two runs of eight at the same place of either half;
+// D / 16 lanes make a head.  What bounds it is memory, and what stood in its way was latency: a row's place in the cache is found
+// by four loads that wait for one another, and a block per token had little else to do meanwhile (packed prompts of 8,441 tokens, 32 query and 8 key heads of 128,
+// 192 MB: 54.5 us).  So four blocks per SM go through units of a token's heads, with the rows of the next units on their way to shared
+// memory (every thread fetches what it works on itself, so nothing waits for a block), and each lane of a warp finds the place of another of the
+// next 32 units: 39.7 us, 4.9 TB/s.
 constexpr int APPEND_WARPS = 4, HEADS_AT_ONCE = 3;
 
 template <typename T, int N> struct alignas((N * sizeof(T) < 16 ? N * sizeof(T) : 16)) Few { T v[N]; };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * APPEND_WARPS)
-rope_append_int8_vec_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const float* table, int table_len, int H, int G, int pairing, int append, int* status) {
+__device__ __forceinline__ void copy16(uint4* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+template <typename T, int D, bool HALVES>
+__global__ void __launch_bounds__(32 * APPEND_WARPS, 4)
+rope_append_int8_vec_kernel(const T* qkv, T* q_out, Int8KV kv, GfbBatch b, const float* table, int table_len, int H, int G, int append, int* status) {
     constexpr int LANES = D / 16, HEADS = 32 / LANES, HALF = D / 2;      // lanes of a head, heads of a warp
+    constexpr int UNIT = APPEND_WARPS * HEADS * HEADS_AT_ONCE;           // heads of a unit
+    constexpr int PIECES = sizeof(T), STAGES = sizeof(T) == 2 ? 3 : 2;   // sixteen numbers are this many pieces of 16 bytes
+    __shared__ uint4 ring[STAGES][HEADS_AT_ONCE][PIECES][32 * APPEND_WARPS];
     gfb_pdl_launch();
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % LANES;
-    const int s = b.tok_seq[t], slot = b.slots[s], q_off = t - b.cu_seqlens[s];
-    // pair i of this lane, of the head's pair 8 li + i, is (x[i], x[i + 8]) with pairs of halves and (x[2i], x[2i + 1]) with neighbours
-    const int at0 = pairing == 1 ? 8 * li : 16 * li, at1 = pairing == 1 ? HALF + 8 * li : 16 * li + 8;
-    const int heads = H + (append ? 2 * G : 0);
-    const T* src = qkv + (size_t)t * (H + 2 * G) * D;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % LANES, mine = warp * HEADS + lane / LANES;
+    // pair i of this lane is (x[i], x[i + 8]) with pairs of halves, the head's pair 8 li + i; with neighbours it is (x[2i], x[2i + 1]), the head's pair 4 li + i
+    // for the first four and D / 4 + 4 li + i - 4 for the rest
+    const int at0 = 8 * li, at1 = HALF + 8 * li;
+    const int heads = H + (append ? 2 * G : 0), per = (heads + UNIT - 1) / UNIT;         // per: units of a token
+    const int units = b.n_tokens * per, step = gridDim.x;
+    auto fetch = [&](int unit, int st) {
+        if (unit < units) {
+            const int t = unit / per, h0 = (unit - t * per) * UNIT + mine;
+#pragma unroll
+            for (int u = 0; u < HEADS_AT_ONCE; u++) {
+                const int head = h0 + u * APPEND_WARPS * HEADS;
+                if (head >= heads) break;
+                const T* p = qkv + ((size_t)t * (H + 2 * G) + head) * D;
+#pragma unroll
+                for (int k = 0; k < PIECES; k++)
+                    copy16(&ring[st][u][k][threadIdx.x], p + (k < PIECES / 2 ? at0 + k * (16 / PIECES) : at1 + (k - PIECES / 2) * (16 / PIECES)));
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     gfb_pdl_wait();
-    bool ok = false;
-    long long row = 0;
-    float cs[8][2];
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) fetch(blockIdx.x + i * step, i);
+    int places = -1;                                                     // of unit blockIdx.x + (i / 32 * 32 + lane) step: its position; -1: none
+    long long rows = -1;                                                 // and its row in the cache
+    int st = 0;
 #pragma unroll 1
-    for (int h0 = warp * HEADS; h0 < heads; h0 += APPEND_WARPS * HEADS * HEADS_AT_ONCE) {
-        Few<T, 8> raw[HEADS_AT_ONCE][2];
-#pragma unroll
-        for (int u = 0; u < HEADS_AT_ONCE; u++) {
-            const int head = h0 + u * APPEND_WARPS * HEADS + lane / LANES;
-            if (head >= heads) continue;
-            const T* p = src + (size_t)head * D;
-            raw[u][0] = *reinterpret_cast<const Few<T, 8>*>(p + at0);
-            raw[u][1] = *reinterpret_cast<const Few<T, 8>*>(p + at1);
-        }
-        if (h0 == warp * HEADS) {
-            const int pos = b.lengths[slot] + q_off;
-            ok = pos >= 0 && pos < table_len;
-            if (ok) {
-                const float4* c = reinterpret_cast<const float4*>(table + ((size_t)pos * HALF + 8 * li) * 2);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 v = c[i];
-                    cs[2 * i][0] = v.x; cs[2 * i][1] = v.y; cs[2 * i + 1][0] = v.z; cs[2 * i + 1][1] = v.w;
-                }
-                if (append) {
-                    row = cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, pos);
-                    ok = row >= 0;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) cs[i][0] = cs[i][1] = 0.f;
+    for (int i = 0, unit = blockIdx.x; unit < units; i++, unit += step) {
+        if ((i & 31) == 0) {
+            const long long other = unit + (long long)lane * step;
+            if (other < units) {
+                const int t = (int)other / per, s = b.tok_seq[t], slot = b.slots[s];
+                places = b.lengths[slot] + (t - b.cu_seqlens[s]);
+                if (places >= table_len) places = -1;
+                rows = append ? cache_row(kv.page_table, kv.max_pages, kv.page_size, kv.n_pages, G, slot, places) : 0;
             }
-            if (!ok && threadIdx.x == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, pos);
+            __syncwarp();
         }
+        const int pos = __shfl_sync(0xffffffffu, places, i & 31), t = unit / per, h0 = (unit - t * per) * UNIT;
+        float4 cs[4];                                                    // (cos, sin) of two pairs each
+        const float4* angles = reinterpret_cast<const float4*>(table + (size_t)max(pos, 0) * D) + (HALVES ? 4 * li : 2 * li);
+#pragma unroll
+        for (int k = 0; k < 4; k++) cs[k] = angles[k + (!HALVES && k >= 2 ? D / 8 - 2 : 0)];
+        const long long row = __shfl_sync(0xffffffffu, rows, i & 31);
+        const bool ok = pos >= 0 && row >= 0;
+        if (!ok && threadIdx.x == 0 && h0 == 0) gfb_report(status, GFB_ERR_CACHE_RANGE, t, b.lengths[b.slots[b.tok_seq[t]]] + (t - b.cu_seqlens[b.tok_seq[t]]));
+        fetch(unit + (STAGES - 1) * step, st == 0 ? STAGES - 1 : st - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
 #pragma unroll
         for (int u = 0; u < HEADS_AT_ONCE; u++) {
-            const int first = h0 + u * APPEND_WARPS * HEADS, head = first + lane / LANES;
+            const int first = h0 + u * APPEND_WARPS * HEADS + warp * HEADS, head = first + lane / LANES;
             if (first >= heads) break;                                   // (the warp's)
+            Few<T, 16> raw;
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) reinterpret_cast<uint4*>(&raw)[k] = ring[st][u][k][threadIdx.x];
             float x[16];
-            uint32_t m = 0;
-            if (head < heads) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = gfb_to_f32(raw[u][i >> 3].v[i & 7]);
-                if (head < H + G) {
-                    if (pairing == 1) {
+            for (int k = 0; k < 16; k++) x[k] = gfb_to_f32(raw.v[k]);
+            if (head < H + G) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) turn(x[i], x[i + 8], cs[i][0], cs[i][1]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) turn(x[2 * i], x[2 * i + 1], cs[i][0], cs[i][1]);
-                    }
-                }
-                if (head < H) {
-                    T* dst = q_out + ((size_t)t * H + head) * D;
-                    Few<T, 8> o[2];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[i >> 3].v[i & 7] = gfb_from_f32<T>(ok ? x[i] : 0.f);      // q stays defined so that later kernels read no garbage
-                    *reinterpret_cast<Few<T, 8>*>(dst + at0) = o[0];
-                    *reinterpret_cast<Few<T, 8>*>(dst + at1) = o[1];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) m = max(m, abs_bits(x[i]));
+                for (int k = 0; k < 8; k++) {
+                    const float c = k & 1 ? cs[k >> 1].z : cs[k >> 1].x, sn = k & 1 ? cs[k >> 1].w : cs[k >> 1].y;
+                    if (HALVES) turn(x[k], x[k + 8], c, sn);
+                    else turn(x[2 * k], x[2 * k + 1], c, sn);
                 }
             }
-            if (first + HEADS <= H) continue;                            // queries only
+            if (head < H) {
+                T* dst = q_out + ((size_t)t * H + head) * D;
+                Few<T, 8> o[2];
+#pragma unroll
+                for (int k = 0; k < 16; k++) o[k >> 3].v[k & 7] = gfb_from_f32<T>(x[k]);
+                if (!ok) o[0] = o[1] = Few<T, 8>{};                      // q stays defined so that later kernels read no garbage
+                *reinterpret_cast<Few<T, 8>*>(dst + at0) = o[0];
+                *reinterpret_cast<Few<T, 8>*>(dst + at1) = o[1];
+            }
+            if (first + HEADS <= H) continue;                            // the warp's are all queries
+            uint32_t m = 0;
+#pragma unroll
+            for (int k = 0; k < 16; k++) m = max(m, abs_bits(x[k]));
 #pragma unroll
             for (int o = LANES / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (head < H || head >= heads || !ok) continue;
-            const RowScale rs(m);
-            const bool key = head < H + G;
-            const size_t place = (size_t)row + (size_t)(head - (key ? H : H + G)) * kv.page_size;
-            if (li == 0) (key ? kv.k_scale : kv.v_scale)[place] = rs.scale;
-            int8_t* dst = (key ? kv.k_pool : kv.v_pool) + place * D;
-            *reinterpret_cast<uint2*>(dst + at0) = make_uint2(rs.of4(x[0], x[1], x[2], x[3]), rs.of4(x[4], x[5], x[6], x[7]));
-            *reinterpret_cast<uint2*>(dst + at1) = make_uint2(rs.of4(x[8], x[9], x[10], x[11]), rs.of4(x[12], x[13], x[14], x[15]));
+            if (head >= H && head < heads && ok) {
+                const RowScale rs(m);
+                const bool key = head < H + G;
+                const size_t place = (size_t)row + (size_t)(head - (key ? H : H + G)) * kv.page_size;
+                if (li == 0) (key ? kv.k_scale : kv.v_scale)[place] = rs.scale;
+                int8_t* dst = (key ? kv.k_pool : kv.v_pool) + place * D;
+                *reinterpret_cast<uint2*>(dst + at0) = rs.of8(x);
+                *reinterpret_cast<uint2*>(dst + at1) = rs.of8(x + 8);
+            }
+            __syncwarp();
         }
+        st = st + 1 == STAGES ? 0 : st + 1;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // What the cache holds at the places of the step's tokens: k_out, v_out [T, G, d].  A block per token; VEC (sixteen, eight or one) numbers per thread at a time.
@@ -349,17 +371,25 @@ GFB_API int gfb_rope_append_int8(const void* qkv, void* q_out, int dt, void* k_p
                                  const float* table, int table_len, int H, int G, int d, int pairing, int append, int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     if (d % 2) return gfb_fail("gfb_rope_append_int8: head_dim %d is odd", d);
+    if (table_len < 1) return gfb_fail("gfb_rope_append_int8: an empty rotary table");
     Int8KV kv{(int8_t*)k_pool, (int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages};
     GfbBatch b{cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens};
     if ((d == 64 || d == 128) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)table) & 15) == 0) {
         cudaError_t ve;
-#define GO(T, D) ve = gfb_launch(rope_append_int8_vec_kernel<T, D>, dim3(n_tokens), dim3(32 * APPEND_WARPS), 0, stream, (const T*)qkv, (T*)q_out, kv, b, table, table_len, H, G, pairing, append, status)
+        const int units = n_tokens * ((H + (append ? 2 * G : 0) + APPEND_WARPS * HEADS_AT_ONCE * 512 / d - 1) / (APPEND_WARPS * HEADS_AT_ONCE * 512 / d));
+        int dev = 0, sms = 148;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        const int grid = min(units, 4 * sms);
+#define GO2(T, D, HALVES) gfb_launch(rope_append_int8_vec_kernel<T, D, HALVES>, dim3(grid), dim3(32 * APPEND_WARPS), 0, stream, (const T*)qkv, (T*)q_out, kv, b, table, table_len, H, G, append, status)
+#define GO(T, D) ve = pairing == 1 ? GO2(T, D, true) : GO2(T, D, false)
         if (dt == GFB_BF16 && d == 128) GO(__nv_bfloat16, 128);
         else if (dt == GFB_BF16) GO(__nv_bfloat16, 64);
         else if (dt == GFB_F32 && d == 128) GO(float, 128);
         else if (dt == GFB_F32) GO(float, 64);
         else return gfb_fail("gfb_rope_append_int8: unknown type %d", dt);
 #undef GO
+#undef GO2
         return gfb_check(ve, "gfb_rope_append_int8");
     }
     dim3 grid(n_tokens, (H + (append ? 2 * G : 0) + 3) / 4);

@@ -136,6 +136,14 @@ def test_append_without_storing():
     assert torch.equal(q, turned(qkv.float().view(6, 8, 64)[:, :4], table, places(batch)[1], "interleaved").to(BF16))
 
 
+def test_an_empty_rotary_table_is_refused():
+    batch = make_batch([0], [2])
+    kv = make_cache(batch, [0], [2], 2, 64)
+    qkv, q = torch.zeros(2, 8 * 64, device="cuda"), torch.empty(2, 4, 64, device="cuda")
+    with pytest.raises(ops.KernelError, match="empty rotary table"):
+        ops.rope_append(qkv, q, kv, batch, rope(4, 64)[:0], 4, 2, 64)
+
+
 def test_missing_pages_are_reported():
     batch = make_batch([60, 0], [10, 3])
     kv = make_cache(batch, [60, 0], [10, 3], 2, 64)
