@@ -798,6 +798,7 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
+constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
 constexpr int SOFT_WARPS = 16, CONV_WARPS = 7, CONV_UNITS = 8, MMA_WARP = SOFT_WARPS + CONV_WARPS, PROMPT_THREADS = 32 * (MMA_WARP + 1);     // six warps per quarter of an SM: 80 registers each
 constexpr int LEAST_EXPONENT = 37, MOST_EXPONENT = 217;      // of k_ref and v_ref, in a float's bits: 2^-90 to 2^90, so that weights over v_ref stay finite
@@ -808,7 +809,7 @@ struct PromptBars {
     unsigned long long sc_full[SC_STAGES];
     unsigned long long s_full[2], p_ready[2], pv_done[2];
     uint32_t tmem_base;
-    int gave_up;
+    int gave_up, n_listed;
 };
 __device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 // two float16 numbers x times the number hi + lo
@@ -826,7 +827,7 @@ template <int D>
 struct PromptSmem {
     static constexpr int TILE = (D / 64) * HALF_BYTES;
     static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, ROWS_AT = SC + SC_STAGES * (int)sizeof(Refs);
-    static constexpr int BARS = ROWS_AT + 2 * 2 * ROWS * 4;
+    static constexpr int LIST = ROWS_AT + 2 * 2 * ROWS * 4, BARS = LIST + LISTED * 16;
     static constexpr int BYTES = 1024 + BARS + (int)sizeof(PromptBars);
 };
 
@@ -939,38 +940,53 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// A pair of tiles: its sequence, its first token and that one's position, the tokens from it to the sequence's end.
+struct alignas(16) TilePair { int seq, t0, pos, left; };
+__device__ __forceinline__ int pairs_of(int tokens, int TQ) { return (tokens + 2 * TQ - 1) / (2 * TQ); }
+
 // One work item; the same for every warp of a block.
 struct PromptItem {
-    int g, z, seq, slot, t0;                 // key head, part of the keys, sequence, its slot, the first tile's first token
+    int g, z, seq, t0;                       // key head, part of the keys, sequence, the first tile's first token
     int nq[2], pos0[2], lo[2], hi[2];        // per tile: tokens, first position, key blocks [lo, hi)
     int blk0, n, last_pos;                   // the item's key blocks, the last position any row sees
-    // items are ordered from a sequence's last tiles (most keys) to its first, heads next to each other; false: no such item
-    __device__ __forceinline__ bool set(const GfbBatch& b, int w, int n_x, int G, int splits, int TQ, int window) {
-        const int xz = w / G, xi = xz / splits;
-        g = w - xz * G;
-        z = xz - xi * splits;
-        int left = n_x - 1 - xi, at = 0, qlen = 0;
-        for (seq = 0; seq < b.n_seqs; seq++) {
-            at = b.cu_seqlens[seq];
-            qlen = b.cu_seqlens[seq + 1] - at;
-            const int nt = (qlen + 2 * TQ - 1) / (2 * TQ);
-            if (left < nt) break;
-            left -= nt;
-        }
-        if (seq == b.n_seqs) return false;
-        slot = b.slots[seq];
-        const int tq0 = left * 2 * TQ, len0 = b.lengths[slot];
-        t0 = at + tq0;
+    __device__ __forceinline__ void tiles(const TilePair& p, int TQ, int window) {
+        seq = p.seq;
+        t0 = p.t0;
 #pragma unroll
         for (int x = 0; x < 2; x++) {
-            nq[x] = max(0, min(TQ, qlen - (tq0 + x * TQ)));
-            pos0[x] = len0 + tq0 + x * TQ;
+            nq[x] = max(0, min(TQ, p.left - x * TQ));
+            pos0[x] = p.pos + x * TQ;
             lo[x] = hi[x] = 0;
             if (nq[x] > 0) {
                 lo[x] = (window > 0 ? max(0, pos0[x] - window + 1) : 0) / KEYS;
                 hi[x] = (pos0[x] + nq[x] - 1) / KEYS + 1;
             }
         }
+    }
+    // Items are ordered by their pair: by weight, or, where there are too many to sort (n_listed < 0), from a sequence's last tiles to its first; heads next to each
+    // other.  false: no such item
+    __device__ __forceinline__ bool set(const GfbBatch& b, const TilePair* list, int n_listed, int w, int n_x, int G, int splits, int TQ, int window) {
+        const int xz = w / G, xi = xz / splits;
+        g = w - xz * G;
+        z = xz - xi * splits;
+        TilePair p;
+        if (n_listed >= 0) {
+            if (xi >= n_listed) return false;
+            p = list[xi];
+        } else {
+            int left = n_x - 1 - xi, at = 0, qlen = 0, k = 0;
+            for (; k < b.n_seqs; k++) {
+                at = b.cu_seqlens[k];
+                qlen = b.cu_seqlens[k + 1] - at;
+                const int nt = pairs_of(qlen, TQ);
+                if (left < nt) break;
+                left -= nt;
+            }
+            if (k == b.n_seqs) return false;
+            const int tq0 = left * 2 * TQ;
+            p = {k, at + tq0, b.lengths[b.slots[k]] + tq0, qlen - tq0};
+        }
+        tiles(p, TQ, window);
         last_pos = pos0[0] + nq[0] + nq[1] - 1;
         const int all = max(hi[0], hi[1]) - lo[0], per = (all + splits - 1) / splits;     // (the second tile's keys begin no earlier)
         blk0 = lo[0] + z * per;
@@ -982,28 +998,59 @@ struct PromptItem {
 // The items are sorted by weight, so blocks take them in a snake: P ascending, P descending, ...
 __device__ __forceinline__ int snake_item(int pass, int block, int P) { return pass * P + ((pass & 1) ? P - 1 - block : block); }
 
-// A row's query into the tile at `tile` (shared memory) as float16 times a power of two, zeros where there is none; one thread writes the dims [first, first + n),
-// and every thread of the row gets what S times a key's scale is worth, log2(e) in it.
-template <int D>
-__device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bfloat16* src, float scale_log2e, int first, int n) {
-    uint32_t top = 0;
-    if (src != nullptr) {
-#pragma unroll 4
-        for (int i = 0; i < D / 8; i++) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + 8 * i);
-            top = max(top, max(max(v.x & 0x7fffu, (v.x >> 16) & 0x7fffu), max(v.y & 0x7fffu, (v.y >> 16) & 0x7fffu)));
-            top = max(top, max(max(v.z & 0x7fffu, (v.z >> 16) & 0x7fffu), max(v.w & 0x7fffu, (v.w >> 16) & 0x7fffu)));
+// All threads of a block: the batch's pairs of tiles into `list`, those with most key blocks first (each is ranked by comparing it with all others, no more
+// than two per thread); `found`: room for as many, count: 0 ahead of a barrier, their number behind this.
+__device__ __forceinline__ void list_pairs(const GfbBatch& b, TilePair* list, TilePair* found, unsigned long long* keys, int* count, int TQ, int window) {
+    for (int k = threadIdx.x; k < b.n_seqs; k += blockDim.x) {
+        const int at = b.cu_seqlens[k], qlen = b.cu_seqlens[k + 1] - at, nt = pairs_of(qlen, TQ), pos = b.lengths[b.slots[k]];
+        const int first = nt > 0 ? atomicAdd(count, nt) : 0;             // any order: they are sorted by weight and token
+        for (int i = 0; i < nt && first + i < LISTED; i++) {
+            const int tq0 = i * 2 * TQ;
+            const TilePair p = {k, at + tq0, pos + tq0, qlen - tq0};
+            PromptItem it;
+            it.tiles(p, TQ, window);
+            found[first + i] = p;
+            keys[first + i] = (unsigned long long)(it.hi[0] - it.lo[0] + it.hi[1] - it.lo[1]) << 32 | (uint32_t)~p.t0;
         }
     }
+    __syncthreads();
+    const int n = min(*count, LISTED);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const unsigned long long mine = keys[i];
+        int rank = 0;
+        for (int k = 0; k < n; k++) rank += keys[k] > mine;
+        list[rank] = found[i];
+    }
+    __syncthreads();
+}
+
+// Half of a row's query (dims [half D / 2, ..)) into the tile at `tile` (shared memory) as float16 times a power of two, zeros where there is none.  Two threads share
+// a row, in warps that `meet`; both get what S times a key's scale is worth, log2(e) in it.
+template <int D, typename Meet>
+__device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bfloat16* src, float scale_log2e, int half, float* mine_at, const float* other_at, Meet meet) {
+    uint4 v[D / 16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+        v[i] = src != nullptr ? *reinterpret_cast<const uint4*>(src + half * (D / 2) + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+        top = max(top, max(max(v[i].x & 0x7fffu, (v[i].x >> 16) & 0x7fffu), max(v[i].y & 0x7fffu, (v[i].y >> 16) & 0x7fffu)));
+        top = max(top, max(max(v[i].z & 0x7fffu, (v[i].z >> 16) & 0x7fffu), max(v[i].w & 0x7fffu, (v[i].w >> 16) & 0x7fffu)));
+    }
+    *mine_at = __uint_as_float(top);                                     // (every thread of the pair reads it ahead of its next write: the scores in between wait for both)
+    meet();
+    top = max(top, __float_as_uint(*other_at));
     const int e = min(max((int)(top >> 7) - 127, -100), 100);
     const float lift = exp2f((float)(14 - e));
-#pragma unroll 2
-    for (int i = first / 8; i < (first + n) / 8; i++) {
-        const uint4 v = src != nullptr ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-        const float f0 = __uint_as_float(v.x << 16) * lift, f1 = __uint_as_float(v.x & 0xffff0000u) * lift;
-        const float f2 = __uint_as_float(v.y << 16) * lift, f3 = __uint_as_float(v.y & 0xffff0000u) * lift;
-        const float f4 = __uint_as_float(v.z << 16) * lift, f5 = __uint_as_float(v.z & 0xffff0000u) * lift;
-        const float f6 = __uint_as_float(v.w << 16) * lift, f7 = __uint_as_float(v.w & 0xffff0000u) * lift;
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) {
+        const int i = half * (D / 16) + k;
+        const float f0 = __uint_as_float(v[k].x << 16) * lift, f1 = __uint_as_float(v[k].x & 0xffff0000u) * lift;
+        const float f2 = __uint_as_float(v[k].y << 16) * lift, f3 = __uint_as_float(v[k].y & 0xffff0000u) * lift;
+        const float f4 = __uint_as_float(v[k].z << 16) * lift, f5 = __uint_as_float(v[k].z & 0xffff0000u) * lift;
+        const float f6 = __uint_as_float(v[k].w << 16) * lift, f7 = __uint_as_float(v[k].w & 0xffff0000u) * lift;
         *reinterpret_cast<uint4*>(tile + (i >> 3) * HALF_BYTES + r * 128 + (((i & 7) ^ (r & 7)) << 4)) =
             make_uint4(pack2_f16(f0, f2), pack2_f16(f1, f3), pack2_f16(f4, f6), pack2_f16(f5, f7));
     }
@@ -1040,7 +1087,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             mbar_init(smem_u32(&bars->v_empty[s]), 1);
         }
         for (int s = 0; s < SC_STAGES; s++) mbar_init(smem_u32(&bars->sc_full[s]), 4);
-        bars->gave_up = 0;
+        bars->gave_up = bars->n_listed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) {
@@ -1054,6 +1101,14 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     gfb_pdl_launch();
     gfb_pdl_wait();
 
+    const TilePair* list = reinterpret_cast<const TilePair*>(smem + S::LIST);
+    int n_listed = -1;
+    if (n_x <= LISTED) {                                                 // (the tiles' shared memory is free yet)
+        list_pairs(b, reinterpret_cast<TilePair*>(smem + S::LIST), reinterpret_cast<TilePair*>(smem), reinterpret_cast<unsigned long long*>(smem + LISTED * 16), &bars->n_listed, TQ, window);
+        n_listed = min(bars->n_listed, LISTED);
+        n_items = n_listed * splits * G;
+    }
+
     PromptItem it;
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         // ---- converters.  A unit is 32 keys of a block's K, or of its V; the block's eight units, K first, go round the warps.  A lane has 16 bytes of a row.
@@ -1064,8 +1119,9 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         int g0 = 0;                                                      // key blocks ahead of the item
         bool ok = true;
         for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
-            if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
-            const int* pt = kv.page_table + (size_t)it.slot * kv.max_pages;
+            if (!it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
+            const int slot = b.slots[it.seq];
+            const int* pt = kv.page_table + (size_t)slot * kv.max_pages;
             const int last_page = it.last_pos / PAGE, first_unit = CONV_UNITS * g0, end = first_unit + CONV_UNITS * it.n;
             int U = first_unit + (warp - SOFT_WARPS + CONV_WARPS - first_unit % CONV_WARPS) % CONV_WARPS;      // the warp's first unit of the item
             // the pages of a unit's block; -1: not needed or not there
@@ -1153,7 +1209,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                         refs[sc].inv_v_ref = __uint_as_float((uint32_t)(254 - ve) << 23);
                     }
                     refs[sc].missing[group] = mine_page < 0 && index <= last_page;
-                    if (mine_page < 0 && index <= last_page) gfb_report(status, GFB_ERR_PAGE_TABLE, it.slot, index);
+                    if (mine_page < 0 && index <= last_page) gfb_report(status, GFB_ERR_PAGE_TABLE, slot, index);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // the tensor cores read it
                 __syncwarp();
@@ -1173,7 +1229,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             int g0 = 0;                                                  // key blocks ahead of the item
             bool ok = true;
             for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
-                if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window) || it.n == 0) continue;
+                if (!it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window) || it.n == 0) continue;
                 for (int x = 0; x < 2 && ok; x++) ok = lane_waits(smem_u32(&bars->q_full[x]), n_item & 1u, gave_up, status, 403);
                 n_item++;
                 uint32_t mine[2] = {0, 0};                               // of this item
@@ -1248,14 +1304,14 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         uint32_t n_done = 0, n_item = 0;                                 // this tile's blocks and items with keys so far
         bool ok = true;
         for (int pass = 0; snake_item(pass, blockIdx.x, P) < n_items; pass++) {
-            if (!it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
+            if (!it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
             float unit = 0.f;
             if (it.n > 0) {
                 const int tq = r / rep;
                 const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
                 ok = ok && warp_waits(smem_u32(&bars->q_empty[x]), (n_item & 1u) ^ 1u, gave_up, status, 411);
                 n_item++;
-                unit = put_query<D>(smem + x * TILE, r, tq < it.nq[x] ? q + at * D : nullptr, scale_log2e, half * (D / 2), D / 2);
+                unit = put_query<D>(smem + x * TILE, r, tq < it.nq[x] ? q + at * D : nullptr, scale_log2e, half, mine_at, other_at, meet);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars->q_full[x]));
@@ -1357,7 +1413,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             if (some) ok = ok && warp_waits(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
             if (ok) {
                 tc_fence_after();
-                it.set(b, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window);
+                it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window);
                 const int tq = r / rep;
                 const bool row_ok = tq < it.nq[x];
                 const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
