@@ -136,9 +136,9 @@ quantize_rows_kernel(const T* x, int8_t* q, float* scale, int K, int pitch, int 
     if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
 }
 
-// Threads of a block for rows of n vectors: one vector each where rows are few and wait for one another's launches, as many as a thread holds otherwise.
+// Threads of a block for rows of n vectors: as many as there can be where rows are few and wait for one another's launches, as many vectors as a thread holds otherwise.
 inline int row_threads(int R, int n) {
-    const int each = R <= 296 && n <= 1024 ? 1 : ROW_VECTORS;
+    const int each = R <= 296 ? (n + 1023) / 1024 : ROW_VECTORS;
     const int t = ((n + each - 1) / each + 31) / 32 * 32;
     return t < 64 ? 64 : t > 1024 ? 1024 : t;
 }

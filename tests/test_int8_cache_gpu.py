@@ -267,6 +267,21 @@ def test_attention_of_prompts(cached, new, window, H, G, d):
     check(out, q, kv, batch, H, G, d, d ** -0.5, window)
 
 
+@pytest.mark.parametrize("n", [1000, 1100])
+def test_attention_of_a_thousand_short_prompts(n):
+    """More pairs of tiles than a block sorts, and as many as it does."""
+    g = torch.Generator().manual_seed(n)
+    cached, new = torch.randint(0, 150, (n,), generator=g).tolist(), torch.randint(1, 4, (n,), generator=g).tolist()
+    new[7] = 300
+    batch = make_batch(cached, new)
+    kv = make_cache(batch, cached, new, 2, 64, seed=3)
+    q = torch.randn((batch.n_tokens, 4, 64), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(BF16)
+    out = torch.empty(batch.n_tokens, 4 * 64, dtype=BF16, device="cuda")
+    ops.attention(q, kv, batch, out, 4, 2, 64, 0.125)
+    ops.check_status(batch.status)
+    check(out, q, kv, batch, 4, 2, 64, 0.125)
+
+
 @pytest.mark.parametrize("H,G,d,page", [(4, 2, 64, 64), (6, 2, 48, 16), (2, 2, 130, 64), (8, 2, 128, 64)])
 @pytest.mark.parametrize("cached,new,window", [([0], [1], 0), ([700, 40], [1, 1], 0), ([0, 130], [90, 33], 0), ([300], [20], 70)])
 def test_attention_in_32_bits(cached, new, window, H, G, d, page):
