@@ -2,7 +2,8 @@
 //
 // For a query q at position p, over the keys j it sees (j <= p, and p - j < window when there is one):
 //     s_j = scale ks_j (q . K_j),   w_j = exp(s_j - max s),   out = sum_j (w_j vs_j) V_j / sum_j w_j
-// with integers K_j, V_j and their scales ks_j, vs_j.  The scales stay out of the products: a key's joins its score, a value's its weight.
+// with integers K_j, V_j and their scales ks_j, vs_j.  For single tokens the scales stay out of the
+// products: a key's joins its score, a value's its weight.  For runs of tokens they are multiplied in ahead of the products, once per key (below).
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -98,7 +99,7 @@ attention_int8_generic_kernel(const T* q, T* out, Int8KV kv, GfbBatch b, int H, 
 // and O^T += V^T (w vs)^T (16 dims x 8 heads per chunk of 16 dims).  Two 8-bit integers become two float16 numbers in two operations (`pair`), exactly.  They
 // are taken as bytes 0, 2 and bytes 1, 3 of a word, so no byte is moved: the order of the dims within a product over 16 of them is free as long as q
 // has it too, and of V's transposed words the two halves are the rows of dims 2g and 2g + 1.  (As bfloat16 numbers they cost twice the integer
-// operations, and the pipe for those, 74 % busy, was the limit: two sequences of 100,000 tokens 96 us, NOW so.)
+// operations, and the pipe for those, 74 % busy, was the limit: two sequences of 100,000 tokens 96 us, 77 so.)
 // float16 has few exponents.  A query row comes times the power of two that takes its largest number to 2^14 .. 2^15: bfloat16 numbers down to 2^-32 of that
 // stay exact.  The weights times their value's scale, w vs, have a reference M of their own beside the scores' reference m: the
 // largest lies between 2^9 and 2^15, one 2^-26 of it keeps eleven bits.  Rounding them there is the only rounding ahead of the result's (a bfloat16 weight
@@ -517,7 +518,8 @@ attention_int8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
 // pairs, whatever the sequences' lengths are, which only the device knows: it adds them up for itself.  A pair that one block has whole is finished there; of the others every
 // block leaves its sums under the common reference in scratch, slot 2 c + 1 for a pair that it begins and does not end, slot 2 c for one that it does not
 // begin, and a second kernel merges a pair's blocks in ascending order.  The producer runs ahead across pairs, so the stream never stops between them.
-// (A block per (token, key head, equal slice) waits for the longest sequence: 64 of 501 to 8,190 tokens 168 us, EVEN so.)
+// (A block per (token, key head, equal slice) waits for the longest sequence: 64 of 501 to 8,190 tokens take 119 to 153 us, by the
+// number of slices, and 106 so, 5.5 TB/s.)
 constexpr int LEAST_UNITS = 4;               // pages that a block takes at least
 
 template <int D, int NS>
@@ -797,6 +799,12 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // kernel; M, the reference of weights with v_ref, follows their maximum in steps of 2^3 or more, and a weight below 2^-37 of the largest is lost.
 // A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
+//
+// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 407 us, 660 TFLOP/s, 41 % of the rate of a plain
+// product; 128 of the 148 SMs have work (two parts each), and there 128 keys of both tiles take about 6,100 cycles: a tile's softmax chain of 3,100 (two
+// fetches of the scores, 64 exponentials a thread, the weights back) next to its products of 2,000, which share shared memory's bandwidth with the
+// converters' stores.  Twelve packed prompts of 17 to 901 tokens with 32 key heads, 900 items of 1 to 8 blocks of keys, take 175 us: there an item's start and end
+// (its queries, the first block's conversion, its rows' output) weigh as much as its blocks.
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16

@@ -337,12 +337,12 @@ read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d
 
 }  // namespace
 
-GFB_API int gfb_quantize_rows(const void* x, int dt, void* q, float* scale, int R, int K, int pitch, int early, cudaStream_t stream) {
+GFB_API int gfb_quantize_rows(const void* x, int dt, void* q, float* scale, int R, int K, int pitch, cudaStream_t stream) {
     if (R <= 0) return 0;
     if (K <= 0 || pitch < K) return gfb_fail("gfb_quantize_rows: rows of %d numbers with a pitch of %d", K, pitch);
     cudaError_t e;
-    if (dt == GFB_BF16) e = quantize_rows_launch((const __nv_bfloat16*)x, (int8_t*)q, scale, R, K, pitch, early, stream);
-    else if (dt == GFB_F32) e = quantize_rows_launch((const float*)x, (int8_t*)q, scale, R, K, pitch, early, stream);
+    if (dt == GFB_BF16) e = quantize_rows_launch((const __nv_bfloat16*)x, (int8_t*)q, scale, R, K, pitch, 0, stream);
+    else if (dt == GFB_F32) e = quantize_rows_launch((const float*)x, (int8_t*)q, scale, R, K, pitch, 0, stream);
     else return gfb_fail("gfb_quantize_rows: unknown type %d", dt);
     return gfb_check(e, "gfb_quantize_rows");
 }

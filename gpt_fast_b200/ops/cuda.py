@@ -1382,7 +1382,7 @@ class CudaKernels:
         _need(x, name="rows")
         pitch = self._need_rows(out, R, K, "quantised rows", here)
         self._need_here(here, x)
-        self._call("quantize", "gfb_quantize_rows", x.data_ptr(), _dt(x), out.q.data_ptr(), out.scale.data_ptr(), R, K, pitch, 0, _stream())
+        self._call("quantize", "gfb_quantize_rows", x.data_ptr(), _dt(x), out.q.data_ptr(), out.scale.data_ptr(), R, K, pitch, _stream())
 
     def rmsnorm_int8(self, x, weight, eps, out, rows=None, pending=None):
         here = _device()
