@@ -549,7 +549,7 @@ constexpr int MOST_TOKENS = 4096;            // whose pages are counted where th
 struct Shares {
     long long U;
     int C;
-    __device__ __forceinline__ Shares(long long units, int blocks) : U(units), C((int)max(1ll, min((long long)blocks, units / LEAST_UNITS))) {}
+    __device__ __forceinline__ Shares(long long units, int blocks, int least = LEAST_UNITS) : U(units), C((int)max(1ll, min((long long)blocks, units / least))) {}
     __device__ __forceinline__ long long begin(int c) const { return (long long)c * U / C; }
     __device__ __forceinline__ int owner(long long u) const { return (int)(((u + 1) * C - 1) / U); }
 };
@@ -783,7 +783,7 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 
 // ---- runs of new tokens on tcgen05: head sizes 64 and 128, pages of 64 ----------------------------------------------------------------
 // A work item is two tiles of 128 rows, a row being (token, head of the group): 2 TQ consecutive tokens of one sequence and key head, TQ = 128 / (heads per
-// group), against the item's keys, or one of `splits` equal parts of them where items are few.  Blocks are persistent, one per SM.  Per 128 keys:
+// group), against all of its keys or a part of them (PromptPlan).  Blocks are persistent, one per SM.  Per 128 keys:
 //
 //   converters (7 warps)    K and V from the cache through registers into shared memory as float16, with the 128-byte swizzle the tensor cores read: integers
 //                           (`pair`) times their row's scale over a power of two that the 128 rows share, k_ref and v_ref
@@ -800,11 +800,11 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
 //
-// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 407 us, 660 TFLOP/s, 41 % of the rate of a plain
-// product; 128 of the 148 SMs have work (two parts each), and there 128 keys of both tiles take about 6,100 cycles: a tile's softmax chain of 3,100 (two
-// fetches of the scores, 64 exponentials a thread, the weights back) next to its products of 2,000, which share shared memory's bandwidth with the
-// converters' stores.  Twelve packed prompts of 17 to 901 tokens with 32 key heads, 900 items of 1 to 8 blocks of keys, take 175 us: there an item's start and end
-// (its queries, the first block's conversion, its rows' output) weigh as much as its blocks.
+// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 358 to 369 us, 740 to 760 TFLOP/s, 46 % of the rate of a plain product.
+// 128 keys of both tiles take about 6,100 cycles: a tile's softmax chain of 3,100 (two fetches of the scores, 64 exponentials a thread, the weights
+// back) next to its products of 2,000, which share shared memory's bandwidth with the converters' stores.  Twelve packed prompts of 17 to 901 tokens with 32 key
+// heads, 900 items of 1 to 8 blocks of keys, take 172 us: there an item's start and end (its queries, the first block's conversion, its rows' output) weigh as
+// much as its blocks.
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
@@ -835,7 +835,7 @@ template <int D>
 struct PromptSmem {
     static constexpr int TILE = (D / 64) * HALF_BYTES;
     static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, ROWS_AT = SC + SC_STAGES * (int)sizeof(Refs);
-    static constexpr int LIST = ROWS_AT + 2 * 2 * ROWS * 4, BARS = LIST + LISTED * 16;
+    static constexpr int LIST = ROWS_AT + 2 * 2 * ROWS * 4, BEFORE = LIST + LISTED * 16, BARS = BEFORE + (LISTED + 2) * 4;
     static constexpr int BYTES = 1024 + BARS + (int)sizeof(PromptBars);
 };
 
@@ -952,12 +952,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 struct alignas(16) TilePair { int seq, t0, pos, left; };
 __device__ __forceinline__ int pairs_of(int tokens, int TQ) { return (tokens + 2 * TQ - 1) / (2 * TQ); }
 
+// What a block's items are made of.  Few pairs (even): the key blocks of all (pair, key head), one after the other and ITEM_UNITS ahead of each for what an item costs besides,
+// are one row of units, of which each block has an equal share, [first, end) here; else whole (pair, key head)s in a snake.
+constexpr int ITEM_UNITS = 3;
+struct PromptPlan {
+    GfbBatch b;
+    const TilePair* list;                    // the pairs, those with most key blocks first
+    const int* before;                       // units ahead of each, and all
+    int n_listed, n_x, n_items, G, TQ, window, end;      // n_listed: -1 where there is no list
+    bool even;
+};
+// The items are sorted by weight, so blocks take them in a snake: P ascending, P descending, ...
+__device__ __forceinline__ int snake_item(int pass, int block, int P) { return pass * P + ((pass & 1) ? P - 1 - block : block); }
+
 // One work item; the same for every warp of a block.
 struct PromptItem {
-    int g, z, seq, t0;                       // key head, part of the keys, sequence, the first tile's first token
+    int g, seq, t0;                          // key head, sequence, the first tile's first token
     int nq[2], pos0[2], lo[2], hi[2];        // per tile: tokens, first position, key blocks [lo, hi)
     int blk0, n, last_pos;                   // the item's key blocks, the last position any row sees
-    __device__ __forceinline__ void tiles(const TilePair& p, int TQ, int window) {
+    int units, to_end;                       // how far the next item is, and the next (pair, key head)
+    int part;                                // -1: all of the rows' keys; else where their sums under a reference of their own go
+    __device__ __forceinline__ int tiles(const TilePair& p, int TQ, int window) {
         seq = p.seq;
         t0 = p.t0;
 #pragma unroll
@@ -970,45 +985,61 @@ struct PromptItem {
                 hi[x] = (pos0[x] + nq[x] - 1) / KEYS + 1;
             }
         }
+        last_pos = pos0[0] + nq[0] + nq[1] - 1;
+        return max(hi[0], hi[1]) - lo[0];                                // (the second tile's keys begin no earlier)
     }
-    // Items are ordered by their pair: by weight, or, where there are too many to sort (n_listed < 0), from a sequence's last tiles to its first; heads next to each
-    // other.  false: no such item
-    __device__ __forceinline__ bool set(const GfbBatch& b, const TilePair* list, int n_listed, int w, int n_x, int G, int splits, int TQ, int window) {
-        const int xz = w / G, xi = xz / splits;
-        g = w - xz * G;
-        z = xz - xi * splits;
-        TilePair p;
-        if (n_listed >= 0) {
-            if (xi >= n_listed) return false;
-            p = list[xi];
-        } else {
-            int left = n_x - 1 - xi, at = 0, qlen = 0, k = 0;
-            for (; k < b.n_seqs; k++) {
-                at = b.cu_seqlens[k];
-                qlen = b.cu_seqlens[k + 1] - at;
-                const int nt = pairs_of(qlen, TQ);
+    // The block's item at `at`, a unit (even) or a pass; false: there is none left.  n == 0: none here.
+    __device__ __forceinline__ bool take(const PromptPlan& p, int at) {
+        if (p.even) {
+            if (at >= p.end) return false;
+            int i = 0;
+            for (int k = p.n_listed; k - i > 1;) {                       // the last pair that does not begin behind `at`
+                const int mid = (i + k) >> 1;
+                if (p.before[mid] <= at) i = mid;
+                else k = mid;
+            }
+            const int most = tiles(p.list[i], p.TQ, p.window), all = most + ITEM_UNITS, rest = at - p.before[i];
+            g = rest / all;
+            const int u = rest - g * all;
+            to_end = all - u;
+            units = min(to_end, p.end - at);
+            const int k0 = max(0, u - ITEM_UNITS), k1 = max(0, u + units - ITEM_UNITS);
+            n = k1 - k0;
+            blk0 = lo[0] + k0;
+            part = n == most ? -1 : 2 * (int)blockIdx.x + (k0 == 0);     // a block begins at most one item that it does not end, and ends at most one that it does not begin
+            return true;
+        }
+        const int w = snake_item(at, blockIdx.x, gridDim.x);
+        if (w >= p.n_items) return false;
+        const int xi = w / p.G;
+        g = w - xi * p.G;
+        part = -1;
+        units = 1;
+        if (p.n_listed >= 0) {
+            n = tiles(p.list[xi], p.TQ, p.window);
+        } else {                                                         // too many to sort: from a sequence's last tiles to its first
+            int left = p.n_x - 1 - xi, from = 0, qlen = 0, k = 0;
+            for (; k < p.b.n_seqs; k++) {
+                from = p.b.cu_seqlens[k];
+                qlen = p.b.cu_seqlens[k + 1] - from;
+                const int nt = pairs_of(qlen, p.TQ);
                 if (left < nt) break;
                 left -= nt;
             }
-            if (k == b.n_seqs) return false;
-            const int tq0 = left * 2 * TQ;
-            p = {k, at + tq0, b.lengths[b.slots[k]] + tq0, qlen - tq0};
+            const int tq0 = left * 2 * p.TQ;
+            n = 0;
+            if (k == p.b.n_seqs) return true;
+            n = tiles({k, from + tq0, p.b.lengths[p.b.slots[k]] + tq0, qlen - tq0}, p.TQ, p.window);
         }
-        tiles(p, TQ, window);
-        last_pos = pos0[0] + nq[0] + nq[1] - 1;
-        const int all = max(hi[0], hi[1]) - lo[0], per = (all + splits - 1) / splits;     // (the second tile's keys begin no earlier)
-        blk0 = lo[0] + z * per;
-        n = max(0, min(per, all - z * per));
+        blk0 = lo[0];
         return true;
     }
     __device__ __forceinline__ bool active(int x, int j) const { return blk0 + j >= lo[x] && blk0 + j < hi[x]; }
 };
-// The items are sorted by weight, so blocks take them in a snake: P ascending, P descending, ...
-__device__ __forceinline__ int snake_item(int pass, int block, int P) { return pass * P + ((pass & 1) ? P - 1 - block : block); }
 
 // All threads of a block: the batch's pairs of tiles into `list`, those with most key blocks first (each is ranked by comparing it with all others, no more
-// than two per thread); `found`: room for as many, count: 0 ahead of a barrier, their number behind this.
-__device__ __forceinline__ void list_pairs(const GfbBatch& b, TilePair* list, TilePair* found, unsigned long long* keys, int* count, int TQ, int window) {
+// than two per thread), and their units into `before`; `found`, `keys`: room for as many, count: 0 ahead of a barrier, their number behind this.
+__device__ __forceinline__ void list_pairs(const GfbBatch& b, TilePair* list, int* before, TilePair* found, ulonglong2* keys, int* count, int G, int TQ, int window) {
     for (int k = threadIdx.x; k < b.n_seqs; k += blockDim.x) {
         const int at = b.cu_seqlens[k], qlen = b.cu_seqlens[k + 1] - at, nt = pairs_of(qlen, TQ), pos = b.lengths[b.slots[k]];
         const int first = nt > 0 ? atomicAdd(count, nt) : 0;             // any order: they are sorted by weight and token
@@ -1016,19 +1047,28 @@ __device__ __forceinline__ void list_pairs(const GfbBatch& b, TilePair* list, Ti
             const int tq0 = i * 2 * TQ;
             const TilePair p = {k, at + tq0, pos + tq0, qlen - tq0};
             PromptItem it;
-            it.tiles(p, TQ, window);
+            const int n = it.tiles(p, TQ, window);
             found[first + i] = p;
-            keys[first + i] = (unsigned long long)(it.hi[0] - it.lo[0] + it.hi[1] - it.lo[1]) << 32 | (uint32_t)~p.t0;
+            keys[first + i] = make_ulonglong2((unsigned long long)(it.hi[0] - it.lo[0] + it.hi[1] - it.lo[1]) << 32 | (uint32_t)~p.t0, n + ITEM_UNITS);
         }
     }
     __syncthreads();
     const int n = min(*count, LISTED);
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const unsigned long long mine = keys[i];
-        int rank = 0;
-        for (int k = 0; k < n; k++) rank += keys[k] > mine;
+        const ulonglong2 mine = keys[i];
+        int rank = 0, ahead = 0;
+        for (int k = 0; k < n; k++) {
+            const ulonglong2 other = keys[k];
+            if (other.x > mine.x) {
+                rank++;
+                ahead += (int)other.y;
+            }
+        }
         list[rank] = found[i];
+        before[rank] = ahead * G;
+        if (rank == n - 1) before[n] = (ahead + (int)mine.y) * G;
     }
+    if (n == 0 && threadIdx.x == 0) before[0] = 0;
     __syncthreads();
 }
 
@@ -1065,11 +1105,14 @@ __device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bflo
     return exp2f((float)(e - 14)) * scale_log2e;
 }
 
-// q [T, H, D], out [T, H * D]; with splits > 1 instead scratch_o [T, H, splits, D] and scratch_ml [T, H, splits, 2] (M, l).
+// q [T, H, D], out [T, H * D].  scratch_o, not null: even shares; parts of rows go to scratch_o [2 gridDim.x][2][ROWS][D] and scratch_ml [..][2] (M, l), and
+// shared [gridDim.x] says what they are parts of.
+struct alignas(16) SharedRows { int t0, left, g, last; };        // the (pair, key head) that a block begins and others, up to `last`, go on with; last < 0: none
+constexpr int LEAST_BLOCKS = 4;              // units that a share has at least
 template <int D>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
-attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* scratch_o, float* scratch_ml, Int8KV kv, GfbBatch b, int H, int G, float scale_log2e,
-                             int window, int splits, int n_x, int n_items, int* status) {
+attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* scratch_o, float* scratch_ml, SharedRows* shared, Int8KV kv, GfbBatch b, int H, int G,
+                             float scale_log2e, int window, int n_x, int* status) {
     using S = PromptSmem<D>;
     constexpr int TILE = S::TILE;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -1079,7 +1122,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     PromptBars* bars = reinterpret_cast<PromptBars*>(smem + S::BARS);
     volatile int* gave_up = &bars->gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rep = H / G, TQ = ROWS / rep, P = gridDim.x;
+    const int rep = H / G, TQ = ROWS / rep;
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; x++) {
             mbar_init(smem_u32(&bars->q_full[x]), SOFT_WARPS / 2);
@@ -1109,15 +1152,21 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     gfb_pdl_launch();
     gfb_pdl_wait();
 
-    const TilePair* list = reinterpret_cast<const TilePair*>(smem + S::LIST);
-    int n_listed = -1;
+    PromptPlan plan = {b, reinterpret_cast<const TilePair*>(smem + S::LIST), reinterpret_cast<const int*>(smem + S::BEFORE), -1, n_x, n_x * G, G, TQ, window, 0, scratch_o != nullptr};
+    int first = 0;
     if (n_x <= LISTED) {                                                 // (the tiles' shared memory is free yet)
-        list_pairs(b, reinterpret_cast<TilePair*>(smem + S::LIST), reinterpret_cast<TilePair*>(smem), reinterpret_cast<unsigned long long*>(smem + LISTED * 16), &bars->n_listed, TQ, window);
-        n_listed = min(bars->n_listed, LISTED);
-        n_items = n_listed * splits * G;
+        list_pairs(b, reinterpret_cast<TilePair*>(smem + S::LIST), reinterpret_cast<int*>(smem + S::BEFORE), reinterpret_cast<TilePair*>(smem),
+                   reinterpret_cast<ulonglong2*>(smem + LISTED * 16), &bars->n_listed, G, TQ, window);
+        plan.n_listed = min(bars->n_listed, LISTED);
+        plan.n_items = plan.n_listed * G;
+        if (plan.even) {
+            const Shares shares(plan.before[plan.n_listed], gridDim.x, LEAST_BLOCKS);
+            first = (int)min(shares.begin(blockIdx.x), shares.U);
+            plan.end = (int)min(shares.begin(blockIdx.x + 1), shares.U);
+        }
     }
-
     PromptItem it;
+
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         // ---- converters.  A unit is 32 keys of a block's K, or of its V; the block's eight units, K first, go round the warps.  A lane has 16 bytes of a row.
         constexpr int CH = D / 16, RPI = 32 / CH, LOADS = 32 / RPI;      // 16-byte chunks of a row, rows per load of a warp, loads
@@ -1126,8 +1175,8 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         const int sub = CH == 8 ? ((lane >> 2) & 1) | ((lane >> 4) << 1) : lane >> 2, c = CH == 8 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3;
         int g0 = 0;                                                      // key blocks ahead of the item
         bool ok = true;
-        for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
-            if (!it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
+        for (int at = first; ok && it.take(plan, at); at += it.units) {
+            if (it.n == 0) continue;
             const int slot = b.slots[it.seq];
             const int* pt = kv.page_table + (size_t)slot * kv.max_pages;
             const int last_page = it.last_pos / PAGE, first_unit = CONV_UNITS * g0, end = first_unit + CONV_UNITS * it.n;
@@ -1236,8 +1285,10 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             uint32_t n_pv[2] = {0, 0}, n_item = 0;                       // products W V issued per tile, items with keys
             int g0 = 0;                                                  // key blocks ahead of the item
             bool ok = true;
-            for (int pass = 0; ok && snake_item(pass, blockIdx.x, P) < n_items; pass++) {
-                if (!it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window) || it.n == 0) continue;
+            SharedRows begun = {0, 0, 0, -1};
+            for (int at = first; ok && it.take(plan, at); at += it.units) {
+                if (it.n == 0) continue;
+                if (it.part >= 0 && (it.part & 1)) begun = {it.t0, it.nq[0] + it.nq[1], it.g, Shares(plan.before[plan.n_listed], gridDim.x, LEAST_BLOCKS).owner(at + it.to_end - 1)};
                 for (int x = 0; x < 2 && ok; x++) ok = lane_waits(smem_u32(&bars->q_full[x]), n_item & 1u, gave_up, status, 403);
                 n_item++;
                 uint32_t mine[2] = {0, 0};                               // of this item
@@ -1299,6 +1350,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 }
                 g0 += it.n;
             }
+            if (plan.even) shared[blockIdx.x] = begun;
         }
     } else {
         // ---- softmax.  A wait that runs out voids the results (the status says so); the warps go on to meet at the barriers of two.
@@ -1311,15 +1363,15 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         int g0 = 0;
         uint32_t n_done = 0, n_item = 0;                                 // this tile's blocks and items with keys so far
         bool ok = true;
-        for (int pass = 0; snake_item(pass, blockIdx.x, P) < n_items; pass++) {
-            if (!it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window)) continue;
-            float unit = 0.f;
-            if (it.n > 0) {
+        for (int at = first; it.take(plan, at); at += it.units) {
+            if (it.n == 0) continue;
+            float unit;
+            {
                 const int tq = r / rep;
-                const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
+                const size_t row = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
                 ok = ok && warp_waits(smem_u32(&bars->q_empty[x]), (n_item & 1u) ^ 1u, gave_up, status, 411);
                 n_item++;
-                unit = put_query<D>(smem + x * TILE, r, tq < it.nq[x] ? q + at * D : nullptr, scale_log2e, half, mine_at, other_at, meet);
+                unit = put_query<D>(smem + x * TILE, r, tq < it.nq[x] ? q + row * D : nullptr, scale_log2e, half, mine_at, other_at, meet);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars->q_full[x]));
@@ -1421,16 +1473,15 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             if (some) ok = ok && warp_waits(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 410);
             if (ok) {
                 tc_fence_after();
-                it.set(b, list, n_listed, snake_item(pass, blockIdx.x, P), n_x, G, splits, TQ, window);
+                it.take(plan, at);                                       // once more: it did not stay in registers
                 const int tq = r / rep;
                 const bool row_ok = tq < it.nq[x];
-                const size_t at = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep);
+                const size_t row = (size_t)(it.t0 + x * TQ + tq) * H + it.g * rep + (r - tq * rep), place = (size_t)(it.part * 2 + x) * ROWS + r;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                if (splits > 1 && row_ok && half == 0)
-                    *reinterpret_cast<float2*>(scratch_ml + (at * splits + it.z) * 2) = make_float2(some ? M : NONE, some ? l : 0.f);
+                if (it.part >= 0 && row_ok && half == 0) *reinterpret_cast<float2*>(scratch_ml + place * 2) = make_float2(some ? M : NONE, some ? l : 0.f);
 #pragma unroll 1
                 for (int c = 0; c < D / 64; c++) {
-                    if (!some && splits > 1) break;                      // nothing of this row in this part: its (M, l) say so
+                    if (!some && it.part >= 0) break;                    // nothing of this row in this part: its (M, l) say so
                     float o[32];
                     if (some) tmem_ld32(col_o + c * 32, o);
                     else {
@@ -1441,12 +1492,12 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                     const int dim = half * (D / 2) + c * 32;
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {                    // dims 0, 2, 1, 3 of every four
-                        if (splits > 1) {
-                            float* dst = scratch_o + (at * splits + it.z) * D + dim + i;
+                        if (it.part >= 0) {
+                            float* dst = scratch_o + place * D + dim + i;
                             *reinterpret_cast<float4*>(dst) = make_float4(o[i], o[i + 2], o[i + 1], o[i + 3]);
                             *reinterpret_cast<float4*>(dst + 4) = make_float4(o[i + 4], o[i + 6], o[i + 5], o[i + 7]);
                         } else {
-                            *reinterpret_cast<uint4*>(out + at * D + dim + i) =
+                            *reinterpret_cast<uint4*>(out + row * D + dim + i) =
                                 make_uint4(pack2(o[i] * inv, o[i + 2] * inv), pack2(o[i + 1] * inv, o[i + 3] * inv),
                                            pack2(o[i + 4] * inv, o[i + 6] * inv), pack2(o[i + 5] * inv, o[i + 7] * inv));
                         }
@@ -1470,28 +1521,42 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     }
 }
 
-// The parts of a row, merged in ascending order: a warp per (token, head).
+// The rows of the (pair, key head) that block x of the kernel ahead began and others went on with, merged over them in ascending order; y: eight rows of either tile.
+// A warp per row, four parts in flight.
 template <int D>
-__global__ void __launch_bounds__(128)
-attention_int8_parts_kernel(const float* scratch_o, const float* scratch_ml, __nv_bfloat16* out, long rows, int splits) {
+__global__ void __launch_bounds__(256)
+attention_int8_parts_kernel(const float* scratch_o, const float* scratch_ml, const SharedRows* shared, __nv_bfloat16* out, int H, int G) {
     constexpr int V = D / 32;
     gfb_pdl_launch();
     gfb_pdl_wait();
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
+    const SharedRows p = shared[blockIdx.x];
+    const int c0 = blockIdx.x, x = blockIdx.y >> 4, rep = H / G, TQ = ROWS / rep, lane = threadIdx.x & 31, r = (blockIdx.y & 15) * 8 + (threadIdx.x >> 5);
+    if (p.last < 0 || r >= max(0, min(TQ, p.left - x * TQ)) * rep) return;
     float top = NONE, sum = 0.f, o[V] = {};
-    for (int k = 0; k < splits; k++) {
-        const float2 ml = *reinterpret_cast<const float2*>(scratch_ml + (row * splits + k) * 2);
-        if (ml.x == NONE) continue;                                      // a part without a key of the row has written nothing
-        const float now = fmaxf(top, ml.x), down = power2(top - now), w = power2(ml.x - now);
-        const float* x = scratch_o + (row * splits + k) * D + lane * V;
-        top = now;
-        sum = sum * down + ml.y * w;
+    for (int c = c0; c <= p.last; c += 4) {
+        float2 ml[4];
+        float from[4][V];
 #pragma unroll
-        for (int v = 0; v < V; v++) o[v] = fmaf(x[v], w, o[v] * down);
+        for (int k = 0; k < 4; k++) {
+            const int cc = min(c + k, p.last);
+            const size_t place = (size_t)((2 * cc + (cc == c0)) * 2 + x) * ROWS + r;
+            ml[k] = *reinterpret_cast<const float2*>(scratch_ml + place * 2);
+#pragma unroll
+            for (int v = 0; v < V; v++) from[k][v] = scratch_o[place * D + lane * V + v];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (c + k > p.last || ml[k].x == NONE) continue;             // a part without a key of the row has written nothing
+            const float now = fmaxf(top, ml[k].x), down = power2(top - now), w = power2(ml[k].x - now);
+            top = now;
+            sum = sum * down + ml[k].y * w;
+#pragma unroll
+            for (int v = 0; v < V; v++) o[v] = fmaf(from[k][v], w, o[v] * down);
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int tq = r / rep;
+    const size_t row = (size_t)(p.t0 + x * TQ + tq) * H + p.g * rep + (r - tq * rep);
 #pragma unroll
     for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(out + row * D + lane * V + v) = pack2(o[v] * inv, o[v + 1] * inv);
 }
@@ -1587,24 +1652,22 @@ int launch_shares(const Decode& a, int blocks, float* scratch) {
 }
 
 template <int D>
-int launch_prompt(const Decode& a, int n_x, int splits, float* scratch) {
+int launch_prompt(const Decode& a, int n_x, int blocks, float* scratch) {
     auto kern = attention_int8_prompt_kernel<D>;
     const size_t smem = PromptSmem<D>::BYTES;
     static bool configured[MAX_DEVICES] = {};
     if (room(kern, smem, configured)) return 1;
-    int dev = 0, sms = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const long items = (long)n_x * a.G * splits;
+    const long items = (long)n_x * a.G;
     if (items > 0x3fffffffL) return gfb_fail("gfb_attention_int8_prompt: %ld work items", items);
-    const long rows = (long)a.b.n_tokens * a.H;
-    float* ml = scratch ? scratch + rows * splits * D : nullptr;
-    if (gfb_check(gfb_launch(kern, dim3((unsigned)(items < sms ? items : sms)), dim3(PROMPT_THREADS), smem, a.stream, (const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out,
-                             scratch, ml, a.kv, a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, splits, n_x, (int)items, a.status),
-                  "gfb_attention_int8_prompt")) return 1;
-    if (splits == 1) return 0;
-    return gfb_check(gfb_launch(attention_int8_parts_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, a.stream, (const float*)scratch, (const float*)ml,
-                                (__nv_bfloat16*)a.out, rows, splits), "gfb_attention_int8_prompt (parts)");
+    const size_t rows = (size_t)4 * blocks * ROWS;
+    float* ml = scratch ? scratch + rows * D : nullptr;
+    SharedRows* shared = scratch ? (SharedRows*)(ml + rows * 2) : nullptr;
+    const unsigned grid = scratch ? blocks : (unsigned)(items < blocks ? items : blocks);
+    if (gfb_check(gfb_launch(kern, dim3(grid), dim3(PROMPT_THREADS), smem, a.stream, (const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out,
+                             scratch, ml, shared, a.kv, a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, n_x, a.status), "gfb_attention_int8_prompt")) return 1;
+    if (scratch == nullptr) return 0;
+    return gfb_check(gfb_launch(attention_int8_parts_kernel<D>, dim3(blocks, 32), dim3(256), 0, a.stream, (const float*)scratch, (const float*)ml, (const SharedRows*)shared,
+                                (__nv_bfloat16*)a.out, a.H, a.G), "gfb_attention_int8_prompt (parts)");
 }
 
 }  // namespace
@@ -1628,22 +1691,22 @@ GFB_API int gfb_attention_int8_decode(const void* q, void* out, const void* k_po
 }
 
 // Any number of new tokens per sequence, bfloat16, d 64 or 128, pages of 64, at most 128 heads per key head, scale > 0.  n_x: at least the tile pairs there are,
-// sum over sequences of ceil(new tokens / (2 floor(128 / (H / G)))).  splits > 1: every pair's keys in that many parts, which merge through scratch (float32
-// [n_tokens * H * splits * (d + 2)]).
+// sum over sequences of ceil(new tokens / (2 floor(128 / (H / G)))).  blocks: one per SM.  With scratch (at most 1,024 pairs; float32 [512 blocks (d + 2) + 4 blocks]) every
+// block has an equal share of all pairs' keys, without it whole pairs.
 GFB_API int gfb_attention_int8_prompt(const void* q, void* out, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                                       const int* page_table, int max_pages, int page_size, int n_pages,
                                       const int* cu_seqlens, const int* tok_seq, const int* slots, const int* lengths, int n_seqs, int n_tokens,
-                                      int H, int G, int d, float scale, int window, int n_x, int splits, float* scratch, int* status, cudaStream_t stream) {
+                                      int H, int G, int d, float scale, int window, int n_x, int blocks, float* scratch, int* status, cudaStream_t stream) {
     if (n_tokens <= 0 || n_seqs <= 0) return 0;
     if ((d != 64 && d != 128) || page_size != PAGE) return gfb_fail("gfb_attention_int8_prompt: heads of %d, pages of %d", d, page_size);
     if (G <= 0 || H % G || H / G > ROWS) return gfb_fail("gfb_attention_int8_prompt: %d heads over %d", H, G);
     if (!(scale > 0.f)) return gfb_fail("gfb_attention_int8_prompt: a scale of %g (the maximum is taken of unscaled scores)", (double)scale);
-    if (splits < 1 || splits > 64 || (splits > 1 && scratch == nullptr) || n_x < 1) return gfb_fail("gfb_attention_int8_prompt: %d parts, %d pairs of tiles", splits, n_x);
+    if (blocks < 1 || n_x < 1 || (scratch && n_x > LISTED)) return gfb_fail("gfb_attention_int8_prompt: %d blocks, %d pairs of tiles", blocks, n_x);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch) & 15)
         return gfb_fail("gfb_attention_int8_prompt: everything must be 16-byte aligned");
     const Decode a{q, out, {(const int8_t*)k_pool, (const int8_t*)v_pool, k_scale, v_scale, page_table, max_pages, page_size, n_pages},
                    {cu_seqlens, tok_seq, slots, lengths, n_seqs, n_tokens}, H, G, scale, window, status, stream};
-    return d == 128 ? launch_prompt<128>(a, n_x, splits, splits > 1 ? scratch : nullptr) : launch_prompt<64>(a, n_x, splits, splits > 1 ? scratch : nullptr);
+    return d == 128 ? launch_prompt<128>(a, n_x, blocks, scratch) : launch_prompt<64>(a, n_x, blocks, scratch);
 }
 
 // q [T, H, d] and out [T, H * d] of type dt.  Any d up to 512, any page size.

@@ -192,18 +192,22 @@ def int8_shares(max_kv_len: int, page_size: int, pairs: int, sm_count: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def int8_parts(n_tokens: int, n_seqs: int, max_kv_len: int, rep: int, n_kv: int, sm_count: int):
-    """(pairs of tiles, parts of their keys) of a prompt's attention over a cache of 8-bit integers: how many pairs of tiles of 128 // rep tokens there are at
-    most, and into how many parts each pair's keys are cut.  A block per SM works on a part at a time, about 2 us per 128 keys and 4 such besides; the parts of
-    a row are 4 d bytes each, written and read again."""
+def int8_pairs(n_tokens: int, n_seqs: int, longest_new: int, max_kv_len: int, rep: int, n_kv: int, sm_count: int):
+    """(pairs of tiles, whether blocks share them evenly) of a prompt's attention over a cache of 8-bit integers: how many pairs of tiles of 128 // rep tokens
+    there are at most, and whether their keys are cut into equal shares, one per SM, whose rows a second kernel merges, or blocks take whole (pair, key head)s.
+
+    Shares pay where a cached context makes the items long and alike and a round of whole ones would leave SMs idle; an item costs three blocks of 128
+    keys (3.2 us each on a B200) besides its own, and a share's ends as much again.  The step knows bounds only: sequences whose lengths it cannot tell
+    apart count as the longest.  us whole | shared, 32 query and 8 key heads of 128: 512 tokens behind 32,001 813 | 358 to 369 (in two equal parts each
+    408), 8 x 64 behind 2,000 74 | 67, 4 of 100 to 700 behind 0 to 4,000 165 | 190, 2,048 behind none 80 | 123, 4,096 239 | 326."""
     two = 2 * (128 // rep)
     pairs = (n_tokens + n_seqs * (two - 1)) // two
-    blocks, best, best_cost = -(-max_kv_len // 128), 1, None
-    for s in range(1, max(1, min(16, blocks // 4)) + 1):
-        cost = -(-pairs * n_kv * s // sm_count) * (-(-blocks // s) + 4) * 2.0 + (4.0 + n_tokens * n_kv * rep * s * 2.5e-4 if s > 1 else 0.0)
-        if best_cost is None or cost < best_cost - 1e-9:
-            best, best_cost = s, cost
-    return pairs, best
+    alike = 4 * n_tokens >= 3 * n_seqs * longest_new
+    items = n_kv * (min(pairs, n_seqs * -(-longest_new // two)) if alike else pairs)
+    if pairs > 1024 or 2 * longest_new > max_kv_len or n_kv * pairs * max_kv_len >= 1 << 36:
+        return pairs, False
+    blocks, rounds = (max_kv_len - longest_new / 2) / 128, items / sm_count
+    return pairs, rounds * (blocks + 6) + 8 < (-(-items // sm_count) if alike else max(1.0, rounds)) * (blocks + 3)
 
 
 def rows_share_keys(rows: int, longest: int, max_kv_len: int, line: int, blocks: Optional[int] = None) -> bool:
@@ -1506,9 +1510,9 @@ class CudaKernels:
             if rep <= 128 and scale > 0:
                 if window:
                     reach = min(reach, window + 256)
-                pairs, splits = int8_parts(T, batch.n_seqs, reach, rep, n_kv, self.sm_count)
-                scratch = torch.empty(T * n_head * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-                return self._call("attention_int8", "gfb_attention_int8_prompt", q.data_ptr(), out.data_ptr(), *args, pairs, splits, _ptr(scratch),
+                pairs, even = int8_pairs(T, batch.n_seqs, batch.max_q_len, reach, rep, n_kv, self.sm_count)
+                scratch = torch.empty(self.sm_count * (512 * (head_dim + 2) + 4), dtype=torch.float32, device=q.device) if even else None
+                return self._call("attention_int8", "gfb_attention_int8_prompt", q.data_ptr(), out.data_ptr(), *args, pairs, self.sm_count, _ptr(scratch),
                                   batch.status.data_ptr(), _stream())
         self._call("attention_int8", "gfb_attention_int8_generic", q.data_ptr(), out.data_ptr(), _dt(q), *args, batch.status.data_ptr(), _stream())
 
