@@ -44,6 +44,7 @@ import torch
 
 from .. import ops
 from ..cache.needs import CacheNeeds, KVNeed, StateNeed
+from ..ops.types import Int8KV
 from ..weights.loader import ParamSpec
 from . import register_mixer
 from .residual import as_residual
@@ -219,8 +220,8 @@ class Attention:
         if not self.shared_kv and not append and self.conv_taps:
             raise ValueError("a run on another run's cache entry cannot advance a convolution over keys and values")
         qkv = torch.empty(T, self.wqkv.shape[0], dtype=self.dtype, device=h.device)
-        # a split sum is finished by the kernel that reads it; a convolution or a gate reads the finished rows
-        partials = ops.linear(h, self.wqkv, qkv, defer=not (self.conv_taps or self.gate))
+        # a split sum is finished by the kernel that reads it; a convolution, a gate or the kernel that quantises keys and values reads the finished rows
+        partials = ops.linear(h, self.wqkv, qkv, defer=not (self.conv_taps or self.gate or isinstance(view.kv, Int8KV)))
         y = torch.empty(T, H * dv, dtype=self.dtype, device=h.device)
         if self.plain:
             ops.rope_append_attention(qkv, partials, view.kv, batch, self.position.table, y, H, G, d, self.position.pairing,

@@ -99,6 +99,30 @@ def test_prompts_chunks_and_decode_steps(backend, folders, name, weights, cache)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("weights,cache", [(None, "int8"), ("int8", None), ("int8", "int8")])
+def test_products_that_are_split_over_their_sums(tmp_path, weights, cache):
+    """A layer as wide as an 8B model's: in bfloat16 the products of a few tokens leave partial sums, which the quantising append does not take."""
+    cfg = dict(BASE, hidden_size=4096, num_attention_heads=32, num_key_value_heads=8, intermediate_size=2048, num_hidden_layers=1)
+    folder = str(tmp_path / "wide")
+    gf.write_model_folder(folder, cfg, 5)
+    model = gf.load(folder, weight_dtype=weights, cache_dtype=cache)
+    p, c = plain_llama.load_folder(folder)
+    toks = torch.randint(0, c["vocab_size"], (12,), generator=torch.Generator().manual_seed(4)).tolist()
+    kv = model.new_cache(128, max_seqs=2)
+    st = Stepper(model, kv)
+    slot = kv.begin(1)
+    got = [st.step(slot, [toks[:9]], want="all").cpu()]
+    kv.reserve(slot[0], 64)
+    batch = st.decode_batch(slot)
+    for t in toks[9:]:
+        batch.tokens.fill_(t)
+        got.append(batch.run().cpu().clone())
+    st.check()
+    emu = plain_int8.forward(toks, p, c, act=torch.bfloat16, weights=bool(weights), cache=bool(cache))
+    judge(torch.cat(got), plain_int8.forward(toks, p, c, weights=False, cache=False), emu, "bfloat16", f"{weights} {cache}", weights)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["heads of 64", "heads of 128"])
 def test_generation_with_and_without_graphs_and_reading_the_cache(folders, name):
     model = gf.load(folders[name], weight_dtype="int8", cache_dtype="int8")
