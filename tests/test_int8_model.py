@@ -226,3 +226,18 @@ def test_a_norm_writes_8_bit_rows_of_a_stream_that_is_owed_something(owes, devic
     finally:
         if device == "cpu":
             ops.use_kernels(prev)
+
+
+@pytest.mark.gpu
+def test_the_command_line(folders, tmp_path):
+    from test_cli_gpu import read_lines, run_cli
+    out = tmp_path / "tokens.jsonl"
+    args = ["--checkpoint_path", folders["heads of 64"], "--prompt", "5,70", "--max_new_tokens", "9", "--temperature", "0", "--num_samples", "1", "--output", str(out)]
+    r = run_cli(*args, "--weight_dtype", "int8", "--cache_dtype", "int8")
+    assert r.returncode == 0, r.stderr[-2000:]
+    rows = read_lines(out)
+    model = gf.load(folders["heads of 64"], weight_dtype="int8", cache_dtype="int8")
+    seqs, _ = gf.generate(model, [x["prompt"] for x in rows], 9, temperature=0.0)
+    assert [x["prompt"] + x["tokens"] for x in rows] == seqs
+    r = run_cli("--random_weights", "--model_name", "dufizen-tiny-a", "--prompt", "5", "--weight_dtype", "int8")
+    assert r.returncode == 2 and "8-bit weights" in r.stderr
