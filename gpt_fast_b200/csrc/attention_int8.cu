@@ -6,6 +6,7 @@
 // products: a key's joins its score, a value's its weight.  For runs of tokens they are multiplied in ahead of the products, once per key (below).
 #include <cuda.h>
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "common.cuh"
 
@@ -1398,7 +1399,8 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 tc_fence_after();
                 const int gone = ref.missing[2 * half] | (ref.missing[2 * half + 1] << 1);       // 32 keys without a page: rare
                 const bool need_mask = j < plain0 || j >= plain1 || gone;
-                const float by = unit * ref.k_ref;
+                // (the smallest normal number at least: scores are 0 below it, but what is masked, at -infinity, has to stay there)
+                const float exact = unit * ref.k_ref, by = exact < FLT_MIN ? FLT_MIN : exact;
                 // 32 of the thread's scores, what the row does not see at -infinity.  They are fetched for the maximum and once more for the weights, since 64 of
                 // them do not stay in registers.
                 auto scores = [&](int c, uint32_t (&v)[32]) {

@@ -1,0 +1,86 @@
+"""Attention over the cache of 8-bit integers where queries, keys and values leave the ordinary: zeros, numbers that are not finite, sizes far apart."""
+import pytest
+import torch
+
+from gpt_fast_b200 import ops
+from gpt_fast_b200.ops.cuda import int8_pairs, int8_shares
+from test_int8_cache_gpu import BF16, check, make_batch, make_cache
+
+pytestmark = pytest.mark.gpu
+
+# cached and new tokens: single tokens in slices and in equal shares of all pages, prompts in whole items and in equal shares of all keys
+SLICES, SHARES = ([300, 70], [1, 1]), ([60000], [1])
+WHOLE, EVEN = ([200, 70], [90, 40]), ([5000], [70])
+WAYS = [SLICES, SHARES, WHOLE, EVEN]
+H, G = 8, 2
+
+
+def set_up(cached, new, d, seed=0):
+    batch = make_batch(cached, new)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    if batch.max_q_len > 1:
+        assert int8_pairs(batch.n_tokens, batch.n_seqs, batch.max_q_len, batch.max_kv_len, H // G, G, sms)[1] == (max(cached) >= 5000)
+    else:
+        assert bool(int8_shares(-(-batch.max_kv_len // 64) * 64, 64, batch.n_tokens * G, sms)[1]) == (max(cached) >= 60000)
+    kv = make_cache(batch, cached, new, G, d, seed=seed)
+    q = torch.randn((batch.n_tokens, H, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed + 5)).to(BF16)
+    return batch, kv, q
+
+
+def attend(q, kv, batch, d, window=None):
+    out = torch.full((batch.n_tokens, H * d), 7.0, dtype=BF16, device="cuda")
+    ops.attention(q, kv, batch, out, H, G, d, d ** -0.5, window)
+    ops.check_status(batch.status)
+    return out
+
+
+def set_rows(kv, batch, seq, first, last, **fields):
+    """Positions first .. last - 1 of a sequence: k_pool=, k_scale=, ... to the given values."""
+    at = torch.arange(first, last, device="cuda")
+    page = kv.page_table[batch.slots[seq].long(), at // 64].long()
+    for name, value in fields.items():
+        getattr(kv, name)[page, :, at % 64] = value
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cached,new,window", [([0], [2], None), ([0], [300], None), ([100, 0], [50, 200], 30), (*WHOLE, None), (*EVEN, None), (*EVEN, 3000), (*SLICES, None), (*SHARES, None),
+                                               ([0, 0], [1, 1], None)])
+def test_zero_queries_over_zero_keys(cached, new, window, d):
+    """Scores of zero, seen or masked beside: the mean of the seen values."""
+    batch = make_batch(cached, new)
+    kv = make_cache(batch, cached, new, G, d)
+    kv.k_pool.zero_(), kv.k_scale.zero_()
+    q = torch.zeros(batch.n_tokens, H, d, dtype=BF16, device="cuda")
+    check(attend(q, kv, batch, d, window), q, kv, batch, H, G, d, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [None, 40])
+def test_a_prompt_that_begins_with_zeros(d, window):
+    """130 rows of zeros, more than a block of keys, ahead of ordinary ones; then zero queries over ordinary keys and the other way round."""
+    batch = make_batch([0, 0], [300, 200])
+    kv = make_cache(batch, [0, 0], [300, 200], G, d)
+    q = torch.randn(500, H, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(BF16)
+    keep = kv.k_pool.clone(), kv.k_scale.clone(), q.clone()
+    set_rows(kv, batch, 0, 0, 130, k_pool=0, k_scale=0.0, v_pool=0, v_scale=0.0)
+    q[:130] = 0
+    check(attend(q, kv, batch, d, window), q, kv, batch, H, G, d, d ** -0.5, window)
+    kv.k_pool.copy_(keep[0]), kv.k_scale.copy_(keep[1])
+    check(attend(q, kv, batch, d, window), q, kv, batch, H, G, d, d ** -0.5, window)
+    set_rows(kv, batch, 0, 0, 130, k_pool=0, k_scale=0.0)
+    check(attend(keep[2], kv, batch, d, window), keep[2], kv, batch, H, G, d, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("cached,new", [([60, 200], [10, 5]), ([5000], [70])])
+def test_zero_queries_and_a_missing_page(cached, new):
+    """Keys without a page are masked like those that a row does not see."""
+    d = 128
+    batch = make_batch(cached, new)
+    kv = make_cache(batch, cached, new, G, d)
+    kv.k_pool.zero_(), kv.k_scale.zero_(), kv.v_pool.fill_(50), kv.v_scale.fill_(0.5)
+    kv.page_table[batch.slots[0].long(), 1] = -1
+    out = torch.empty(batch.n_tokens, H * d, dtype=BF16, device="cuda")
+    ops.attention(torch.zeros(batch.n_tokens, H, d, dtype=BF16, device="cuda"), kv, batch, out, H, G, d, d ** -0.5)
+    with pytest.raises(ops.KernelError, match="no page"):
+        ops.check_status(batch.status)
+    assert (out == 25).all()                                  # the mean of what is there, every value being 25
