@@ -1548,7 +1548,7 @@ attention_int8_parts_kernel(const float* scratch_o, const float* scratch_ml, con
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (c + k > p.last || ml[k].x == NONE) continue;             // a part without a key of the row has written nothing
+            if (c + k > p.last || ml[k].y == 0.f) continue;              // a part without a key of the row has written nothing (NaN scores make a NaN sum, which stays)
             const float now = fmaxf(top, ml[k].x), down = power2(top - now), w = power2(ml[k].x - now);
             top = now;
             sum = sum * down + ml[k].y * w;

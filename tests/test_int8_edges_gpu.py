@@ -1,4 +1,6 @@
 """Attention over the cache of 8-bit integers where queries, keys and values leave the ordinary: zeros, numbers that are not finite, sizes far apart."""
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -84,3 +86,48 @@ def test_zero_queries_and_a_missing_page(cached, new):
     with pytest.raises(ops.KernelError, match="no page"):
         ops.check_status(batch.status)
     assert (out == 25).all()                                  # the mean of what is there, every value being 25
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cached,new", WAYS)
+def test_queries_that_are_nan(cached, new, d):
+    """A query with a NaN is NaN whichever way its keys are cut up, and no other query notices."""
+    batch, kv, q = set_up(cached, new, d)
+    clean = attend(q, kv, batch, d).view(-1, H, d)
+    row, whole = batch.n_tokens // 2, q.clone()
+    q[row, 3, 5] = float("nan")
+    out = attend(q, kv, batch, d).view(-1, H, d)
+    assert out[row, 3].isnan().all()
+    # The single-token kernels move the references of a key head's queries together, when one of them has to be moved: what is kept in float16 under another
+    # reference is rounded elsewhere.  So these four queries are held to the bounds of `check`, all others to their bits.
+    mates = out[row, :H // G].clone()
+    mates[3] = clean[row, 3]
+    out[row, :H // G] = clean[row, :H // G]
+    assert torch.equal(out, clean)
+    out[row, :H // G] = mates
+    check(out, whole, kv, batch, H, G, d, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("field", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("cached,new", WAYS)
+def test_many_rows_that_stand_for_nan(cached, new, field, d):
+    """Parts of the keys in which every row stands for NaN: whoever sees them is NaN, a window that passes them by is not."""
+    batch, kv, q = set_up(cached, new, d)
+    clean = replace(kv, **{field: getattr(kv, field).clone()})
+    for seq in range(len(new)):
+        set_rows(kv, batch, seq, 0, cached[seq] // 2, **{field: float("nan")})
+    assert attend(q, kv, batch, d).isnan().all()
+    window = min(c - c // 2 for c in cached)
+    check(attend(q, kv, batch, d, window), q, clean, batch, H, G, d, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_part_of_a_row_is_nan(d):
+    """All keys of some parts of the shared prompt stand for NaN, other parts are clean: the rows are NaN, wherever the parts are cut."""
+    batch, kv, q = set_up(*EVEN, d)
+    for first, n in ((0, 128), (0, 640), (640, 512), (1152, 1024), (2000, 900), (4224, 700)):       # whole shares of four blocks of keys among them
+        keep = kv.k_scale.clone()
+        set_rows(kv, batch, 0, first, first + n, k_scale=float("nan"))
+        assert attend(q, kv, batch, d).isnan().all()
+        kv.k_scale.copy_(keep)
