@@ -224,6 +224,12 @@ __device__ __forceinline__ float power2(float x) {
     return y;
 }
 
+// What a score of a query row, lifted by 2^(14 - e), is worth, log2(e) in it.  top: the bfloat16 pattern of its largest number; a row with an infinity or a NaN has no
+// softmax (infinite scores of one sign would pass for keys that are not seen): NaN, which reaches every score.
+__device__ __forceinline__ float unit_of(uint32_t top, int e, float scale_log2e) {
+    return top >= 0x7f80u ? __uint_as_float(0x7fc00000u) : exp2f((float)(e - 14)) * scale_log2e;
+}
+
 // What a warp keeps of a (token, key head) while it walks over pages: of every lane the heads 2 t4 and 2 t4 + 1 (e = 0, 1), dims 16 c + 2 g4 and + 1.
 template <int D>
 struct WarpRows {
@@ -261,7 +267,7 @@ struct WarpRows {
             qb[c][0] = pack2_f16(f0, f2);
             qb[c][1] = pack2_f16(f1, f3);
         }
-        const float mine = exp2f((float)(e - 14)) * scale_log2e;
+        const float mine = unit_of(top, e, scale_log2e);
         unit[0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
         unit[1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
     }
@@ -1103,7 +1109,7 @@ __device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bflo
         *reinterpret_cast<uint4*>(tile + (i >> 3) * HALF_BYTES + r * 128 + (((i & 7) ^ (r & 7)) << 4)) =
             make_uint4(pack2_f16(f0, f2), pack2_f16(f1, f3), pack2_f16(f4, f6), pack2_f16(f5, f7));
     }
-    return exp2f((float)(e - 14)) * scale_log2e;
+    return unit_of(top, e, scale_log2e);
 }
 
 // q [T, H, D], out [T, H * D].  scratch_o, not null: even shares; parts of rows go to scratch_o [2 gridDim.x][2][ROWS][D] and scratch_ml [..][2] (M, l), and

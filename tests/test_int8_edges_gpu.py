@@ -89,13 +89,16 @@ def test_zero_queries_and_a_missing_page(cached, new):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
 @pytest.mark.parametrize("cached,new", WAYS)
-def test_queries_that_are_nan(cached, new, d):
-    """A query with a NaN is NaN whichever way its keys are cut up, and no other query notices."""
+def test_queries_that_are_not_finite(cached, new, what, d):
+    """A query with a NaN or an infinity is NaN whichever way its keys are cut up, and no other query notices.  One number of all keys has one sign, so that the
+    infinite scores are all +infinity or all -infinity."""
     batch, kv, q = set_up(cached, new, d)
+    kv.k_pool[..., 5] = kv.k_pool[..., 5].abs().clamp(min=1)
     clean = attend(q, kv, batch, d).view(-1, H, d)
     row, whole = batch.n_tokens // 2, q.clone()
-    q[row, 3, 5] = float("nan")
+    q[row, 3, 5] = float(what)
     out = attend(q, kv, batch, d).view(-1, H, d)
     assert out[row, 3].isnan().all()
     # The single-token kernels move the references of a key head's queries together, when one of them has to be moved: what is kept in float16 under another
