@@ -257,8 +257,8 @@ struct WarpRows {
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // exponent of the row's largest number (of zeros, tiny and huge ones as far as the factor stays within a float's exponents)
-        const int e = min(max((int)(top >> 7) - 127, -100), 100);
+        // exponent of the row's largest number (of zeros and tiny ones as far as the factor stays within a float's exponents)
+        const int e = max((int)(top >> 7) - 127, -100);
         const float lift = exp2f((float)(14 - e));
 #pragma unroll
         for (int c = 0; c < CH; c++) {
@@ -816,7 +816,8 @@ constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
 constexpr int SOFT_WARPS = 16, CONV_WARPS = 7, CONV_UNITS = 8, MMA_WARP = SOFT_WARPS + CONV_WARPS, PROMPT_THREADS = 32 * (MMA_WARP + 1);     // six warps per quarter of an SM: 80 registers each
-constexpr int LEAST_EXPONENT = 37, MOST_EXPONENT = 217;      // of k_ref and v_ref, in a float's bits: 2^-90 to 2^90, so that weights over v_ref stay finite
+// of k_ref and v_ref, in a float's bits: 2^-125 to 2^125, so that both they and their reciprocals are normal; and v_ref 2^-90 to 2^90, so that weights over it stay finite
+constexpr int LEAST_K_EXPONENT = 2, MOST_K_EXPONENT = 252, LEAST_EXPONENT = 37, MOST_EXPONENT = 217;
 
 struct PromptBars {
     unsigned long long q_full[2], q_empty[2];
@@ -1097,7 +1098,7 @@ __device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bflo
     *mine_at = __uint_as_float(top);                                     // (every thread of the pair reads it ahead of its next write: the scores in between wait for both)
     meet();
     top = max(top, __float_as_uint(*other_at));
-    const int e = min(max((int)(top >> 7) - 127, -100), 100);
+    const int e = max((int)(top >> 7) - 127, -100);
     const float lift = exp2f((float)(14 - e));
 #pragma unroll
     for (int k = 0; k < D / 16; k++) {
@@ -1242,7 +1243,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                         odd = here && (kb >= 0x7f800000u || vb >= 0x7f800000u);
                     }
                 }
-                const int ke = min(max((int)(warp_max_bits(kt) >> 23) + 1, LEAST_EXPONENT), MOST_EXPONENT);
+                const int ke = min(max((int)(warp_max_bits(kt) >> 23) + 1, LEAST_K_EXPONENT), MOST_K_EXPONENT);
                 const int ve = min(max((int)(warp_max_bits(vt) >> 23) + 1, LEAST_EXPONENT), MOST_EXPONENT);
                 const float over = mine * __uint_as_float((uint32_t)(254 - (is_v ? ve : ke)) << 23);
                 const __half hi = __float2half_rn(over), lo = __float2half_rn(over - __half2float(hi));
@@ -1405,8 +1406,8 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 tc_fence_after();
                 const int gone = ref.missing[2 * half] | (ref.missing[2 * half + 1] << 1);       // 32 keys without a page: rare
                 const bool need_mask = j < plain0 || j >= plain1 || gone;
-                // (the smallest normal number at least: scores are 0 below it, but what is masked, at -infinity, has to stay there)
-                const float exact = unit * ref.k_ref, by = exact < FLT_MIN ? FLT_MIN : exact;
+                // (the smallest normal number at least: scores are 0 below it, but what is masked, at -infinity, has to stay there; finite, for scores that are 0)
+                const float exact = unit * ref.k_ref, by = exact < FLT_MIN ? FLT_MIN : exact > FLT_MAX ? FLT_MAX : exact;
                 // 32 of the thread's scores, what the row does not see at -infinity.  They are fetched for the maximum and once more for the weights, since 64 of
                 // them do not stay in registers.
                 auto scores = [&](int c, uint32_t (&v)[32]) {

@@ -134,3 +134,15 @@ def test_one_part_of_a_row_is_nan(d):
         set_rows(kv, batch, 0, first, first + n, k_scale=float("nan"))
         assert attend(q, kv, batch, d).isnan().all()
         kv.k_scale.copy_(keep)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -60, 2.0 ** 60, 2.0 ** 102, 2.0 ** 112, 2.0 ** 120])
+@pytest.mark.parametrize("cached,new", WAYS)
+def test_queries_and_keys_of_any_size(cached, new, size):
+    """Queries of 2^-112 to 2^122 and keys as much smaller or larger, so that their products are ordinary."""
+    d = 128
+    batch, kv, q = set_up(cached, new, d)
+    kv.k_scale.mul_(1 / size)
+    q.mul_(size)
+    assert q.isfinite().all() and kv.k_scale.isfinite().all()
+    check(attend(q, kv, batch, d), q, kv, batch, H, G, d, d ** -0.5)
