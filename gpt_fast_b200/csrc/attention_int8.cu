@@ -803,7 +803,11 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // is rounded to float16, half a step being 2^-11 of it, an eighth of what a bfloat16 cache has.  (With the scales applied to scores and weights, exactly, the
 // softmax warps took 2.3 times the instructions, two thirds of their loads from shared memory among them, and the step 476 us.)  The scale itself
 // enters as two float16 numbers, so its own rounding does not add up over a row.  Queries are float16 times a power of two per row, as in the single-token
-// kernel; M, the reference of weights with v_ref, follows their maximum in steps of 2^3 or more, and a weight below 2^-37 of the largest is lost.
+// kernel; M, the reference of weights with v_ref, follows their maximum in steps of 2^3 or more, and a weight is off by half a step of its own and 2^-37 of the row's largest
+// (2^-25 where v_ref is as far above the values that the row sees as V_SPREAD allows).
+// float16 has five bits of exponent, so this holds while the scales of a block's keys are within 2^K_SPREAD of their largest and those of its values within 2^V_SPREAD, zeros
+// aside.  Beyond, one key would decide what is left of another for rows that do not see it.  A block of threads that met such
+// keys goes through its items once more with powers of two per key that the softmax warps multiply in, a word of shared memory for each (WIDE).
 // A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
 //
@@ -816,8 +820,11 @@ constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences
 constexpr int HALF_BYTES = 128 * 128;        // 128 rows x 64 float16
 constexpr int SOFT_WARPS = 16, CONV_WARPS = 7, CONV_UNITS = 8, MMA_WARP = SOFT_WARPS + CONV_WARPS, PROMPT_THREADS = 32 * (MMA_WARP + 1);     // six warps per quarter of an SM: 80 registers each
-// of k_ref and v_ref, in a float's bits: 2^-125 to 2^125, so that both they and their reciprocals are normal; and v_ref 2^-90 to 2^90, so that weights over it stay finite
-constexpr int LEAST_K_EXPONENT = 2, MOST_K_EXPONENT = 252, LEAST_EXPONENT = 37, MOST_EXPONENT = 217;
+// k_ref and v_ref are 2^ROOM below the power of two above the largest scale, so that the largest numbers are just within float16.  As exponents in a float's bits they are 2 to
+// 252, so that both they and their reciprocals are normal; v_ref 37 at least, so that weights over it stay finite.
+constexpr int ROOM = 8, LEAST_K_EXPONENT = 2, LEAST_V_EXPONENT = 37, MOST_EXPONENT = 252;
+constexpr int K_SPREAD = 18;                 // a scale over k_ref is 2^-11 at least: its integers are normal float16 numbers, and it keeps 14 bits itself
+constexpr int V_SPREAD = 12;                 // less, since M counts values as if they had the largest scale
 
 struct PromptBars {
     unsigned long long q_full[2], q_empty[2];
@@ -825,8 +832,14 @@ struct PromptBars {
     unsigned long long sc_full[SC_STAGES];
     unsigned long long s_full[2], p_ready[2], pv_done[2];
     uint32_t tmem_base;
-    int gave_up, n_listed;
+    int gave_up, n_listed, wide;             // wide: scales were met that are too far apart
 };
+// the reference's exponent for a largest scale, by its bits
+__device__ __forceinline__ int ref_exponent(uint32_t bits, int least) { return min(max((int)(bits >> 23) + 1 - ROOM, least), MOST_EXPONENT); }
+__device__ __forceinline__ float of_exponent(uint32_t e) { return __uint_as_float(e << 23); }
+// What a raw score is worth: the smallest normal number at least (scores are 0 below it, but what is masked, at -infinity, has to stay there), and finite (for
+// scores that are 0).
+__device__ __forceinline__ float worth(float x) { return x < FLT_MIN ? FLT_MIN : x > FLT_MAX ? FLT_MAX : x; }
 __device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 // two float16 numbers x times the number hi + lo
 __device__ __forceinline__ uint32_t times(uint32_t x, uint32_t hi, uint32_t lo) {
@@ -843,7 +856,7 @@ template <int D>
 struct PromptSmem {
     static constexpr int TILE = (D / 64) * HALF_BYTES;
     static constexpr int K = 2 * TILE, V = K + KV_STAGES * TILE, SC = V + KV_STAGES * TILE, ROWS_AT = SC + SC_STAGES * (int)sizeof(Refs);
-    static constexpr int LIST = ROWS_AT + 2 * 2 * ROWS * 4, BEFORE = LIST + LISTED * 16, BARS = BEFORE + (LISTED + 2) * 4;
+    static constexpr int WORDS = ROWS_AT + 2 * 2 * ROWS * 4, LIST = WORDS + SC_STAGES * KEYS * 4, BEFORE = LIST + LISTED * 16, BARS = BEFORE + (LISTED + 2) * 4;
     static constexpr int BYTES = 1024 + BARS + (int)sizeof(PromptBars);
 };
 
@@ -1117,62 +1130,47 @@ __device__ __forceinline__ float put_query(uint8_t* tile, int r, const __nv_bflo
 // shared [gridDim.x] says what they are parts of.
 struct alignas(16) SharedRows { int t0, left, g, last; };        // the (pair, key head) that a block begins and others, up to `last`, go on with; last < 0: none
 constexpr int LEAST_BLOCKS = 4;              // units that a share has at least
-template <int D>
-__global__ void __launch_bounds__(PROMPT_THREADS, 1)
-attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* scratch_o, float* scratch_ml, SharedRows* shared, Int8KV kv, GfbBatch b, int H, int G,
-                             float scale_log2e, int window, int n_x, int* status) {
+struct PromptArgs {
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    float *scratch_o, *scratch_ml;
+    SharedRows* shared;
+    Int8KV kv;
+    GfbBatch b;
+    int H, G;
+    float scale_log2e;
+    int window, n_x;
+    int* status;
+};
+// Where a warp's role is: key blocks ahead of the item, items with keys, its tile's blocks (softmax), products W V issued per tile (MMA).
+struct Progress {
+    int g0;
+    uint32_t n_item, n_done, n_pv[2];
+};
+
+// A block's items, each warp in its role.
+template <int D, bool WIDE>
+__device__ __forceinline__ void prompt_roles(const PromptArgs& p, const PromptPlan& plan, int first, Progress& done) {
     using S = PromptSmem<D>;
     constexpr int TILE = S::TILE;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
     Refs* refs = reinterpret_cast<Refs*>(smem + S::SC);
+    uint32_t* words = reinterpret_cast<uint32_t*>(smem + S::WORDS);      // WIDE, per key of a block: the exponent of its own k_ref, and 256 times that of its v_ref
     PromptBars* bars = reinterpret_cast<PromptBars*>(smem + S::BARS);
     volatile int* gave_up = &bars->gave_up;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rep = H / G, TQ = ROWS / rep;
-    if (threadIdx.x == 0) {
-        for (int x = 0; x < 2; x++) {
-            mbar_init(smem_u32(&bars->q_full[x]), SOFT_WARPS / 2);
-            mbar_init(smem_u32(&bars->q_empty[x]), 1);
-            mbar_init(smem_u32(&bars->s_full[x]), 1);
-            mbar_init(smem_u32(&bars->p_ready[x]), SOFT_WARPS / 2);
-            mbar_init(smem_u32(&bars->pv_done[x]), 1);
-        }
-        for (int s = 0; s < KV_STAGES; s++) {
-            mbar_init(smem_u32(&bars->k_full[s]), 4);
-            mbar_init(smem_u32(&bars->k_empty[s]), 1);
-            mbar_init(smem_u32(&bars->v_full[s]), 4);
-            mbar_init(smem_u32(&bars->v_empty[s]), 1);
-        }
-        for (int s = 0; s < SC_STAGES; s++) mbar_init(smem_u32(&bars->sc_full[s]), 4);
-        bars->gave_up = bars->n_listed = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == MMA_WARP) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    const __nv_bfloat16* q = p.q;
+    __nv_bfloat16* out = p.out;
+    float *scratch_o = p.scratch_o, *scratch_ml = p.scratch_ml;
+    const Int8KV& kv = p.kv;
+    const GfbBatch& b = p.b;
+    int* status = p.status;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = p.H, G = p.G, window = p.window, rep = H / G, TQ = ROWS / rep;
+    const float scale_log2e = p.scale_log2e;
     const uint32_t tmem = bars->tmem_base;
-    gfb_pdl_launch();
-    gfb_pdl_wait();
-
-    PromptPlan plan = {b, reinterpret_cast<const TilePair*>(smem + S::LIST), reinterpret_cast<const int*>(smem + S::BEFORE), -1, n_x, n_x * G, G, TQ, window, 0, scratch_o != nullptr};
-    int first = 0;
-    if (n_x <= LISTED) {                                                 // (the tiles' shared memory is free yet)
-        list_pairs(b, reinterpret_cast<TilePair*>(smem + S::LIST), reinterpret_cast<int*>(smem + S::BEFORE), reinterpret_cast<TilePair*>(smem),
-                   reinterpret_cast<ulonglong2*>(smem + LISTED * 16), &bars->n_listed, G, TQ, window);
-        plan.n_listed = min(bars->n_listed, LISTED);
-        plan.n_items = plan.n_listed * G;
-        if (plan.even) {
-            const Shares shares(plan.before[plan.n_listed], gridDim.x, LEAST_BLOCKS);
-            first = (int)min(shares.begin(blockIdx.x), shares.U);
-            plan.end = (int)min(shares.begin(blockIdx.x + 1), shares.U);
-        }
-    }
+    int& g0 = done.g0;
+    uint32_t &n_item = done.n_item, &n_done = done.n_done, (&n_pv)[2] = done.n_pv;
     PromptItem it;
 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
@@ -1181,7 +1179,6 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         // which row of a load's and which chunk: every eight lanes have four chunks of the same 64 dims of two neighbouring rows, whose 16-byte pieces meet
         // eight bank groups
         const int sub = CH == 8 ? ((lane >> 2) & 1) | ((lane >> 4) << 1) : lane >> 2, c = CH == 8 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3;
-        int g0 = 0;                                                      // key blocks ahead of the item
         bool ok = true;
         for (int at = first; ok && it.take(plan, at); at += it.units) {
             if (it.n == 0) continue;
@@ -1229,7 +1226,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 const bool is_v = U & 4;
                 // the powers of two above the largest finite scales of the block's keys, and this lane's key's scale over its own
                 const int key0 = (it.blk0 + gj - g0) * KEYS + lane;
-                uint32_t kt = 0, vt = 0;
+                uint32_t kt = 0, vt = 0, km = 0, vm = 0;                 // km, vm: the lane's key's (0: not there or not finite)
                 float mine = 0.f;
                 bool odd = false;                                        // a scale that is not finite
 #pragma unroll
@@ -1241,11 +1238,18 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                     if (i == group) {
                         mine = here ? (is_v ? vs[i] : ks[i]) : 0.f;
                         odd = here && (kb >= 0x7f800000u || vb >= 0x7f800000u);
+                        if (WIDE && here && !odd) {
+                            km = kb;
+                            vm = vb;
+                        }
                     }
                 }
-                const int ke = min(max((int)(warp_max_bits(kt) >> 23) + 1, LEAST_K_EXPONENT), MOST_K_EXPONENT);
-                const int ve = min(max((int)(warp_max_bits(vt) >> 23) + 1, LEAST_EXPONENT), MOST_EXPONENT);
-                const float over = mine * __uint_as_float((uint32_t)(254 - (is_v ? ve : ke)) << 23);
+                int ke = ref_exponent(warp_max_bits(kt), LEAST_K_EXPONENT), ve = ref_exponent(warp_max_bits(vt), LEAST_V_EXPONENT);
+                if constexpr (WIDE) {                                    // of the lane's own key
+                    ke = ref_exponent(km, LEAST_K_EXPONENT);
+                    ve = ref_exponent(vm, LEAST_V_EXPONENT);
+                } else if (mine != 0.f && __float_as_int(mine) < ((is_v ? ve - V_SPREAD : ke - K_SPREAD) + ROOM - 1) << 23) bars->wide = 1;
+                const float over = mine * of_exponent(254 - (is_v ? ve : ke));
                 const __half hi = __float2half_rn(over), lo = __float2half_rn(over - __half2float(hi));
                 uint32_t factor = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
                 if (odd) factor = is_v ? 0u : 0x7fff7fffu;
@@ -1266,12 +1270,13 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 }
                 fetch(U + CONV_WARPS, next, v);                          // in flight during what is left of this unit and the wait for the next one's place
                 fetch_scales(next, ks, vs);
+                if (WIDE && !is_v) words[sc * KEYS + group * 32 + lane] = (uint32_t)(ke | ve << 8);
                 if (!is_v && lane == 0) {
                     const int mine_page = (group & 2) ? page.y : page.x, index = (it.blk0 + gj - g0) * 2 + (group >> 1);
                     if (group == 0) {
-                        refs[sc].k_ref = __uint_as_float((uint32_t)ke << 23);
+                        refs[sc].k_ref = of_exponent(ke);
                         refs[sc].log_v_ref = (float)(ve - 127);
-                        refs[sc].inv_v_ref = __uint_as_float((uint32_t)(254 - ve) << 23);
+                        refs[sc].inv_v_ref = of_exponent(254 - ve);
                     }
                     refs[sc].missing[group] = mine_page < 0 && index <= last_page;
                     if (mine_page < 0 && index <= last_page) gfb_report(status, GFB_ERR_PAGE_TABLE, slot, index);
@@ -1290,8 +1295,6 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
     } else if (warp == MMA_WARP) {
         if (lane == 0) {
             constexpr uint32_t idesc_s = idesc_f16(ROWS, KEYS, 0), idesc_o = idesc_f16(ROWS, D, 1);
-            uint32_t n_pv[2] = {0, 0}, n_item = 0;                       // products W V issued per tile, items with keys
-            int g0 = 0;                                                  // key blocks ahead of the item
             bool ok = true;
             SharedRows begun = {0, 0, 0, -1};
             for (int at = first; ok && it.take(plan, at); at += it.units) {
@@ -1358,7 +1361,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 }
                 g0 += it.n;
             }
-            if (plan.even) shared[blockIdx.x] = begun;
+            if (plan.even) p.shared[blockIdx.x] = begun;
         }
     } else {
         // ---- softmax.  A wait that runs out voids the results (the status says so); the warps go on to meet at the barriers of two.
@@ -1368,8 +1371,6 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
         float* mine_at = reinterpret_cast<float*>(smem + S::ROWS_AT) + (x * 2 + half) * ROWS + r;
         const float* other_at = reinterpret_cast<const float*>(smem + S::ROWS_AT) + (x * 2 + (half ^ 1)) * ROWS + r;
         auto meet = [&]() { asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(1 + x * 4 + w4) : "memory"); };     // the two warps of 32 rows
-        int g0 = 0;
-        uint32_t n_done = 0, n_item = 0;                                 // this tile's blocks and items with keys so far
         bool ok = true;
         for (int at = first; it.take(plan, at); at += it.units) {
             if (it.n == 0) continue;
@@ -1406,8 +1407,7 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                 tc_fence_after();
                 const int gone = ref.missing[2 * half] | (ref.missing[2 * half + 1] << 1);       // 32 keys without a page: rare
                 const bool need_mask = j < plain0 || j >= plain1 || gone;
-                // (the smallest normal number at least: scores are 0 below it, but what is masked, at -infinity, has to stay there; finite, for scores that are 0)
-                const float exact = unit * ref.k_ref, by = exact < FLT_MIN ? FLT_MIN : exact > FLT_MAX ? FLT_MAX : exact;
+                const float by = worth(unit * ref.k_ref);
                 // 32 of the thread's scores, what the row does not see at -infinity.  They are fetched for the maximum and once more for the weights, since 64 of
                 // them do not stay in registers.
                 auto scores = [&](int c, uint32_t (&v)[32]) {
@@ -1420,40 +1420,74 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
                             if (i > t || i < f) v[i] = 0xff800000u;
                     }
                 };
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                const uint32_t* word = words + ((g0 + j) & (SC_STAGES - 1)) * KEYS + 64 * half;
+                float y;
+                if constexpr (WIDE) {
+                    y = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                    uint32_t v[32];
-                    scores(c, v);
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t v[32];
+                        scores(c, v);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        for (int i = 0; i < 32; i++) {
+                            const uint32_t w = word[32 * c + i];
+                            y = fmaxf(y, fmaf(__uint_as_float(v[i]), worth(unit * of_exponent(w & 255)), (float)((int)(w >> 8) - 127)));
+                        }
+                    }
+                } else {
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t v[32];
+                        scores(c, v);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                    }
+                    y = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), by, ref.log_v_ref);
                 }
-                float y = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), by, ref.log_v_ref);
                 *mine_at = y;
                 meet();
                 y = fmaxf(y, *other_at);
-                const float M_new = y > M + (15.f - LIFT) ? y : M, corr = power2(M - M_new), off = ref.log_v_ref + LIFT - M_new;
+                const float M_new = y > M + (15.f - LIFT) ? y : M, corr = power2(M - M_new), off = (WIDE ? 0.f : ref.log_v_ref) + LIFT - M_new;
                 M = M_new;
-                const uint64_t by2 = both(by, by), off2 = both(off, off);
-                uint64_t sums[2] = {0ull, 0ull};
+                if constexpr (WIDE) {
+                    l *= corr;
 #pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                    uint32_t v[32], pk[16];
-                    scores(c, v);
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t v[32], pk[16];
+                        scores(c, v);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float t0, t1;
-                        apart(fma2(both(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), by2, off2), t0, t1);
-                        const float w0 = power2(t0), w1 = power2(t1);
-                        sums[(i >> 1) & 1] = add2(sums[(i >> 1) & 1], both(w0, w1));
-                        pk[i >> 1] = pack2_f16(w0, w1);
+                        for (int i = 0; i < 32; i += 2) {
+                            const uint32_t wa = word[32 * c + i], wb = word[32 * c + i + 1];
+                            const float e0 = power2(fmaf(__uint_as_float(v[i]), worth(unit * of_exponent(wa & 255)), off));
+                            const float e1 = power2(fmaf(__uint_as_float(v[i + 1]), worth(unit * of_exponent(wb & 255)), off));
+                            l += e0 + e1;
+                            pk[i >> 1] = pack2_f16(e0 * of_exponent(wa >> 8), e1 * of_exponent(wb >> 8));
+                        }
+                        tmem_st16(col_s + c * 16, pk);
                     }
-                    tmem_st16(col_s + c * 16, pk);
+                } else {
+                    const uint64_t by2 = both(by, by), off2 = both(off, off);
+                    uint64_t sums[2] = {0ull, 0ull};
+#pragma unroll 1
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t v[32], pk[16];
+                        scores(c, v);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float t0, t1;
+                            apart(fma2(both(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), by2, off2), t0, t1);
+                            const float w0 = power2(t0), w1 = power2(t1);
+                            sums[(i >> 1) & 1] = add2(sums[(i >> 1) & 1], both(w0, w1));
+                            pk[i >> 1] = pack2_f16(w0, w1);
+                        }
+                        tmem_st16(col_s + c * 16, pk);
+                    }
+                    float s0, s1, s2, s3;
+                    apart(sums[0], s0, s1);
+                    apart(sums[1], s2, s3);
+                    l = fmaf(l, corr, ((s0 + s1) + (s2 + s3)) * ref.inv_v_ref);
                 }
-                float s0, s1, s2, s3;
-                apart(sums[0], s0, s1);
-                apart(sums[1], s2, s3);
-                l = fmaf(l, corr, ((s0 + s1) + (s2 + s3)) * ref.inv_v_ref);
                 // O follows the reference, rarely (S of this block was issued behind the tile's previous W V, so that phase is over)
                 if (was != (int)n_done && __any_sync(0xffffffffu, corr != 1.f)) {
                     ok = warp_waits(smem_u32(&bars->pv_done[x]), (n_done - 1u) & 1u, gave_up, status, 409);
@@ -1517,6 +1551,68 @@ attention_int8_prompt_kernel(const __nv_bfloat16* q, __nv_bfloat16* out, float* 
             g0 += item_n;
         }
     }
+}
+
+// The same once more for scales that are far apart: a function of its own, so that the common one keeps its registers.
+template <int D>
+__device__ __noinline__ void prompt_again(const PromptArgs& p, const PromptPlan plan, int first, Progress done) { prompt_roles<D, true>(p, plan, first, done); }
+
+template <int D>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+attention_int8_prompt_kernel(const __grid_constant__ PromptArgs p) {
+    using S = PromptSmem<D>;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+    PromptBars* bars = reinterpret_cast<PromptBars*>(smem + S::BARS);
+    volatile int* gave_up = &bars->gave_up;
+    const int warp = threadIdx.x >> 5, G = p.G, TQ = ROWS / (p.H / G);
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < 2; x++) {
+            mbar_init(smem_u32(&bars->q_full[x]), SOFT_WARPS / 2);
+            mbar_init(smem_u32(&bars->q_empty[x]), 1);
+            mbar_init(smem_u32(&bars->s_full[x]), 1);
+            mbar_init(smem_u32(&bars->p_ready[x]), SOFT_WARPS / 2);
+            mbar_init(smem_u32(&bars->pv_done[x]), 1);
+        }
+        for (int s = 0; s < KV_STAGES; s++) {
+            mbar_init(smem_u32(&bars->k_full[s]), 4);
+            mbar_init(smem_u32(&bars->k_empty[s]), 1);
+            mbar_init(smem_u32(&bars->v_full[s]), 4);
+            mbar_init(smem_u32(&bars->v_empty[s]), 1);
+        }
+        for (int s = 0; s < SC_STAGES; s++) mbar_init(smem_u32(&bars->sc_full[s]), 4);
+        bars->gave_up = bars->n_listed = bars->wide = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+    gfb_pdl_launch();
+    gfb_pdl_wait();
+
+    PromptPlan plan = {p.b, reinterpret_cast<const TilePair*>(smem + S::LIST), reinterpret_cast<const int*>(smem + S::BEFORE), -1, p.n_x, p.n_x * G, G, TQ, p.window, 0, p.scratch_o != nullptr};
+    int first = 0;
+    if (p.n_x <= LISTED) {                                                 // (the tiles' shared memory is free yet)
+        list_pairs(p.b, reinterpret_cast<TilePair*>(smem + S::LIST), reinterpret_cast<int*>(smem + S::BEFORE), reinterpret_cast<TilePair*>(smem),
+                   reinterpret_cast<ulonglong2*>(smem + LISTED * 16), &bars->n_listed, G, TQ, p.window);
+        plan.n_listed = min(bars->n_listed, LISTED);
+        plan.n_items = plan.n_listed * G;
+        if (plan.even) {
+            const Shares shares(plan.before[plan.n_listed], gridDim.x, LEAST_BLOCKS);
+            first = (int)min(shares.begin(blockIdx.x), shares.U);
+            plan.end = (int)min(shares.begin(blockIdx.x + 1), shares.U);
+        }
+    }
+    Progress done = {0, 0, 0, {0, 0}};
+    prompt_roles<D, false>(p, plan, first, done);
+    __syncthreads();
+    if (bars->wide && !*gave_up) prompt_again<D>(p, plan, first, done);
 
     tc_fence_before();
     __syncthreads();
@@ -1671,9 +1767,9 @@ int launch_prompt(const Decode& a, int n_x, int blocks, float* scratch) {
     const size_t rows = (size_t)4 * blocks * ROWS;
     float* ml = scratch ? scratch + rows * D : nullptr;
     SharedRows* shared = scratch ? (SharedRows*)(ml + rows * 2) : nullptr;
+    const PromptArgs args{(const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out, scratch, ml, shared, a.kv, a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, n_x, a.status};
     const unsigned grid = scratch ? blocks : (unsigned)(items < blocks ? items : blocks);
-    if (gfb_check(gfb_launch(kern, dim3(grid), dim3(PROMPT_THREADS), smem, a.stream, (const __nv_bfloat16*)a.q, (__nv_bfloat16*)a.out,
-                             scratch, ml, shared, a.kv, a.b, a.H, a.G, a.scale * 1.4426950408889634f, a.window, n_x, a.status), "gfb_attention_int8_prompt")) return 1;
+    if (gfb_check(gfb_launch(kern, dim3(grid), dim3(PROMPT_THREADS), smem, a.stream, args), "gfb_attention_int8_prompt")) return 1;
     if (scratch == nullptr) return 0;
     return gfb_check(gfb_launch(attention_int8_parts_kernel<D>, dim3(blocks, 32), dim3(256), 0, a.stream, (const float*)scratch, (const float*)ml, (const SharedRows*)shared,
                                 (__nv_bfloat16*)a.out, a.H, a.G), "gfb_attention_int8_prompt (parts)");

@@ -146,3 +146,45 @@ def test_queries_and_keys_of_any_size(cached, new, size):
     q.mul_(size)
     assert q.isfinite().all() and kv.k_scale.isfinite().all()
     check(attend(q, kv, batch, d), q, kv, batch, H, G, d, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("k,v", [(2.0 ** 4, 2.0 ** 4), (2.0 ** 12, 1.0), (2.0 ** 20, 1.0), (2.0 ** 40, 1.0), (2.0 ** 120, 1.0), (1.0, 2.0 ** 12), (1.0, 2.0 ** 20), (1.0, 2.0 ** 40), (1.0, 2.0 ** 95),
+                                 (1.0, 2.0 ** 120), (2.0 ** -40, 2.0 ** -40), (2.0 ** 60, 2.0 ** 60)])
+@pytest.mark.parametrize("cached,new", [([10, 0], [100, 300]), EVEN])
+def test_a_row_unlike_its_neighbours_reaches_who_sees_it(cached, new, k, v, d):
+    """Keys and values far larger (or smaller) than those beside them: queries ahead of them, and queries whose window is past them, have the result they have without."""
+    batch, kv, q = set_up(cached, new, d)
+    last, n = cached[0] + new[0] - 1, int(batch.cu_seqlens[1]) - 1
+    at = [last, cached[0] - 3] if cached[0] >= 5000 else [last]
+    clean = attend(q, kv, batch, d, 3)
+    for i in at:
+        page = kv.page_table[batch.slots[0].long(), i // 64].long()
+        kv.k_scale[page, :, i % 64] *= k
+        kv.v_scale[page, :, i % 64] *= v
+    out = attend(q, kv, batch, d, 3)
+    # rows 3 .. n - 1 of the first sequence see neither of them: exact sums aside, whose order is the same, the references of a block may differ by a power of two and
+    # a weight's float16 rounding with them, so these are held to the bounds of `check`
+    plain = replace(kv, k_scale=kv.k_scale.clone(), v_scale=kv.v_scale.clone())
+    for i in at:
+        page = kv.page_table[batch.slots[0].long(), i // 64].long()
+        plain.k_scale[page, :, i % 64] /= k
+        plain.v_scale[page, :, i % 64] /= v
+    out[:3], out[n] = clean[:3], clean[n]
+    check(out, q, plain, batch, H, G, d, d ** -0.5, 3)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("span", [2, 9, 14, 30, 80])
+@pytest.mark.parametrize("cached,new", WAYS)
+def test_scales_that_span_many_powers_of_two(cached, new, span, d):
+    """Keys and values whose scales lie anywhere in a range of 2^span, zeros among them, all seen and two at a time."""
+    batch, kv, q = set_up(cached, new, d)
+    g = torch.Generator(device="cuda").manual_seed(span)
+    for scale in (kv.k_scale, kv.v_scale):
+        scale.mul_(torch.exp2(torch.rand(scale.shape, generator=g, device="cuda") * span - span))
+        scale.masked_fill_(torch.rand(scale.shape, generator=g, device="cuda") < 0.05, 0.0)
+    kv.k_pool.masked_fill_(kv.k_scale[..., None] == 0, 0)
+    kv.v_pool.masked_fill_(kv.v_scale[..., None] == 0, 0)
+    check(attend(q, kv, batch, d), q, kv, batch, H, G, d, d ** -0.5)
+    check(attend(q, kv, batch, d, 2), q, kv, batch, H, G, d, d ** -0.5, 2)
