@@ -173,14 +173,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 // ---- what becomes of a sum ----------------------------------------------------------------------------------
-// The same expressions in both kernels: a row's bits do not depend on which of them made it.
+// The same expressions in both kernels, with every product rounded by itself where a sum follows (a compiler that may draw the two together does so in one place and not
+// in another): a row's bits do not depend on which of them made it.
 __device__ __forceinline__ float scaled(uint32_t sum, float row_scale) { return __fmul_rn(__int2float_rn((int)sum), row_scale); }
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 __device__ __forceinline__ float gated(float g, float u) { return silu(g) * u; }
 __device__ __forceinline__ float unary(int epi, float x) {
-    if (epi == EPI_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f));
+    if (epi == EPI_GELU) return 0.5f * x * __fadd_rn(1.0f, erff(x * 0.70710678118654752440f));
     if (epi == EPI_GELU_TANH)           // 0.5 x (1 + tanh(z)) = x / (1 + e^(-2z)), z = sqrt(2 / pi) (x + 0.044715 x^3)
-        return __fdividef(x, 1.0f + __expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+        return __fdividef(x, __fadd_rn(1.0f, __expf(-1.5957691216057308f * __fmaf_rn(0.044715f * x * x, x, x))));
     if (epi == EPI_SILU) return silu(x);
     if (epi == EPI_RELU2) { const float r = fmaxf(x, 0.f); return r * r; }
     return x;
@@ -356,7 +357,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 const float4 p = gfb_cluster_load4(tile + j * BM + 4 * lane, k);
                 v.x += __float_as_uint(p.x); v.y += __float_as_uint(p.y); v.z += __float_as_uint(p.z); v.w += __float_as_uint(p.w);
             }
-            const float e[4] = {scaled(v.x, sm) * ws[0], scaled(v.y, sm) * ws[1], scaled(v.z, sm) * ws[2], scaled(v.w, sm) * ws[3]};
+            const float e[4] = {__fmul_rn(scaled(v.x, sm), ws[0]), __fmul_rn(scaled(v.y, sm), ws[1]), __fmul_rn(scaled(v.z, sm), ws[2]), __fmul_rn(scaled(v.w, sm), ws[3])};
             finish4<KIND, TO>(out, e, (size_t)(col0 + j), n, N, ldo, vec && n + 3 < N, epi);
         }
     }
@@ -428,9 +429,9 @@ __device__ __forceinline__ void drain_chunk(float* stage, uint32_t taddr, int c0
         const int n = gc + lane;
         const float w = n < N ? w_scale[n] : 0.f, w1 = n + 1 < N ? w_scale[n + 1] : 0.f;
         for (int r = 0; r < rows; r++) {
-            const float y = stage[r * PSP + lane] * w;
+            const float y = __fmul_rn(stage[r * PSP + lane], w);
             if (KIND == KIND_SWIGLU) {
-                if (n < N && !(lane & 1)) put(out + (grow0 + r) * ldo + (n >> 1), gated(y, stage[r * PSP + lane + 1] * w1));
+                if (n < N && !(lane & 1)) put(out + (grow0 + r) * ldo + (n >> 1), gated(y, __fmul_rn(stage[r * PSP + lane + 1], w1)));
             } else if (n < N) {
                 TO* o = out + (grow0 + r) * ldo + n;
                 if (KIND == KIND_ADD) *(float*)o += y;
@@ -466,7 +467,7 @@ __device__ __forceinline__ void drain_chunk(float* stage, uint32_t taddr, int c0
 #pragma unroll
             for (int u = 0; u < COLS; u += 4) {
                 const float4 t = *reinterpret_cast<const float4*>(stage + r * PSP + col + u);
-                y[u] = t.x * w[u]; y[u + 1] = t.y * w[u + 1]; y[u + 2] = t.z * w[u + 2]; y[u + 3] = t.w * w[u + 3];
+                y[u] = __fmul_rn(t.x, w[u]); y[u + 1] = __fmul_rn(t.y, w[u + 1]); y[u + 2] = __fmul_rn(t.z, w[u + 2]); y[u + 3] = __fmul_rn(t.w, w[u + 3]);
             }
             TO* o = out + (grow0 + r) * ldo;
             if constexpr (KIND == KIND_SWIGLU) {
