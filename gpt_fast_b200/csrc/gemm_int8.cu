@@ -176,21 +176,27 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // The same expressions in both kernels, with every product rounded by itself where a sum follows (a compiler that may draw the two together does so in one place and not
 // in another): a row's bits do not depend on which of them made it.
 __device__ __forceinline__ float scaled(uint32_t sum, float row_scale) { return __fmul_rn(__int2float_rn((int)sum), row_scale); }
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
-__device__ __forceinline__ float gated(float g, float u) { return silu(g) * u; }
+// x / (1 + e^t), which SiLU (t = -x) and the tanh form of GELU are.  Outputs of 16 bits take the short exponential and quotient, off by up to 2 + 1.2 |t| steps of 32 bits, 2^-17 of
+// the result where it counts; 32-bit outputs take the full ones, off by a few.
+template <typename TO>
+__device__ __forceinline__ float over_one_plus_exp(float x, float t) {
+    return sizeof(TO) == 4 ? __fdiv_rn(x, __fadd_rn(1.f, expf(t))) : __fdividef(x, __fadd_rn(1.f, __expf(t)));
+}
+template <typename TO> __device__ __forceinline__ float gated(float g, float u) { return over_one_plus_exp<TO>(g, -g) * u; }
+template <typename TO>
 __device__ __forceinline__ float unary(int epi, float x) {
     if (epi == EPI_GELU) return 0.5f * x * __fadd_rn(1.0f, erff(x * 0.70710678118654752440f));
     if (epi == EPI_GELU_TANH)           // 0.5 x (1 + tanh(z)) = x / (1 + e^(-2z)), z = sqrt(2 / pi) (x + 0.044715 x^3)
-        return __fdividef(x, __fadd_rn(1.0f, __expf(-1.5957691216057308f * __fmaf_rn(0.044715f * x * x, x, x))));
-    if (epi == EPI_SILU) return silu(x);
+        return over_one_plus_exp<TO>(x, -1.5957691216057308f * __fmaf_rn(0.044715f * x * x, x, x));
+    if (epi == EPI_SILU) return over_one_plus_exp<TO>(x, -x);
     if (epi == EPI_RELU2) { const float r = fmaxf(x, 0.f); return r * r; }
     return x;
 }
 
 // kinds of epilogue that are kernels of their own; UNARY's function is an argument
 enum { KIND_STORE = 0, KIND_ADD = 1, KIND_SWIGLU = 2, KIND_UNARY = 3 };
-template <int KIND>
-__device__ __forceinline__ float fin(int epi, float x) { return KIND == KIND_UNARY ? unary(epi, x) : x; }
+template <int KIND, typename TO>
+__device__ __forceinline__ float fin(int epi, float x) { return KIND == KIND_UNARY ? unary<TO>(epi, x) : x; }
 
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -205,7 +211,7 @@ template <int KIND, typename TO>
 __device__ __forceinline__ void finish4(TO* out, const float (&e)[4], size_t m, int n, int N, int ldo, bool vec, int epi) {
     TO* row = out + m * ldo;
     if (KIND == KIND_SWIGLU) {
-        const float a = gated(e[0], e[1]), b = gated(e[2], e[3]);
+        const float a = gated<TO>(e[0], e[1]), b = gated<TO>(e[2], e[3]);
         if (vec) put2(row + (n >> 1), a, b);
         else {
             if (n < N) put(row + (n >> 1), a);
@@ -222,11 +228,11 @@ __device__ __forceinline__ void finish4(TO* out, const float (&e)[4], size_t m, 
                 if (n + u < N) ((float*)row)[n + u] += e[u];
         }
     } else {
-        if (vec) put4(row + n, fin<KIND>(epi, e[0]), fin<KIND>(epi, e[1]), fin<KIND>(epi, e[2]), fin<KIND>(epi, e[3]));
+        if (vec) put4(row + n, fin<KIND, TO>(epi, e[0]), fin<KIND, TO>(epi, e[1]), fin<KIND, TO>(epi, e[2]), fin<KIND, TO>(epi, e[3]));
         else {
 #pragma unroll
             for (int u = 0; u < 4; u++)
-                if (n + u < N) put(row + n + u, fin<KIND>(epi, e[u]));
+                if (n + u < N) put(row + n + u, fin<KIND, TO>(epi, e[u]));
         }
     }
 }
@@ -431,11 +437,11 @@ __device__ __forceinline__ void drain_chunk(float* stage, uint32_t taddr, int c0
         for (int r = 0; r < rows; r++) {
             const float y = __fmul_rn(stage[r * PSP + lane], w);
             if (KIND == KIND_SWIGLU) {
-                if (n < N && !(lane & 1)) put(out + (grow0 + r) * ldo + (n >> 1), gated(y, __fmul_rn(stage[r * PSP + lane + 1], w1)));
+                if (n < N && !(lane & 1)) put(out + (grow0 + r) * ldo + (n >> 1), gated<TO>(y, __fmul_rn(stage[r * PSP + lane + 1], w1)));
             } else if (n < N) {
                 TO* o = out + (grow0 + r) * ldo + n;
                 if (KIND == KIND_ADD) *(float*)o += y;
-                else put(o, fin<KIND>(epi, y));
+                else put(o, fin<KIND, TO>(epi, y));
             }
         }
         __syncwarp();
@@ -471,17 +477,17 @@ __device__ __forceinline__ void drain_chunk(float* stage, uint32_t taddr, int c0
             }
             TO* o = out + (grow0 + r) * ldo;
             if constexpr (KIND == KIND_SWIGLU) {
-                put4(o + ((gc + col) >> 1), gated(y[0], y[1]), gated(y[2], y[3]), gated(y[4], y[5]), gated(y[6], y[7]));
+                put4(o + ((gc + col) >> 1), gated<TO>(y[0], y[1]), gated<TO>(y[2], y[3]), gated<TO>(y[4], y[5]), gated<TO>(y[6], y[7]));
             } else if constexpr (KIND == KIND_ADD) {
                 float4 x = *reinterpret_cast<const float4*>((float*)o + gc + col);
                 x.x += y[0]; x.y += y[1]; x.z += y[2]; x.w += y[3];
                 *reinterpret_cast<float4*>((float*)o + gc + col) = x;
             } else if constexpr (WIDE) {
-                put4(o + gc + col, fin<KIND>(epi, y[0]), fin<KIND>(epi, y[1]), fin<KIND>(epi, y[2]), fin<KIND>(epi, y[3]));
+                put4(o + gc + col, fin<KIND, TO>(epi, y[0]), fin<KIND, TO>(epi, y[1]), fin<KIND, TO>(epi, y[2]), fin<KIND, TO>(epi, y[3]));
             } else {
                 uint4 pk;
-                pk.x = pack_bf16(fin<KIND>(epi, y[0]), fin<KIND>(epi, y[1])); pk.y = pack_bf16(fin<KIND>(epi, y[2]), fin<KIND>(epi, y[3]));
-                pk.z = pack_bf16(fin<KIND>(epi, y[4]), fin<KIND>(epi, y[5])); pk.w = pack_bf16(fin<KIND>(epi, y[6]), fin<KIND>(epi, y[7]));
+                pk.x = pack_bf16(fin<KIND, TO>(epi, y[0]), fin<KIND, TO>(epi, y[1])); pk.y = pack_bf16(fin<KIND, TO>(epi, y[2]), fin<KIND, TO>(epi, y[3]));
+                pk.z = pack_bf16(fin<KIND, TO>(epi, y[4]), fin<KIND, TO>(epi, y[5])); pk.w = pack_bf16(fin<KIND, TO>(epi, y[6]), fin<KIND, TO>(epi, y[7]));
                 *reinterpret_cast<uint4*>(o + gc + col) = pk;
             }
         }

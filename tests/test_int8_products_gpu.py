@@ -24,3 +24,30 @@ def test_a_rows_bits_depend_on_nothing_else(mode, dtype, N):
         part = base[:n].clone()
         ops.linear(x[:n].contiguous(), w, part, mode=mode)
         assert torch.equal(part, whole[:n]), n
+
+
+@pytest.mark.parametrize("M", [127, 700])
+@pytest.mark.parametrize("mode", ["swiglu", "silu", "gelu_tanh"])
+def test_32_bit_outputs_of_gates_have_32_bits(mode, M):
+    """Gates that are exact: one integer of either side, with powers of two for scales, i j 2^-6 for i up to 127 and j from -127 to 127; so the function's own error is
+    all there is, far below zero too."""
+    i, j = torch.arange(1, M + 1) % 127 + 1, torch.arange(-127, 128)
+    a = ops.Int8Rows(torch.zeros(M, 16, dtype=torch.int8), torch.ones(M), 16)
+    a.q[:, 3] = i.to(torch.int8)
+    rows = torch.stack([j, torch.full_like(j, 64)], 1).flatten() if mode == "swiglu" else j
+    w = ops.Int8Rows(torch.zeros(len(rows), 16, dtype=torch.int8), torch.full((len(rows),), 2.0 ** -6), 16)
+    w.q[:, 3] = rows.to(torch.int8)
+    a, w = (ops.Int8Rows(r.q.cuda(), r.scale.cuda(), 16) for r in (a, w))
+    out = torch.empty(M, len(j), device="cuda")
+    ops.linear(a, w, out, mode=mode)
+    x = (i[:, None] * j[None]).to(F64).cuda() / 64
+    up = i[:, None].to(F64).cuda() if mode == "swiglu" else 1.0
+    # the exponent t of x / (1 + e^t): exact for SiLU; for the tanh form of GELU four roundings of numbers no larger than itself, each 2^-24 of it
+    t = -x if mode != "gelu_tanh" else -2 * (2 / torch.pi) ** 0.5 * (x + 0.044715 * x ** 3)
+    want = x / (1 + torch.exp(t)) * up
+    # half steps: the exponential 2, the sum, the quotient and the product by `up` 1 each; the last step of 2^-24 is for their products.  Below t = 88.72 e^t leaves 32 bits and the
+    # result is 0, where |x| / e^t is less than 2^-121; results below 2^-126 have steps of 2^-149
+    rel = (6 + (4 * t.abs() if mode == "gelu_tanh" else 0)) * 2.0 ** -24
+    tol = want.abs() * rel + torch.as_tensor(up) * (2.0 ** -149 + torch.where(t > 88.72, x.abs() * 2.0 ** -127, 0.0))
+    bad = (out.to(F64) - want).abs() / tol.clamp(min=1e-60)
+    assert bool(bad.le(1).all()), float(bad.max())
