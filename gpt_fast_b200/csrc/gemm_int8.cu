@@ -189,7 +189,7 @@ __device__ __forceinline__ float unary(int epi, float x) {
     if (epi == EPI_GELU_TANH)           // 0.5 x (1 + tanh(z)) = x / (1 + e^(-2z)), z = sqrt(2 / pi) (x + 0.044715 x^3)
         return over_one_plus_exp<TO>(x, -1.5957691216057308f * __fmaf_rn(0.044715f * x * x, x, x));
     if (epi == EPI_SILU) return over_one_plus_exp<TO>(x, -x);
-    if (epi == EPI_RELU2) { const float r = fmaxf(x, 0.f); return r * r; }
+    if (epi == EPI_RELU2) { const float r = x < 0.f ? 0.f : x; return r * r; }      // (a maximum would make 0 of NaN)
     return x;
 }
 

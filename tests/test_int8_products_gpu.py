@@ -51,3 +51,22 @@ def test_32_bit_outputs_of_gates_have_32_bits(mode, M):
     tol = want.abs() * rel + torch.as_tensor(up) * (2.0 ** -149 + torch.where(t > 88.72, x.abs() * 2.0 ** -127, 0.0))
     bad = (out.to(F64) - want).abs() / tol.clamp(min=1e-60)
     assert bool(bad.le(1).all()), float(bad.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", [3, 40, 300])
+@pytest.mark.parametrize("mode", ["store", "add", "swiglu", "gelu", "gelu_tanh", "silu", "relu2"])
+def test_rows_that_stand_for_nan_stay_nan(mode, M, dtype):
+    """Through every function, in activations and in weights, and nowhere else."""
+    K, N = 256, 392
+    x, w = draw((M, K), 1, dtype, outliers=False), ops.quantize_rows(draw((N, K), 2, outliers=False) * K ** -0.5)
+    base = draw((M, N // 2 if mode == "swiglu" else N), 3).to(torch.float32 if mode == "add" else dtype)
+    clean, out = base.clone(), base.clone()
+    ops.linear(x, w, clean, mode=mode)
+    x[M - 2, 7] = float("nan")
+    w.scale[11] = float("nan")
+    ops.linear(x, w, out, mode=mode)
+    column = 5 if mode == "swiglu" else 11                   # row 11 of W is the up row of output 5
+    assert out[M - 2].isnan().all() and out[:, column].isnan().all()
+    out[M - 2], out[:, column] = clean[M - 2], clean[:, column]
+    assert torch.equal(out, clean)
