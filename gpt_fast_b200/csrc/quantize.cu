@@ -325,12 +325,16 @@ read_cache_int8_kernel(Int8KV kv, GfbBatch b, TO* k_out, TO* v_out, int G, int d
     for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
         const bool key = i < n;
         const int j = (key ? i : i - n) * VEC, g = j / d;
-        const size_t at = (size_t)(row < 0 ? 0 : row) + (size_t)g * kv.page_size;
-        const Few<int8_t, VEC> q = *reinterpret_cast<const Few<int8_t, VEC>*>((key ? kv.k_pool : kv.v_pool) + at * d + (j - g * d));
-        const float sc = (key ? kv.k_scale : kv.v_scale)[at];
+        const size_t at = (size_t)row + (size_t)g * kv.page_size;
+        Few<int8_t, VEC> q = {};
+        float sc = 0.f;
+        if (row >= 0) {                                     // (a pool can have no row at all)
+            q = *reinterpret_cast<const Few<int8_t, VEC>*>((key ? kv.k_pool : kv.v_pool) + at * d + (j - g * d));
+            sc = (key ? kv.k_scale : kv.v_scale)[at];
+        }
         Few<TO, VEC> o;
 #pragma unroll
-        for (int u = 0; u < VEC; u++) o.v[u] = gfb_from_f32<TO>(row < 0 ? 0.f : __fmul_rn((float)q.v[u], sc));
+        for (int u = 0; u < VEC; u++) o.v[u] = gfb_from_f32<TO>(__fmul_rn((float)q.v[u], sc));
         *reinterpret_cast<Few<TO, VEC>*>((key ? k_out : v_out) + (size_t)t * G * d + j) = o;
     }
 }

@@ -188,3 +188,26 @@ def test_scales_that_span_many_powers_of_two(cached, new, span, d):
     kv.v_pool.masked_fill_(kv.v_scale[..., None] == 0, 0)
     check(attend(q, kv, batch, d), q, kv, batch, H, G, d, d ** -0.5)
     check(attend(q, kv, batch, d, 2), q, kv, batch, H, G, d, d ** -0.5, 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("d", [128, 24, 20])
+def test_a_cache_without_pages(d, dtype):
+    """Nothing is written, zeros are read, and the status says so."""
+    batch = make_batch([3], [2])
+    pool, scale = torch.empty((0, G, 64, d), dtype=torch.int8, device="cuda"), torch.empty((0, G, 64), device="cuda")
+    kv = ops.Int8KV(pool, pool.clone(), torch.zeros((1, 1), dtype=torch.int32, device="cuda"), 64, k_scale=scale, v_scale=scale.clone())
+    qkv, q = torch.randn(2, (H + 2 * G) * d, device="cuda").to(dtype), torch.empty(2, H, d, dtype=dtype, device="cuda")
+    ops.rope_append(qkv, q, kv, batch, torch.ones(8, d // 2, 2, device="cuda"), H, G, d)
+    with pytest.raises(ops.KernelError, match="position beyond"):
+        ops.check_status(batch.status)
+    k, v = (torch.full((2, G, d), 3.0, dtype=dtype, device="cuda") for _ in range(2))
+    ops.read_cache(kv, batch, k, v)
+    with pytest.raises(ops.KernelError, match="position beyond"):
+        ops.check_status(batch.status)
+    assert (k == 0).all() and (v == 0).all() and (q == 0).all()
+    out = torch.full((2, H * d), 3.0, dtype=dtype, device="cuda")
+    ops.attention(q, kv, batch, out, H, G, d, d ** -0.5)
+    with pytest.raises(ops.KernelError, match="no page"):
+        ops.check_status(batch.status)
+    assert (out == 0).all()
