@@ -70,3 +70,25 @@ def test_rows_that_stand_for_nan_stay_nan(mode, M, dtype):
     assert out[M - 2].isnan().all() and out[:, column].isnan().all()
     out[M - 2], out[:, column] = clean[M - 2], clean[:, column]
     assert torch.equal(out, clean)
+
+
+def test_products_beyond_two_to_the_31_numbers():
+    """The last rows of 70,000 x 32,768 outputs have the bits they have by themselves; the same for rows and norms of as many numbers."""
+    M, K, N = 70000, 64, 32768
+    x, w = draw((M, K), 1, torch.bfloat16), ops.quantize_rows(draw((N, K), 2))
+    for mode, n in (("store", N), ("swiglu", N // 2)):
+        out, part = torch.empty(M, n, dtype=torch.bfloat16, device="cuda"), torch.empty(300, n, dtype=torch.bfloat16, device="cuda")
+        ops.linear(x, w, out, mode=mode)
+        ops.linear(x[-300:].contiguous(), w, part, mode=mode)
+        assert torch.equal(out[-300:], part)
+    out = torch.randn(M, N, dtype=torch.bfloat16, device="cuda")
+    whole, part = ops.quantize_rows(out), ops.quantize_rows(out[-300:].contiguous())
+    assert torch.equal(whole.q[-300:], part.q) and torch.equal(whole.scale[-300:], part.scale)
+    del whole
+    x32, weight = out.float(), torch.rand(N, device="cuda")
+    del out
+    whole, part = ops.int8_rows(M, N, "cuda"), ops.int8_rows(300, N, "cuda")
+    ops.rmsnorm(x32, weight, 1e-5, whole)
+    ops.rmsnorm(x32[-300:].contiguous(), weight, 1e-5, part)
+    # (few rows have more threads each, so the sum of squares has another order: scales within 2 (N / 2 + 4) steps, integers one apart next to a tie)
+    assert (whole.q[-300:].int() - part.q.int()).abs().max() <= 1 and (whole.scale[-300:] / part.scale - 1).abs().max() <= (N + 8) * 2.0 ** -24
