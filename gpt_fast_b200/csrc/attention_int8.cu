@@ -103,7 +103,7 @@ attention_int8_generic_kernel(const T* q, T* out, Int8KV kv, GfbBatch b, int H, 
 // operations, and the pipe for those, 74 % busy, was the limit: two sequences of 100,000 tokens 96 us, 77 so.)
 // float16 has few exponents.  A query row comes times the power of two that takes its largest number to 2^14 .. 2^15: bfloat16 numbers down to 2^-32 of that
 // stay exact.  The weights times their value's scale, w vs, have a reference M of their own beside the scores' reference m: the
-// largest lies between 2^9 and 2^15, one 2^-26 of it keeps eleven bits.  Rounding them there is the only rounding ahead of the result's (a bfloat16 weight
+// largest lies between 2^12 and 2^15, one 2^-26 of it keeps eleven bits.  Rounding them there is the only rounding ahead of the result's (a bfloat16 weight
 // would be eight times coarser).  The sum of weights is of the unrounded ones.  Both references follow their maximum in steps, so a rescale is rare.
 constexpr int DEC_WARPS = 4, DEC_THREADS = 32 * (DEC_WARPS + 1);
 constexpr int PAGE = 64;
@@ -807,14 +807,15 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // (2^-25 where v_ref is as far above the values that the row sees as V_SPREAD allows).
 // float16 has five bits of exponent, so this holds while the scales of a block's keys are within 2^K_SPREAD of their largest and those of its values within 2^V_SPREAD, zeros
 // aside.  Beyond, one key would decide what is left of another for rows that do not see it.  A block of threads that met such
-// keys goes through its items once more with powers of two per key that the softmax warps multiply in, a word of shared memory for each (WIDE).
+// keys goes through its items once more with powers of two per key that the softmax warps multiply in, a word of shared memory for each (WIDE): the 512 tokens behind
+// 32,001 then take 1.2 ms.
 // A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
 //
-// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 358 to 369 us, 740 to 760 TFLOP/s, 46 % of the rate of a plain product.
+// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 375 to 387 us, 700 to 720 TFLOP/s, 45 % of the rate of a plain product.
 // 128 keys of both tiles take about 6,100 cycles: a tile's softmax chain of 3,100 (two fetches of the scores, 64 exponentials a thread, the weights
 // back) next to its products of 2,000, which share shared memory's bandwidth with the converters' stores.  Twelve packed prompts of 17 to 901 tokens with 32 key
-// heads, 900 items of 1 to 8 blocks of keys, take 172 us: there an item's start and end (its queries, the first block's conversion, its rows' output) weigh as
+// heads, 900 items of 1 to 8 blocks of keys, take 173 us: there an item's start and end (its queries, the first block's conversion, its rows' output) weigh as
 // much as its blocks.
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences

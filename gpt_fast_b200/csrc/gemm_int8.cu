@@ -8,11 +8,11 @@
 // Both operands lie K-major, a byte per number, and arrive by TMA as tiles of 128 bytes of K with 128-byte swizzle (zeros beyond K and beyond the last row).
 //   few tokens   (gemm_int8_few_kernel): 128 weight rows are the rows of the MMA, the tokens, padded to 16, 32, 64 or 128, its columns.  A step streams every
 //                weight once; what bounds it is that stream.  The K axis is split over a cluster of up to 8 blocks, as far as all blocks are on the
-//                chip at once, and the blocks add up their integers through shared memory.  8 tokens, 28,672 x 4,096: 21.0 us, 5.6 TB/s; one token, 6,144 x
-//                4,096: 7.5 us, 3.3 TB/s, where the kernel's start and its merge weigh as much as the stream.
+//                chip at once, and the blocks add up their integers through shared memory.  8 tokens, 28,672 x 4,096: 21.4 us, 5.5 TB/s; one token, 6,144 x
+//                4,096: 7.4 us, 3.4 TB/s, where the kernel's start and its merge weigh as much as the stream.
 //   many tokens  (gemm_int8_pair_kernel): 256 x 256 tiles on pairs of SMs (cta_group::2), persistent, two accumulators in tensor memory, so that a tile's
-//                epilogue runs under the next one's products.  What bounds it is the tensor pipe, 91 % busy, and the power it takes: 8,192 tokens, 28,672 x
-//                4,096: 561 us, 3.4 POP/s, as a single launch.
+//                epilogue runs under the next one's products.  What bounds it is the tensor pipe, 90 % busy, and the power it takes: 8,192 tokens, 28,672 x
+//                4,096: 562 us, 3.4 POP/s, as a single launch.
 // Roles in a block of 192 threads: warp 0 = TMA producer (one lane), warp 1 = tensor-memory allocation and MMA issue (one lane), warps 2..5 = epilogue.
 // Waits on barriers are bounded by wall-clock time, as in gemm_tc.cu; those for the preceding kernel, for tensor memory and for the other blocks of a
 // cluster end for the reasons given there.

@@ -437,6 +437,9 @@ def linear(a, w, out, mode: str = "store", defer: bool = False):
     `pending`, `rope_append`'s `partials`, or `add_partials`).  Returns None when
     `out` is complete.
 
+    w is complete before the call ahead of this one: a kernel may fetch it while its predecessor runs, so what `rmsnorm` has just
+    written is an activation and no weight.
+
     w an `Int8Rows` [N, K]: a product of 8-bit integers with a scale per row of each side.  a is quantised per row on the way, or comes as an
     `Int8Rows` [M, K]; the sum over K (at most 133,144) is an exact 32-bit integer, scaled and passed through the mode's function in 32 bits;
     out is bfloat16 or float32 and always complete."""
@@ -502,7 +505,8 @@ def attention(q, kv: PagedKV, batch: BatchMeta, out, n_head: int, n_kv: int, hea
     a cached key row holds two keys; each (query, key) pair is a softmax of its own over the same values, and the head's
     output is (o_1 - lambda o_2) / sqrt(mean((o_1 - lambda o_2)^2) + eps) * out_scale.  q may come spread out
     ([T, H * 2, 2 d], see `spread_queries`).
-    kv an `Int8KV`: keys and values are integers times their row's scale; causal attention, with or without a window, is all it has."""
+    kv an `Int8KV`: keys and values are integers times their row's scale; causal attention, with or without a window, is all it has.  A query
+    that holds a NaN or an infinity, or sees a row whose scale is NaN, is NaN; no other query is."""
     if isinstance(kv, Int8KV):
         if (chunk is not None or sink is not None or v_head_dim not in (None, head_dim) or values_in_keys or bias is not None
                 or slopes is not None or softcap or keep_first or maps != 1 or diff is not None):

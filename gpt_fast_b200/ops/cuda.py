@@ -153,6 +153,9 @@ def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
     """(bn, splits, stages) of a product of 8-bit integers.  Few tokens: 128 weight rows x bn tokens per block, K split over a cluster of up to 8
     blocks; many tokens: 256 x 256 tiles on pairs of SMs (bn 256).  Between 129 and 512 tokens the
     first form, with several tiles of 128 tokens, while the second would leave most pairs without a tile; and for matrices of fewer than 256 rows.
+    us on a B200 in the first | second form: 6,144 x 4,096 stored, 256 tokens 16 | 21, 512 22 | 22, 640 22 | 22, 1,024 42 | 30; 4,096 x 4,096 stored, 400 tokens 16 | 21,
+    800 24 | 23, 1,300 42 | 31; SwiGLU of 28,672 x 4,096, 129 tokens 45 | 34, 512 102 | 55.  The second form's sums into the residual wait for it in their
+    epilogue and are behind for longer: 4,096 x 14,336, 512 tokens 36 | 82, 1,024 60 | 86, 2,048 128 | 135, 4,096 270 | 237.
 
     Two blocks share an SM, but clusters of them do not fill the chip: from 7/4 blocks per SM on some start when others have ended, and a product of
     one wave takes two (norm and product of one token, us on a B200, parts of K: 6,144 x 4,096 in 5 8.0, in 6 13.9; 5,120 x 5,120 in 6 8.2, in 7
@@ -198,8 +201,8 @@ def int8_pairs(n_tokens: int, n_seqs: int, longest_new: int, max_kv_len: int, re
 
     Shares pay where a cached context makes the items long and alike and a round of whole ones would leave SMs idle; an item costs three blocks of 128
     keys (3.2 us each on a B200) besides its own, and a share's ends as much again.  The step knows bounds only: sequences whose lengths it cannot tell
-    apart count as the longest.  us whole | shared, 32 query and 8 key heads of 128: 512 tokens behind 32,001 721 | 366 (in two equal parts each
-    408), 128 behind 32,001 720 | 126, 8 x 64 behind 2,000 70 | 67, 4 of 100 to 700 behind 0 to 4,000 160 | 190, 2,048 behind none 78 | 123, 4,096 229 | 326."""
+    apart count as the longest.  us whole | shared, 32 query and 8 key heads of 128: 512 tokens behind 32,001 728 | 375, 128 behind 32,001
+    726 | 127, 8 x 64 behind 2,000 72 | 69, 4 of 100 to 700 behind 0 to 4,000 163 | 191, 2,048 behind none 80 | 124, 4,096 232 | 328."""
     two = 2 * (128 // rep)
     pairs = (n_tokens + n_seqs * (two - 1)) // two
     alike = 4 * n_tokens >= 3 * n_seqs * longest_new
