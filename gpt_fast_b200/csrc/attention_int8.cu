@@ -812,10 +812,10 @@ attention_int8_merge_kernel(const float* scratch_o, const float* scratch_ml, con
 // A key whose key or value scale is not finite has NaN for K and zeros for V: rows that see it become NaN through their score, and no other row meets a NaN.
 // The order of four neighbouring dims is 0, 2, 1, 3 in Q, K and O, as `pair` leaves them; rows of Q are written so, rows of O read back so.
 //
-// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 375 to 387 us, 700 to 720 TFLOP/s, 45 % of the rate of a plain product.
+// What bounds it: 512 new tokens behind 32,001 cached ones, 32 query and 8 key heads of 128, take 361 to 371 us, 730 to 750 TFLOP/s, 46 % of the rate of a plain product.
 // 128 keys of both tiles take about 6,100 cycles: a tile's softmax chain of 3,100 (two fetches of the scores, 64 exponentials a thread, the weights
 // back) next to its products of 2,000, which share shared memory's bandwidth with the converters' stores.  Twelve packed prompts of 17 to 901 tokens with 32 key
-// heads, 900 items of 1 to 8 blocks of keys, take 173 us: there an item's start and end (its queries, the first block's conversion, its rows' output) weigh as
+// heads, 900 items of 1 to 8 blocks of keys, take 169 us: there an item's start and end (its queries, the first block's conversion, its rows' output) weigh as
 // much as its blocks.
 constexpr int ROWS = 128, KEYS = 128, KV_STAGES = 2, SC_STAGES = 4;
 constexpr int LISTED = 1024;                 // pairs of tiles that a block sorts by weight; more of them come in the order of the sequences
@@ -1151,7 +1151,7 @@ struct Progress {
 
 // A block's items, each warp in its role.
 template <int D, bool WIDE>
-__device__ __forceinline__ void prompt_roles(const PromptArgs& p, const PromptPlan& plan, int first, Progress& done) {
+__device__ __forceinline__ void prompt_roles(const PromptArgs& p, Progress& done) {
     using S = PromptSmem<D>;
     constexpr int TILE = S::TILE;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -1172,6 +1172,17 @@ __device__ __forceinline__ void prompt_roles(const PromptArgs& p, const PromptPl
     const uint32_t tmem = bars->tmem_base;
     int& g0 = done.g0;
     uint32_t &n_item = done.n_item, &n_done = done.n_done, (&n_pv)[2] = done.n_pv;
+    PromptPlan plan = {b, reinterpret_cast<const TilePair*>(smem + S::LIST), reinterpret_cast<const int*>(smem + S::BEFORE), -1, p.n_x, p.n_x * G, G, TQ, window, 0, scratch_o != nullptr};
+    int first = 0;
+    if (p.n_x <= LISTED) {
+        plan.n_listed = min(bars->n_listed, LISTED);
+        plan.n_items = plan.n_listed * G;
+        if (plan.even) {
+            const Shares shares(plan.before[plan.n_listed], gridDim.x, LEAST_BLOCKS);
+            first = (int)min(shares.begin(blockIdx.x), shares.U);
+            plan.end = (int)min(shares.begin(blockIdx.x + 1), shares.U);
+        }
+    }
     PromptItem it;
 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
@@ -1556,7 +1567,7 @@ __device__ __forceinline__ void prompt_roles(const PromptArgs& p, const PromptPl
 
 // The same once more for scales that are far apart: a function of its own, so that the common one keeps its registers.
 template <int D>
-__device__ __noinline__ void prompt_again(const PromptArgs& p, const PromptPlan plan, int first, Progress done) { prompt_roles<D, true>(p, plan, first, done); }
+__device__ __noinline__ void prompt_again(const PromptArgs& p, Progress done) { prompt_roles<D, true>(p, done); }
 
 template <int D>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
@@ -1567,7 +1578,7 @@ attention_int8_prompt_kernel(const __grid_constant__ PromptArgs p) {
     uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
     PromptBars* bars = reinterpret_cast<PromptBars*>(smem + S::BARS);
     volatile int* gave_up = &bars->gave_up;
-    const int warp = threadIdx.x >> 5, G = p.G, TQ = ROWS / (p.H / G);
+    const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; x++) {
             mbar_init(smem_u32(&bars->q_full[x]), SOFT_WARPS / 2);
@@ -1597,23 +1608,14 @@ attention_int8_prompt_kernel(const __grid_constant__ PromptArgs p) {
     gfb_pdl_launch();
     gfb_pdl_wait();
 
-    PromptPlan plan = {p.b, reinterpret_cast<const TilePair*>(smem + S::LIST), reinterpret_cast<const int*>(smem + S::BEFORE), -1, p.n_x, p.n_x * G, G, TQ, p.window, 0, p.scratch_o != nullptr};
-    int first = 0;
-    if (p.n_x <= LISTED) {                                                 // (the tiles' shared memory is free yet)
+    if (p.n_x <= LISTED)                                                 // (the tiles' shared memory is free yet)
         list_pairs(p.b, reinterpret_cast<TilePair*>(smem + S::LIST), reinterpret_cast<int*>(smem + S::BEFORE), reinterpret_cast<TilePair*>(smem),
-                   reinterpret_cast<ulonglong2*>(smem + LISTED * 16), &bars->n_listed, G, TQ, p.window);
-        plan.n_listed = min(bars->n_listed, LISTED);
-        plan.n_items = plan.n_listed * G;
-        if (plan.even) {
-            const Shares shares(plan.before[plan.n_listed], gridDim.x, LEAST_BLOCKS);
-            first = (int)min(shares.begin(blockIdx.x), shares.U);
-            plan.end = (int)min(shares.begin(blockIdx.x + 1), shares.U);
-        }
-    }
+                   reinterpret_cast<ulonglong2*>(smem + LISTED * 16), &bars->n_listed, p.G, ROWS / (p.H / p.G), p.window);
+
     Progress done = {0, 0, 0, {0, 0}};
-    prompt_roles<D, false>(p, plan, first, done);
+    prompt_roles<D, false>(p, done);
     __syncthreads();
-    if (bars->wide && !*gave_up) prompt_again<D>(p, plan, first, done);
+    if (bars->wide && !*gave_up) prompt_again<D>(p, done);
 
     tc_fence_before();
     __syncthreads();

@@ -201,8 +201,8 @@ def int8_pairs(n_tokens: int, n_seqs: int, longest_new: int, max_kv_len: int, re
 
     Shares pay where a cached context makes the items long and alike and a round of whole ones would leave SMs idle; an item costs three blocks of 128
     keys (3.2 us each on a B200) besides its own, and a share's ends as much again.  The step knows bounds only: sequences whose lengths it cannot tell
-    apart count as the longest.  us whole | shared, 32 query and 8 key heads of 128: 512 tokens behind 32,001 728 | 375, 128 behind 32,001
-    726 | 127, 8 x 64 behind 2,000 72 | 69, 4 of 100 to 700 behind 0 to 4,000 163 | 191, 2,048 behind none 80 | 124, 4,096 232 | 328."""
+    apart count as the longest.  us whole | shared, 32 query and 8 key heads of 128: 512 tokens behind 32,001 717 | 361, 128 behind 32,001
+    712 | 124, 8 x 64 behind 2,000 71 | 68, 4 of 100 to 700 behind 0 to 4,000 157 | 192, 2,048 behind none 79 | 122, 4,096 229 | 325."""
     two = 2 * (128 // rep)
     pairs = (n_tokens + n_seqs * (two - 1)) // two
     alike = 4 * n_tokens >= 3 * n_seqs * longest_new
