@@ -211,3 +211,45 @@ def test_a_cache_without_pages(d, dtype):
     with pytest.raises(ops.KernelError, match="no page"):
         ops.check_status(batch.status)
     assert (out == 0).all()
+
+
+MANY = [([i * 37 % 300 for i in range(40)], [30 + i % 5 for i in range(40)]), ([i * 7 % 150 for i in range(1100)], [1 + i % 3 for i in range(1100)]), ([32000, 5], [300, 40])]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cached,new", MANY)
+def test_scales_far_apart_in_many_items(cached, new, d):
+    """Blocks of threads that go through several items twice, among them such as have no scale of the kind; more pairs of tiles than are sorted; shares.  The same bits each time."""
+    batch = make_batch(cached, new)
+    kv = make_cache(batch, cached, new, G, d)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for scale in (kv.k_scale, kv.v_scale):
+        scale[torch.rand(scale.shape, generator=g, device="cuda") < 0.002] *= 2.0 ** -30
+    kv.v_scale[torch.rand(kv.v_scale.shape, generator=g, device="cuda") < 0.002] *= 2.0 ** 14
+    q = torch.randn((batch.n_tokens, H, d), generator=g, device="cuda").to(BF16)
+    out = attend(q, kv, batch, d)
+    check(out, q, kv, batch, H, G, d, d ** -0.5)
+    assert torch.equal(out, attend(q, kv, batch, d))
+
+
+@pytest.mark.parametrize("cached,new", [([200, 70], [90, 40]), ([5000], [70])])
+def test_scales_far_apart_beside_nan_and_missing_pages(cached, new):
+    d = 128
+    batch, kv, q = set_up(cached, new, d)
+    end = cached[0] + new[0]
+    set_rows(kv, batch, 0, 70, 71, v_scale=1e9, k_scale=1e-12)
+    set_rows(kv, batch, 0, end - 20, end - 19, k_scale=float("nan"))        # seen by the first sequence's last 20 queries
+    n = new[0] - 20
+    clean = replace(kv, k_scale=kv.k_scale.clone())
+    clean.k_scale[kv.page_table[batch.slots[0].long(), (end - 20) // 64].long(), :, (end - 20) % 64] = 0.01
+    out = attend(q, kv, batch, d)
+    assert out[n:new[0]].isnan().all()
+    sound = attend(q, clean, batch, d)
+    out[n:new[0]] = sound[n:new[0]]
+    check(out, q, clean, batch, H, G, d, d ** -0.5)
+    kv.page_table[batch.slots[0].long(), 0] = -1
+    out = torch.empty(batch.n_tokens, H * d, dtype=BF16, device="cuda")
+    ops.attention(q, kv, batch, out, H, G, d, d ** -0.5)
+    with pytest.raises(ops.KernelError, match="no page"):
+        ops.check_status(batch.status)
+    assert out[n:new[0]].isnan().all() and not out[:n].isnan().any()
