@@ -154,15 +154,18 @@ def int8_plan(M: int, N: int, K: int, mode: str, sm_count: int):
     blocks; many tokens: 256 x 256 tiles on pairs of SMs (bn 256).  Between 129 and 512 tokens the
     first form, with several tiles of 128 tokens, while the second would leave most pairs without a tile; and for matrices of fewer than 256 rows.
     us on a B200 in the first | second form: 6,144 x 4,096 stored, 256 tokens 16 | 21, 512 22 | 22, 640 22 | 22, 1,024 42 | 30; 4,096 x 4,096 stored, 400 tokens 16 | 21,
-    800 24 | 23, 1,300 42 | 31; SwiGLU of 28,672 x 4,096, 129 tokens 45 | 34, 512 102 | 55.  The second form's sums into the residual wait for it in their
-    epilogue and are behind for longer: 4,096 x 14,336, 512 tokens 36 | 82, 1,024 60 | 86, 2,048 128 | 135, 4,096 270 | 237.
+    800 24 | 23, 1,300 42 | 31; SwiGLU of 28,672 x 4,096, 129 tokens 45 | 34, 512 102 | 55.  Sums into the residual wait for it in the second form's
+    epilogue, which only a long K behind many tiles makes up for: 4,096 x 14,336, 1,000 tokens 60 | 85, 2,000 127 | 136, 2,500 196 | 177, 4,096 270 | 237;
+    8,192 x 28,672, 400 tokens 110 | 120, 600 197 | 181; 8,192 x 8,192, 2,000 tokens 195 | 220, 8,192 781 | 725; 12,288 x 4,096, 300 tokens 31 | 87; 4,096 x 4,096,
+    8,192 tokens 258 | 356.
 
     Two blocks share an SM, but clusters of them do not fill the chip: from 7/4 blocks per SM on some start when others have ended, and a product of
     one wave takes two (norm and product of one token, us on a B200, parts of K: 6,144 x 4,096 in 5 8.0, in 6 13.9; 5,120 x 5,120 in 6 8.2, in 7
     14.8).  So as many parts as stay below that, none shorter than 4 stages of 128 numbers (2 for up to 16 tokens, whose sums are joined
     faster: 2,048 x 2,048 in 4 6.1, in 8 5.6; with 64 tokens 7.4 and over 7.6)."""
     tiles = -(-M // 256) * -(-N // 256)
-    if M > 128 and N >= 256 and (M > 512 or mode == "swiglu" or tiles >= sm_count // 2):
+    many = K > 8192 and tiles * K >= 2_000_000 if mode == "add" else M > 512 or mode == "swiglu" or tiles >= sm_count // 2
+    if M > 128 and N >= 256 and many:
         return 256, 1, 6
     bn = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
     blocks = -(-N // 128) * -(-M // bn)
