@@ -180,7 +180,7 @@ __device__ __forceinline__ float scaled(uint32_t sum, float row_scale) { return 
 // the result where it counts; 32-bit outputs take the full ones, off by a few.
 template <typename TO>
 __device__ __forceinline__ float over_one_plus_exp(float x, float t) {
-    return sizeof(TO) == 4 ? __fdiv_rn(x, __fadd_rn(1.f, expf(t))) : __fdividef(x, __fadd_rn(1.f, __expf(t)));
+    return sizeof(TO) == 4 ? __fdiv_rn(x, __fadd_rn(1.f, expf(t))) : __fdividef(x, 1.f + __expf(t));
 }
 template <typename TO> __device__ __forceinline__ float gated(float g, float u) { return over_one_plus_exp<TO>(g, -g) * u; }
 template <typename TO>
